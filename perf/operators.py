@@ -10,8 +10,9 @@ Three kinds of pass:
           (mz_token_scores)
 
 A cache holds blocks of 32 positions x 64 channels per (slot, head): 8-bit codes and one scale for the keys' block, one
-for the values'. Code c stands for c * scale; scale = the block's largest magnitude / 127 (signed whole numbers, "i8")
-or / 448 (OCP e4m3). A block that is not full yet is held as it was given, in fp16, until its last position arrives.
+for the values'. Values are kept by pairs of channels and groups of eight positions. Code c stands for c * scale;
+scale = the block's largest magnitude / 127 (signed whole numbers, "i8") or / 448 (OCP e4m3). A block that is not full
+yet is held as it was given, in fp16 and in the same order, until its last position arrives.
 """
 import math
 
@@ -153,6 +154,13 @@ def _from_value_order(c):
     return c.movedim((-4, -3, -2, -1), (-2, -4, -1, -3)).flatten(-2, -1).flatten(-3, -2)
 
 
+def _natural(kv, name):
+    """Codes and open blocks of the keys or the values, positions by channels."""
+    if name == "k":
+        return kv["k"], kv["k_open"]
+    return _from_value_order(kv["v"]).contiguous(), _from_value_order(kv["v_open"]).contiguous()
+
+
 def _cache(case, g, slots, heads, held):
     """A cache whose slots hold `held` positions each; what lies behind them was left by earlier sequences."""
     fmt, blocks = case["format"], -(-case["max_t"] // BLK)
@@ -165,7 +173,8 @@ def _cache(case, g, slots, heads, held):
         c = _as_codes(c, fmt).reshape(slots, heads, blocks, BLK, HD)
         kv[name] = c if name == "k" else _value_order(c)
         kv[name + "_scale"] = s.contiguous()
-        kv[name + "_open"] = _randn(g, (slots, heads, BLK, HD), 0.7)
+        x = _randn(g, (slots, heads, BLK, HD), 0.7)
+        kv[name + "_open"] = x if name == "k" else _value_order(x)
     return kv
 
 
@@ -328,10 +337,9 @@ def _write(s):
         x = s[name] if case["layout"] == "tiles" else s[name].transpose(1, 2)
         src = (i[None] - off[:, None]).clamp(0, t - 1)
         new = torch.gather(x, 2, src[:, None, :, None].expand(n, h, blocks * BLK, HD))
-        c = kv[name][rows, :, b0]
-        c = _as_numbers(c if name == "k" else _from_value_order(c).contiguous(), fmt)
-        old = (c * kv[name + "_scale"][rows, :, b0][..., None, None]).half()
-        old = torch.where((kv["open"] == (b0 + 1)[:, None])[..., None, None], kv[name + "_open"], old)
+        c, o = _natural(kv, name)
+        old = (_as_numbers(c[rows, :, b0], fmt) * kv[name + "_scale"][rows, :, b0][..., None, None]).half()
+        old = torch.where((kv["open"] == (b0 + 1)[:, None])[..., None, None], o, old)
         old = torch.nn.functional.pad(old, (0, 0, 0, (blocks - 1) * BLK))
         x = torch.where((i[None] < off[:, None])[:, None, :, None], old, new).unflatten(2, (blocks, BLK))
         c, sc = _divided(x, fmt)
@@ -345,10 +353,10 @@ def _write(s):
 
 def _held(kv, name):
     """Every position of a cache in 32 bits: [slots, heads, positions, 64]."""
-    c = kv[name] if name == "k" else _from_value_order(kv[name]).contiguous()
+    c, o = _natural(kv, name)
     x = _as_numbers(c, kv["format"]) * kv[name + "_scale"][..., None, None]
     b = torch.arange(1, kv["blocks"] + 1, device="cuda", dtype=torch.int32)
-    x = torch.where((kv["open"][..., None] == b)[..., None, None], kv[name + "_open"].float()[:, :, None], x)
+    x = torch.where((kv["open"][..., None] == b)[..., None, None], o.float()[:, :, None], x)
     return x.flatten(2, 3)
 
 
@@ -474,7 +482,8 @@ def _position64(kv, name, slot, p):
     c = kv[name][slot, :, b, i] if name == "k" else kv[name][slot, :, b, :, i // 8, :, i % 8].flatten(1)
     x = _numbers64(c, kv["format"]) * kv[name + "_scale"][slot, :, b].double()[:, None]
     still = kv["open"][slot] == b + 1
-    return torch.where(still[:, None], kv[name + "_open"][slot, :, i].double(), x)
+    o = kv["k_open"][slot, :, i] if name == "k" else kv["v_open"][slot, :, :, i // 8, :, i % 8].flatten(1)
+    return torch.where(still[:, None], o.double(), x)
 
 
 def _exact_write(case, s):
@@ -510,7 +519,8 @@ def _exact_attend(case, s):
         v = v * kv["v_scale"][w].double()[..., None, None]
         b = int(kv["open"][w, 0]) - 1
         if b >= 0:
-            k[:, b], v[:, b] = kv["k_open"][w].double(), kv["v_open"][w].double()
+            k[:, b] = kv["k_open"][w].double()
+            v[:, b] = kv["v_open"][w].double().permute(0, 2, 4, 1, 3).reshape(k[:, b].shape)
         k, v = k.flatten(1, 2), v.flatten(1, 2)
         lo = 0 if s["first"] is None else int(s["first"][r])
         for a in range(h):
