@@ -115,6 +115,123 @@ int mz_enc_attention(mz_ctx* c, uint64_t qkvh, uint64_t out, int clips, int nh);
 /* log-mel f32 [clips][n_mels][3000] -> f16 [clips][3000][n_mels] (the conv stem's source layout). */
 int mz_mel_transpose(mz_ctx* c, uint64_t mel, uint64_t melT, int clips, int n_mels);
 
+/* ------------------------------------------------------------------ key/value caches held in 8 bits, token scores
+ *
+ * No counterpart in the reference, whose caches are fp16 (src/model.rs:436-452) and whose decoder keeps no
+ * probabilities. As the kernels above: device addresses, 64-wide heads, work enqueued on the context's stream and
+ * capturable (no allocation, no host synchronisation). Positions, lengths and slots are read on the device, so that a
+ * captured graph can be replayed while they change; one that lies outside a cache touches nothing, as stated below.
+ *
+ * A cache holds `slots` sequences of up to blocks * 32 positions. Each block of 32 positions x 64 channels of a (slot,
+ * head) has one scale for its keys and one for its values; code c stands for c * scale, with
+ *   MZ_KV8_I8:   c a signed whole number, scale = f32(top / 127), c = 127 x / top to the nearest, halves to even
+ *   MZ_KV8_E4M3: c an OCP e4m3 number,    scale = f32(top / 448), c = 448 x / top to the nearest, halves to even
+ * where top is the block's largest magnitude (0: scale 0 and codes 0). A block is coded when its last position is
+ * written; until then it is the open block of its (slot, head) (at most one) and holds its positions in fp16 as they
+ * were given. A block with a NaN or an infinity in it gets the scale NaN: all of its positions stand for NaN. */
+#define MZ_KV8_I8 0
+#define MZ_KV8_E4M3 1
+#define MZ_KV8_BLOCK 32
+typedef struct {
+    int format, slots, heads, blocks;
+    uint64_t k;       /* codes [slots][heads][blocks][32 positions][64 channels] */
+    uint64_t v;       /* codes [slots][heads][blocks][32 pairs of channels][4][2 channels][8 positions]: position t and
+                       * channel d at ((d / 2) * 4 + t / 8) * 16 + d % 2 * 8 + t % 8 */
+    uint64_t k_scale; /* f32 [slots][heads][blocks] */
+    uint64_t v_scale;
+    uint64_t k_open;  /* f16 [slots][heads][32][64]: the open block, positions in the order of k */
+    uint64_t v_open;  /* f16 [slots][heads][32][4][2][8]: in the order of v */
+    uint64_t open;    /* i32 [slots][heads]: 1 + the open block, 0: none */
+} mz_kv8;
+/* Lays a cache for max_tokens positions a slot out in one buffer at `base` (256-byte aligned; 0 to ask for the size
+ * only): fills in *kv and the buffer's size (either may be null). A zero-filled buffer (mz_alloc) is an empty cache. */
+int mz_kv8_place(int format, int slots, int heads, int max_tokens, uint64_t base, mz_kv8* kv, size_t* bytes);
+
+/* Keys and values f16 of `rows` sequences, strides in elements (multiples of 8, every address a multiple of 16 bytes):
+ * row r's token i, head h at k + r * row_stride + i * token_stride + h * head_stride, its 64 channels together. Row r
+ * is the sequence in slot slot[r] (slot 0: r), its token i has position pos[r * pos_stride] + pos_add + i (pos 0:
+ * pos_add + i), and count[r] of its `tokens` tokens are there (count 0: all; at most `tokens`). */
+typedef struct {
+    uint64_t k, v;
+    int64_t row_stride, token_stride, head_stride;
+    int rows, tokens;
+    uint64_t slot; /* i32 [rows] */
+    uint64_t pos;  /* i32 */
+    int pos_stride, pos_add;
+    uint64_t count; /* i32 [rows] */
+} mz_kv8_io;
+/* Writes the rows' tokens at their positions. Sequences are written in order: a row's first position is at most the
+ * number of positions its slot holds, and what a slot held behind the last position written is gone. A write that
+ * begins inside a coded block opens it again: its earlier positions become what their codes stand for, in fp16. A row
+ * whose slot or positions lie outside the cache writes nothing, and neither does one whose slot a later row names
+ * too. */
+int mz_kv8_write(mz_ctx* c, const mz_kv8* kv, const mz_kv8_io* a);
+/* Reads positions back: f16(f32(code * scale)), or an open block's fp16. Here k and v are written (either may be 0: not
+ * wanted); rows whose slot lies outside the cache, tokens whose position does and tokens from count[r] on are left as
+ * they were. Rows may share slots. */
+int mz_kv8_read(mz_ctx* c, const mz_kv8* kv, const mz_kv8_io* a);
+
+/* out = softmax(scale q . k) v over the positions that each query sees; row r's query token i, head h at
+ * q + r * q_row + i * q_token + h * q_head (f16, strides in elements, multiples of 8, addresses multiples of 16 bytes;
+ * the same for out, whose 64-channel rows must not overlap). Query head h reads the cache's head h / (heads /
+ * kv->heads). Rows may share slots (beams over one encoder output). */
+typedef struct {
+    uint64_t q, out;
+    int64_t q_row, q_token, q_head, out_row, out_token, out_head;
+    int rows, tokens, heads; /* heads: a multiple of the cache's, at most 64 times as many */
+    int causal;
+    float scale;    /* > 0, at most 2^20 */
+    uint64_t slot;  /* i32 [rows], 0: row r is slot r */
+    uint64_t count; /* i32 [rows]: tokens of row r that are there (0: all); the others' outputs are left as they were */
+    /* token i sees positions from first[r] (first 0: from 0) to below len[r * len_stride] + len_add (len 0: len_add),
+     * and with `causal` i more; never past the cache. A query that sees nothing, or whose row's slot lies outside the
+     * cache, gets out 0 and lse -inf. What lies outside the positions seen is never looked at, NaN or not. */
+    uint64_t len; /* i32 */
+    int len_stride, len_add;
+    uint64_t first; /* i32 [rows] */
+    uint64_t lse;   /* f32 [rows][tokens][heads]: ln of the sum of exp(scale q . k), 0: not wanted */
+    /* alignment rows of chosen heads: head h's probabilities go to align [rows][tokens][align_heads][align_cols] (f32)
+     * at index head_slot[h] (i32 [heads]; outside 0 .. align_heads - 1: none; of heads with one index the first
+     * counts), 0 at positions not seen. align 0: not wanted. */
+    uint64_t head_slot, align;
+    int align_heads, align_cols;
+    uint64_t work; /* mz_kv8_attention_bytes bytes of device memory (256-byte aligned), not shared with calls that may
+                    * run at the same time */
+    size_t work_bytes;
+} mz_kv8_attention_args;
+int mz_kv8_attention(mz_ctx* c, const mz_kv8* kv, const mz_kv8_attention_args* a);
+/* The workspace that the call needs (`work` and `work_bytes` are not looked at); may be 0. */
+int mz_kv8_attention_bytes(mz_ctx* c, const mz_kv8* kv, const mz_kv8_attention_args* a, size_t* bytes);
+
+/* What a model's answers are worth: for each of `rows` rows of `vocab` logits the log probability of a given token, the
+ * distribution's entropy (both natural logarithms) and the `alts` (0 .. 16) most probable tokens with theirs, ties to
+ * the lowest id. Ids with a nonzero mask byte have probability 0, as have logits of -inf; tokens of probability 0 are
+ * no alternatives: where fewer are left, ids are -1 and log probabilities -inf. A row with a NaN or a logit of +inf
+ * (unmasked) gets NaN throughout and ids -1; one with nothing left -inf, entropy 0 and ids -1. */
+typedef struct {
+    int dtype; /* MZ_DT_F16 or MZ_DT_F32 */
+    int rows, vocab, alts;
+    uint64_t logits; /* row r at element r * ld (ld >= vocab); any alignment of the element */
+    int64_t ld;
+    uint64_t mask; /* u8 [vocab], 0: none */
+    /* row r's token is tokens[r * token_stride + n] (i32) and its results go to index r * out_stride + n of logp and
+     * entropy (f32) and the same times alts of alt_ids (i32) and alt_logp (f32), with n = *at + at_add (at 0: n = 0): a
+     * captured step keeps its scores beside its tokens, with `at` the step's position. A row whose n is outside
+     * 0 .. out_stride - 1 writes nothing. A negative token, or an n outside 0 .. token_stride - 1: no token, log
+     * probability 0; a token >= vocab: NaN. Any of logp, entropy, alt_ids and alt_logp may be 0: not wanted. */
+    uint64_t tokens;
+    int64_t token_stride;
+    uint64_t at; /* i32 */
+    int at_add;
+    uint64_t logp, entropy;
+    int64_t out_stride;
+    uint64_t alt_ids, alt_logp;
+    uint64_t work; /* mz_token_scores_bytes bytes, as mz_kv8_attention_args.work */
+    size_t work_bytes;
+} mz_score_args;
+int mz_token_scores(mz_ctx* c, const mz_score_args* a);
+int mz_token_scores_bytes(mz_ctx* c, const mz_score_args* a, size_t* bytes);
+
 /* ------------------------------------------------------------------ engine (src/model.rs, src/transcribe.rs) */
 
 /* Model geometry (Dims, src/model.rs:14-25). */

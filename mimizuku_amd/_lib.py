@@ -41,10 +41,38 @@ class Times(C.Structure):
     _fields_ = [("enc", C.c_double), ("dec", C.c_double), ("post", C.c_double), ("steps", C.c_int)]
 
 
+class Kv8(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("format", "slots", "heads", "blocks")] +
+                [(n, u64) for n in ("k", "v", "k_scale", "v_scale", "k_open", "v_open", "open")])
+
+
+class Kv8Io(C.Structure):
+    _fields_ = [("k", u64), ("v", u64), ("row_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("rows", C.c_int), ("tokens", C.c_int), ("slot", u64), ("pos", u64),
+                ("pos_stride", C.c_int), ("pos_add", C.c_int), ("count", u64)]
+
+
+class Kv8Attention(C.Structure):
+    _fields_ = ([("q", u64), ("out", u64)] +
+                [(n, C.c_int64) for n in ("q_row", "q_token", "q_head", "out_row", "out_token", "out_head")] +
+                [(n, C.c_int) for n in ("rows", "tokens", "heads", "causal")] +
+                [("scale", C.c_float), ("slot", u64), ("count", u64), ("len", u64), ("len_stride", C.c_int),
+                 ("len_add", C.c_int), ("first", u64), ("lse", u64), ("head_slot", u64), ("align", u64),
+                 ("align_heads", C.c_int), ("align_cols", C.c_int), ("work", u64), ("work_bytes", C.c_size_t)])
+
+
+class ScoreArgs(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("dtype", "rows", "vocab", "alts")] +
+                [("logits", u64), ("ld", C.c_int64), ("mask", u64), ("tokens", u64), ("token_stride", C.c_int64),
+                 ("at", u64), ("at_add", C.c_int), ("logp", u64), ("entropy", u64), ("out_stride", C.c_int64),
+                 ("alt_ids", u64), ("alt_logp", u64), ("work", u64), ("work_bytes", C.c_size_t)])
+
+
 EPI_F16, EPI_GELU_F16, EPI_RESID_F32, EPI_GELU_POS, EPI_HEADS = range(5)
 (BUF_TOK, BUF_DONE, BUF_CTR, BUF_ALIGN, BUF_ENC_OUT, BUF_LOGITS, BUF_TRACE, BUF_XKV, BUF_DEC_X, BUF_ENC_X,
  BUF_DEC_TRACE, BUF_SELF_K, BUF_SELF_V, BUF_ALIGN_H) = range(14)
 DT_F16, DT_F32 = 0, 1
+KV8_I8, KV8_E4M3, KV8_BLOCK = 0, 1, 32
 # kernel classes of mz_engine_profile_read
 K_NAMES = ["mel", "conv1", "conv2", "ln", "qkv", "attn", "oproj", "fc1", "fc2", "xkv", "step",
            "dec_embed", "dec_qkv", "dec_self", "dec_oproj", "dec_addln", "dec_cross", "dec_xo", "dec_fc1", "dec_fc2",
@@ -77,6 +105,13 @@ SIGNATURES = {
     "mz_add_layernorm": (i32, [P, u64, u64, u64, u64, u64, i32, i32, f32]),
     "mz_enc_attention": (i32, [P, u64, u64, i32, i32]),
     "mz_mel_transpose": (i32, [P, u64, u64, i32, i32]),
+    "mz_kv8_place": (i32, [i32, i32, i32, i32, u64, C.POINTER(Kv8), C.POINTER(sz)]),
+    "mz_kv8_write": (i32, [P, C.POINTER(Kv8), C.POINTER(Kv8Io)]),
+    "mz_kv8_read": (i32, [P, C.POINTER(Kv8), C.POINTER(Kv8Io)]),
+    "mz_kv8_attention": (i32, [P, C.POINTER(Kv8), C.POINTER(Kv8Attention)]),
+    "mz_kv8_attention_bytes": (i32, [P, C.POINTER(Kv8), C.POINTER(Kv8Attention), C.POINTER(sz)]),
+    "mz_token_scores": (i32, [P, C.POINTER(ScoreArgs)]),
+    "mz_token_scores_bytes": (i32, [P, C.POINTER(ScoreArgs), C.POINTER(sz)]),
     "mz_scratch_bytes": (sz, [C.POINTER(Dims), i32, i32, i32]),
     "mz_engine_new": (i32, [P, C.POINTER(Dims), C.POINTER(GenCfgC), i32, i32, C.POINTER(P)]),
     "mz_engine_put": (i32, [P, C.c_char_p, i32, P, C.POINTER(C.c_int64), i32]),

@@ -254,3 +254,67 @@ struct MzMel {
 };
 // frames: those of all clips that hold audio
 hipError_t mz_log_mel_launch(hipStream_t s, const MzMel& p, long frames);
+
+// ---------------------------------------------------------------- key/value caches held in 8 bits (mz_kv8 in mimizuku.h)
+#define MZ_KV_BLK 32            // positions of a block
+#define MZ_KV_TILE (32 * 64)    // its elements: codes in bytes, or an open block's fp16
+struct MzKv8 {
+    int format, slots, heads, blocks;
+    unsigned char *k, *v;
+    float *k_scale, *v_scale;
+    f16 *k_open, *v_open;
+    int* open;
+};
+struct MzKv8Io {
+    f16 *k, *v;  // read: either may be null
+    long row_stride, token_stride, head_stride;
+    int rows, tokens;
+    const int *slot, *pos;
+    int pos_stride, pos_add;
+    const int* count;
+};
+// workgroups of a launch; the caller keeps them below 2^31
+long mz_kv8_write_grid(const MzKv8& kv, const MzKv8Io& a);
+long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a);
+hipError_t mz_kv8_write_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a);
+hipError_t mz_kv8_read_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a);
+
+struct MzKv8Attn {
+    const f16* q;
+    f16* out;
+    long q_row, q_token, q_head, out_row, out_token, out_head;
+    int rows, tokens, heads, causal;
+    float scale;
+    const int *slot, *count, *len;
+    int len_stride, len_add;
+    const int* first;
+    float* lse;
+    const int* head_slot;  // null without alignment rows
+    float* align;
+    int align_heads, align_cols;
+    float* work;
+};
+long mz_kv8_attn_grid(const MzKv8& kv, const MzKv8Attn& a);
+size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a);
+hipError_t mz_kv8_attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a);
+
+// ---------------------------------------------------------------- token scores (mz_score_args in mimizuku.h)
+#define MZ_SCORE_ALTS 16
+struct MzScores {
+    int half;  // logits fp16
+    int rows, vocab, alts;
+    const void* logits;
+    long ld;
+    const unsigned char* mask;
+    const int* tokens;
+    long token_stride;
+    const int* at;
+    int at_add;
+    float *logp, *entropy;
+    long out_stride;
+    int* alt_ids;
+    float* alt_logp;
+    float* work;
+};
+size_t mz_scores_work(const MzScores& p);
+hipError_t mz_scores_launch(hipStream_t s, const MzScores& p);

@@ -26,6 +26,7 @@ class Context:
     def __init__(self, device: int = 0):
         self.h = C.c_void_p()
         self.engines = weakref.WeakSet()
+        self.work = (0, 0)
         check(L.lib().mz_init(device, C.byref(self.h)))
 
     def close(self):
@@ -34,6 +35,7 @@ class Context:
                 e.close()
             L.lib().mz_ctx_free(self.h)
             self.h = C.c_void_p()
+            self.work = (0, 0)
 
     def __del__(self):
         try:
@@ -63,6 +65,15 @@ class Context:
         out = np.empty(shape, dtype)
         check(L.lib().mz_download(self.h, ptr(out), src, out.nbytes))
         return out
+
+    def workspace(self, nbytes: int) -> tuple[int, int]:
+        """(address, bytes) of a scratch buffer of at least nbytes for calls on this context's stream, which run one
+        after the other and share it. Grown by a new buffer; the smaller one stays allocated until the context is
+        closed, for graphs captured with it. It allocates: the first call of a size comes before a capture."""
+        if nbytes > self.work[1]:
+            n = max(2 * self.work[1], nbytes, 1 << 20)
+            self.work = (self.alloc(n), n)
+        return self.work
 
     def sync(self):
         check(L.lib().mz_sync(self.h))
