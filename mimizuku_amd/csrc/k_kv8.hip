@@ -1,5 +1,5 @@
 // Key/value caches held in 8 bits: writing, reading back, and attention over them (layout and definitions: mz_kv8 in
-// mimizuku.h). Plain kernels: one wave per (row, head), or per query.
+// mimizuku.h).
 #include "mz_common.h"
 #include "mz_kernels.h"
 
@@ -11,141 +11,6 @@ enum { I8 = 0, E4M3 = 1 };
 
 // element of position t (of its block) and channel d in a block of values
 __device__ __forceinline__ int v_at(int t, int d) { return ((d >> 1) * 4 + (t >> 3)) * 16 + (d & 1) * 8 + (t & 7); }
-
-// what a code stands for, without its scale
-template <int FMT>
-__device__ __forceinline__ float code_value(unsigned char c) {
-    if (FMT == I8) return (float)(signed char)c;
-    const int e = (c >> 3) & 15, m = c & 7;
-    if (e == 15 && m == 7) return NAN;
-    return copysignf(e ? ldexpf(1.f + m * 0.125f, e - 7) : ldexpf((float)m, -9), c & 128 ? -1.f : 1.f);
-}
-
-// f16(f32(code * scale)). The product is kept from the compiler: it would fold it and the conversion into one mixed-width
-// multiply-add of a positive zero, which rounds once and makes -0 to +0.
-__device__ __forceinline__ f16 stands_for(float code, float scale) {
-    float v = code * scale;
-    asm("" : "+v"(v));
-    return (f16)v;
-}
-
-// T x / top rounded as the real quotient would be. y = T x is exact in 32 bits (an fp16 value times 127 or 7 * 64), and
-// the quotient of two such numbers is either halfway between two codes, and then a number of 32 bits, or at least 2^-19
-// (relative) away from halfway; v is the quotient to the nearest 32-bit number (one correction of q by the exact
-// remainder), so that rounding it again gives the code of the real quotient. rc = 1 / top.
-template <int FMT>
-__device__ __forceinline__ float quotient(float x, float top, float rc) {
-    const float y = x * (FMT == I8 ? 127.f : 448.f), q = y * rc;
-    return fmaf(fmaf(-q, top, y), rc, q);
-}
-
-// a block's scale and 1 / top from the largest magnitude's fp16 bits (NaN and infinities above every number's)
-template <int FMT>
-__device__ __forceinline__ void block_scale(unsigned bits, float& top, float& rc, float& scale) {
-    top = (float)__builtin_bit_cast(f16, (unsigned short)bits);
-    scale = bits < 0x7c00u ? top / (FMT == I8 ? 127.f : 448.f) : NAN;
-    if (bits == 0 || bits >= 0x7c00u) top = rc = 0.f;  // codes 0
-    else rc = 1.f / top;
-}
-
-template <int FMT>
-__device__ __forceinline__ unsigned char code_of(f16 x, float top, float rc) {
-    const float v = top > 0.f ? quotient<FMT>((float)x, top, rc) : 0.f;
-    if (FMT == I8) return (unsigned char)(signed char)(int)rintf(v);
-    return (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 255);
-}
-
-__device__ __forceinline__ unsigned magnitude(f16 x) { return __builtin_bit_cast(unsigned short, x) & 0x7fffu; }
-
-// row r's slot and positions; false if there is nothing to do for it
-struct Row {
-    long slot;
-    int p, n;
-};
-__device__ __forceinline__ bool row_of(const MzKv8& kv, const MzKv8Io& a, int r, Row& o) {
-    o.slot = a.slot ? a.slot[r] : r;
-    const long p = (long)a.pos_add + (a.pos ? a.pos[(long)r * a.pos_stride] : 0);
-    o.n = a.count ? min(max(a.count[r], 0), a.tokens) : a.tokens;
-    o.p = (int)p;
-    return o.slot >= 0 && o.slot < kv.slots && p >= 0 && p <= (long)kv.blocks * MZ_KV_BLK;
-}
-
-template <int FMT>
-__global__ void __launch_bounds__(64) write_kernel(MzKv8 kv, MzKv8Io a) {
-    const int r = blockIdx.x / kv.heads, h = blockIdx.x - r * kv.heads, lane = threadIdx.x;
-    Row w;
-    if (!row_of(kv, a, r, w) || w.n <= 0 || w.p + (long)w.n > (long)kv.blocks * MZ_KV_BLK) return;
-    if (a.slot)
-        for (int i = r + 1; i < a.rows; i++)
-            if (a.slot[i] == w.slot) return;
-    const long sh = w.slot * kv.heads + h;
-    const int open = kv.open[sh], first = w.p / MZ_KV_BLK, last = (w.p + w.n - 1) / MZ_KV_BLK;
-    for (int side = 0; side < 2; side++) {
-        const f16* src = (side ? a.v : a.k) + r * a.row_stride + h * a.head_stride;
-        unsigned char* codes = (side ? kv.v : kv.k) + sh * kv.blocks * MZ_KV_TILE;
-        float* scales = (side ? kv.v_scale : kv.k_scale) + sh * kv.blocks;
-        f16* op = (side ? kv.v_open : kv.k_open) + sh * MZ_KV_TILE;
-        auto at = [&](int t) { return side ? v_at(t, lane) : t * 64 + lane; };  // lane: the channel
-        for (int b = first; b <= last; b++) {
-            const int off = max(w.p - b * MZ_KV_BLK, 0), end = min(w.p + w.n - b * MZ_KV_BLK, MZ_KV_BLK);
-            f16 x[MZ_KV_BLK];
-            unsigned top = 0;
-            for (int t = 0; t < end; t++) {
-                if (t >= off) x[t] = src[(long)(b * MZ_KV_BLK + t - w.p) * a.token_stride + lane];
-                else if (open == b + 1) x[t] = op[at(t)];
-                else x[t] = stands_for(code_value<FMT>(codes[(long)b * MZ_KV_TILE + at(t)]), scales[b]);
-                top = max(top, magnitude(x[t]));
-            }
-            if (end < MZ_KV_BLK) {
-                for (int t = open == b + 1 ? off : 0; t < end; t++) op[at(t)] = x[t];
-                continue;
-            }
-            float ft, rc, sc;
-            block_scale<FMT>((unsigned)wave_max((float)top), ft, rc, sc);
-            for (int t = 0; t < MZ_KV_BLK; t++) codes[(long)b * MZ_KV_TILE + at(t)] = code_of<FMT>(x[t], ft, rc);
-            if (lane == 0) scales[b] = sc;
-        }
-    }
-    if (lane == 0) kv.open[sh] = (w.p + w.n) % MZ_KV_BLK ? last + 1 : 0;
-}
-
-template <int FMT>
-__global__ void __launch_bounds__(64) read_kernel(MzKv8 kv, MzKv8Io a) {
-    const int r = blockIdx.x / kv.heads, h = blockIdx.x - r * kv.heads, lane = threadIdx.x;
-    Row w;
-    if (!row_of(kv, a, r, w)) return;
-    const long sh = w.slot * kv.heads + h;
-    const int open = kv.open[sh];
-    for (int i = 0; i < w.n && w.p + i < kv.blocks * MZ_KV_BLK; i++) {
-        const int b = (w.p + i) / MZ_KV_BLK, t = (w.p + i) % MZ_KV_BLK;
-        const long o = r * a.row_stride + i * a.token_stride + h * a.head_stride + lane, e = (sh * kv.blocks + b) * MZ_KV_TILE;
-        if (a.k)
-            a.k[o] = open == b + 1 ? kv.k_open[sh * MZ_KV_TILE + t * 64 + lane]
-                                   : stands_for(code_value<FMT>(kv.k[e + t * 64 + lane]), kv.k_scale[sh * kv.blocks + b]);
-        if (a.v)
-            a.v[o] = open == b + 1 ? kv.v_open[sh * MZ_KV_TILE + v_at(t, lane)]
-                                   : stands_for(code_value<FMT>(kv.v[e + v_at(t, lane)]), kv.v_scale[sh * kv.blocks + b]);
-    }
-}
-
-// ---------------------------------------------------------------- attention
-//
-// One pass over the cache with the running maximum and sum of the softmax. A workgroup takes 16 QT queries of one (row,
-// cache head) (its tokens times the query heads that share the cache head) and a share of the blocks; its four waves
-// take the blocks in turn, each with a state of its own, and join them at the end.
-//
-// Per block of 32 positions, with 16x16x32 products: S^T = K Q^T, the rows of tile j being positions 8 (i / 4) + 4 j + i % 4,
-// so that lane (query c, group g) of the two results holds the eight positions 8 g .. 8 g + 7 of its query. These
-// are, in this order, the k values of that lane in the product O^T = V^T P^T: the probabilities go from one product to the
-// other in registers, with no exchange between lanes. The values are kept so that one 16-byte load gives a lane
-// both channels 2 p and 2 p + 1 of its eight positions, the keys so that one gives 16 channels of a position.
-//
-// Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' into
-// the block's addition to the state. P is rounded to fp16 (half a step 2^-11 relative, as the output's own rounding); it is
-// at most 2^8, because the maximum of a state is moved only when a score passes it by more than 8 (in powers of two): most
-// blocks need no exchange between lanes and no rescaling.
-
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
 
 // eight codes as fp16
 template <int FMT>
@@ -166,6 +31,293 @@ __device__ __forceinline__ f16x8 widen(unsigned lo, unsigned hi) {
     }
     return f16x8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
+
+// f16(f32(code * scale)). The product is kept from the compiler: it would fold it and the conversion into one mixed-width
+// multiply-add of a positive zero, which rounds once and makes -0 to +0.
+__device__ __forceinline__ f16 stands_for(f16 code, float scale) {
+    float v = (float)code * scale;
+    asm("" : "+v"(v));
+    return (f16)v;
+}
+__device__ __forceinline__ f16x8 stand_for(f16x8 code, float scale) {
+    f16x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; e++) r[e] = stands_for(code[e], scale);
+    return r;
+}
+template <int FMT>
+__device__ __forceinline__ f16 one_stands_for(unsigned char code, float scale) {
+    return stands_for(widen<FMT>(code, 0)[0], scale);
+}
+
+// T x / top rounded as the real quotient would be. y = T x is exact in 32 bits (an fp16 value times 127 or 7 * 64), and
+// the quotient of two such numbers is either halfway between two codes, and then a number of 32 bits, or at least 2^-19
+// (relative) away from halfway; v is the quotient to the nearest 32-bit number (one correction of q by the exact
+// remainder), so that rounding it again gives the code of the real quotient. rc = 1 / top.
+template <int FMT>
+__device__ __forceinline__ float quotient(f16 x, float top, float rc) {
+    const float y = (float)x * (FMT == I8 ? 127.f : 448.f), q = y * rc;
+    return fmaf(fmaf(-q, top, y), rc, q);
+}
+
+// four codes in a word. Whole numbers: adding 1.5 * 2^23 rounds to one, halves to even, and leaves it in the low byte.
+template <int FMT>
+__device__ __forceinline__ unsigned codes4(f16 a, f16 b, f16 c, f16 d, float top, float rc) {
+    const float x[4] = {quotient<FMT>(a, top, rc), quotient<FMT>(b, top, rc), quotient<FMT>(c, top, rc), quotient<FMT>(d, top, rc)};
+    if (FMT == I8) {
+        unsigned u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[i] = __builtin_bit_cast(unsigned, x[i] + 12582912.f);
+        const unsigned lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+        return lo | hi;
+    }
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
+}
+
+// the larger magnitudes of two pairs of fp16 numbers as bits (NaN above infinity above every number)
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 larger(u16x2 m, unsigned pair) {
+    return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, pair & 0x7fff7fffu));
+}
+
+// a block's top, 1 / top (both 0 where all codes are 0) and scale, from every lane's largest magnitudes
+template <int FMT>
+__device__ __forceinline__ float block_scale(u16x2 m, float& top, float& rc) {
+    const unsigned bits = (unsigned)wave_max((float)max(m[0], m[1]));
+    top = rc = 0.f;
+    if (bits >= 0x7c00u) return NAN;
+    if (bits == 0) return 0.f;
+    top = (float)__builtin_bit_cast(f16, (unsigned short)bits);
+    rc = 1.f / top;
+    return top / (FMT == I8 ? 127.f : 448.f);
+}
+
+// row r's slot and positions; false if there is nothing to do for it
+struct Row {
+    long slot;
+    int p, n;
+};
+__device__ __forceinline__ bool row_of(const MzKv8& kv, const MzKv8Io& a, int r, Row& o) {
+    o.slot = a.slot ? a.slot[r] : r;
+    const long p = (long)a.pos_add + (a.pos ? a.pos[(long)r * a.pos_stride] : 0);
+    o.n = a.count ? min(max(a.count[r], 0), a.tokens) : a.tokens;
+    o.p = (int)p;
+    return o.n > 0 && o.slot >= 0 && o.slot < kv.slots && p >= 0 && p < (long)kv.blocks * MZ_KV_BLK;
+}
+
+// Lanes over a block, keys: 8 channels of positions lane / 8 + 8 i; values: 4 channels of 8 positions, so that whole
+// 16-byte pieces of the order of v are a lane's own.
+//
+// A wave codes one side of one block: its positions below `off` were there before (in the open block if `open`, else as
+// codes), those below `end` are new. Positions that only stay in an open block are not touched.
+template <int FMT>
+struct Writer {
+    const MzKv8& kv;
+    const MzKv8Io& a;
+    long sh;
+    const f16* src;  // row, head and side applied
+    int side, lane, p, n, open;
+
+    int off, end;
+    bool full, old;
+    f16x8 x[4];  // keys: position lane / 8 + 8 i; values: channel 4 c + i, positions 8 g .. 8 g + 7
+
+    __device__ __forceinline__ void load(int b) {
+        off = max(p - b * MZ_KV_BLK, 0);
+        end = min(p + n - b * MZ_KV_BLK, MZ_KV_BLK);
+        full = end == MZ_KV_BLK;
+        old = off > 0 && (full || open != b);  // earlier positions are wanted
+        const f16* s = src + (long)(b * MZ_KV_BLK - p) * a.token_stride;
+        const long blk = sh * kv.blocks + b;
+        if (side == 0) {
+            const int d = (lane & 7) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int t = (lane >> 3) + 8 * i;
+                x[i] = f16x8{};
+                if (t >= off && t < end) x[i] = __builtin_nontemporal_load((const f16x8*)(s + t * a.token_stride + d));
+                else if (old && t < off) {
+                    if (open == b) x[i] = ld8(kv.k_open + sh * MZ_KV_TILE + t * 64 + d);
+                    else {
+                        const uint2 c = *(const uint2*)(kv.k + blk * MZ_KV_TILE + t * 64 + d);
+                        x[i] = stand_for(widen<FMT>(c.x, c.y), kv.k_scale[blk]);
+                    }
+                }
+            }
+        } else {
+            const int d = (lane & 15) * 4, t0 = (lane >> 4) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int t = t0 + j;
+                f16x4 y = {};
+                if (t >= off && t < end) y = __builtin_nontemporal_load((const f16x4*)(s + t * a.token_stride + d));
+                else if (old && t < off) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        y[e] = open == b ? kv.v_open[sh * MZ_KV_TILE + v_at(t, d + e)]
+                                         : one_stands_for<FMT>(kv.v[blk * MZ_KV_TILE + v_at(t, d + e)], kv.v_scale[blk]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e][j] = y[e];
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(int b) {
+        const long blk = sh * kv.blocks + b;
+        if (full) {
+            u16x2 m = {};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint4 u = __builtin_bit_cast(uint4, x[i]);
+                m = larger(larger(larger(larger(m, u.x), u.y), u.z), u.w);
+            }
+            float top, rc;
+            const float scale = block_scale<FMT>(m, top, rc);
+            uint2 c[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                c[i] = uint2{codes4<FMT>(x[i][0], x[i][1], x[i][2], x[i][3], top, rc), codes4<FMT>(x[i][4], x[i][5], x[i][6], x[i][7], top, rc)};
+                if (top == 0.f) c[i] = uint2{0, 0};
+            }
+            if (side == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) *(uint2*)(kv.k + blk * MZ_KV_TILE + lane * 8 + 512 * i) = c[i];
+                if (lane == 0) kv.k_scale[blk] = scale;
+            } else {
+                unsigned char* v = kv.v + blk * MZ_KV_TILE + (lane & 15) * 128 + (lane >> 4) * 16;
+                *(uint4*)v = uint4{c[0].x, c[0].y, c[1].x, c[1].y};
+                *(uint4*)(v + 64) = uint4{c[2].x, c[2].y, c[3].x, c[3].y};
+                if (lane == 0) kv.v_scale[blk] = scale;
+            }
+            return;
+        }
+        const int lo = old ? 0 : off;
+        if (side == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int t = (lane >> 3) + 8 * i;
+                if (t >= lo && t < end) *(f16x8*)(kv.k_open + sh * MZ_KV_TILE + t * 64 + (lane & 7) * 8) = x[i];
+            }
+        } else {
+            const int d = (lane & 15) * 4, t0 = (lane >> 4) * 8;
+            f16* v = kv.v_open + sh * MZ_KV_TILE;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (t0 + j >= lo && t0 + j < end)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[v_at(t0 + j, d + e)] = x[e][j];
+        }
+    }
+};
+
+// Workgroup 0 of a (row, head) takes its first and its last block, which may want the open block and may leave one; the
+// others two of those between each. Waves: keys and values of the one, keys and values of the other.
+template <int FMT>
+__global__ void __launch_bounds__(256) write_kernel(MzKv8 kv, MzKv8Io a, int groups) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = blockIdx.x % groups;
+    const int rh = blockIdx.x / groups, r = rh / kv.heads, h = rh - r * kv.heads;
+    Row w;
+    if (!row_of(kv, a, r, w) || w.p + (long)w.n > (long)kv.blocks * MZ_KV_BLK) return;
+    const int first = w.p / MZ_KV_BLK, last = (w.p + w.n - 1) / MZ_KV_BLK;
+    const int b = grp ? first + 2 * grp - 1 + (wave >> 1) : wave < 2 ? first : last;
+    if (grp && first + 2 * grp - 1 >= last) return;
+    if (a.slot)  // the last row of a slot counts
+        for (int i = r + 1; i < a.rows; i += 64)
+            if (__ballot(i + lane < a.rows && a.slot[i + lane < a.rows ? i + lane : i] == w.slot)) return;
+    const long sh = w.slot * kv.heads + h;
+    const int side = wave & 1;
+    Writer<FMT> x{kv, a, sh, (side ? a.v : a.k) + r * a.row_stride + h * a.head_stride, side, lane, w.p, w.n, grp ? -1 : kv.open[sh] - 1};
+    const bool mine = grp ? b < last : wave < 2 || last > first;
+    if (mine) x.load(b);
+    if (grp == 0) __syncthreads();  // the open block is read before it is written
+    if (mine) x.store(b);
+    if (grp == 0 && threadIdx.x == 0) kv.open[sh] = (w.p + w.n) % MZ_KV_BLK ? last + 1 : 0;
+}
+
+// a wave: one side of one block of a (row, head)
+template <int FMT>
+__global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a, int blocks, long units) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long unit = (long)blockIdx.x * 4 + wave, bh = unit / 2;
+    const int side = (int)(unit & 1);
+    f16* const base = side ? a.v : a.k;
+    if (unit >= units || !base) return;
+    const long rh = bh / blocks;
+    const int r = (int)(rh / kv.heads), h = (int)(rh - (long)r * kv.heads);
+    Row w;
+    if (!row_of(kv, a, r, w)) return;
+    const int b = w.p / MZ_KV_BLK + (int)(bh - rh * blocks);
+    const int lo = max(w.p - b * MZ_KV_BLK, 0), hi = min((int)min((long)w.p + w.n, (long)kv.blocks * MZ_KV_BLK) - b * MZ_KV_BLK, MZ_KV_BLK);
+    if (hi <= lo) return;
+    const long sh = w.slot * kv.heads + h, blk = sh * kv.blocks + b;
+    const bool open = kv.open[sh] == b + 1;
+    f16* o = base + r * a.row_stride + h * a.head_stride + (long)(b * MZ_KV_BLK - w.p) * a.token_stride;
+    if (side == 0) {
+        const int d = (lane & 7) * 8;
+        f16x8 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = (lane >> 3) + 8 * i;
+            if (open) x[i] = ld8(kv.k_open + sh * MZ_KV_TILE + t * 64 + d);
+            else {
+                const uint2 c = *(const uint2*)(kv.k + blk * MZ_KV_TILE + t * 64 + d);
+                x[i] = stand_for(widen<FMT>(c.x, c.y), kv.k_scale[blk]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = (lane >> 3) + 8 * i;
+            if (t >= lo && t < hi) *(f16x8*)(o + t * a.token_stride + d) = x[i];
+        }
+    } else {
+        const int c = lane & 15, g = lane >> 4;
+        f16x8 x[4];  // channel 4 c + i, positions 8 g ..
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int at = ((2 * c + e) * 4 + g) * 16;
+            if (open) {
+                x[2 * e] = ld8(kv.v_open + sh * MZ_KV_TILE + at);
+                x[2 * e + 1] = ld8(kv.v_open + sh * MZ_KV_TILE + at + 8);
+            } else {
+                const uint4 u = *(const uint4*)(kv.v + blk * MZ_KV_TILE + at);
+                const float s = kv.v_scale[blk];
+                x[2 * e] = stand_for(widen<FMT>(u.x, u.y), s);
+                x[2 * e + 1] = stand_for(widen<FMT>(u.z, u.w), s);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int t = 8 * g + j;
+            if (t >= lo && t < hi) *(f16x4*)(o + t * a.token_stride + 4 * c) = f16x4{x[0][j], x[1][j], x[2][j], x[3][j]};
+        }
+    }
+}
+
+// the most blocks that `tokens` positions of a row can lie in
+long spanned(int tokens) { return ((long)tokens + MZ_KV_BLK - 2) / MZ_KV_BLK + 1; }
+// workgroups of a (row, head): the first and the last block, and two of the others each
+long write_groups(int tokens) { return 1 + std::max(0L, spanned(tokens) - 1) / 2; }
+
+// ---------------------------------------------------------------- attention
+//
+// One pass over the cache with the running maximum and sum of the softmax. A workgroup takes 16 QT queries of one (row,
+// cache head) (its tokens times the query heads that share the cache head) and a share of the blocks; its four waves
+// take the blocks in turn, each with a state of its own, and join them at the end.
+//
+// Per block of 32 positions, with 16x16x32 products: S^T = K Q^T, the rows of tile j being positions 8 (i / 4) + 4 j + i % 4,
+// so that lane (query c, group g) of the two results holds the eight positions 8 g .. 8 g + 7 of its query. These
+// are, in this order, the k values of that lane in the product O^T = V^T P^T: the probabilities go from one product to the
+// other in registers, with no exchange between lanes. The values are kept so that one 16-byte load gives a lane
+// both channels 2 p and 2 p + 1 of its eight positions, the keys so that one gives 16 channels of a position.
+//
+// Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' into
+// the block's addition to the state. P is rounded to fp16 (half a step 2^-11 relative, as the output's own rounding); it is
+// at most 2^8, because the maximum of a state is moved only when a score passes it by more than 8 (in powers of two): most
+// blocks need no exchange between lanes and no rescaling.
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
 
 // maximum / sum over the four lanes of a column (lane ^ 16, ^ 32), in each of them
 __device__ __forceinline__ float column_max(float v) {
@@ -491,9 +643,8 @@ void attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a, const Launc
 
 }  // namespace
 
-long mz_kv8_write_grid(const MzKv8& kv, const MzKv8Io& a) { return (long)a.rows * kv.heads; }
-long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a) { return (long)a.rows * kv.heads; }
-
+long mz_kv8_write_grid(const MzKv8& kv, const MzKv8Io& a) { return (long)a.rows * kv.heads * write_groups(a.tokens); }
+long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a) { return ((long)a.rows * kv.heads * spanned(a.tokens) * 2 + 3) / 4; }
 long mz_kv8_attn_grid(const MzKv8& kv, const MzKv8Attn& a) {
     const Launch n = attn_shape(kv, a);
     const long main = ((long)a.rows * kv.heads + 7) / 8 * 8 * n.tiles * n.splits, join = (long)a.rows * a.tokens * a.heads;
@@ -506,16 +657,19 @@ size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a) {
 }
 
 hipError_t mz_kv8_write_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) {
-    const dim3 grid(mz_kv8_write_grid(kv, a));
-    if (kv.format == I8) hipLaunchKernelGGL(write_kernel<I8>, grid, dim3(64), 0, s, kv, a);
-    else hipLaunchKernelGGL(write_kernel<E4M3>, grid, dim3(64), 0, s, kv, a);
+    const dim3 grid(mz_kv8_write_grid(kv, a)), block(a.tokens == 1 ? 128 : 256);  // (one token: one block)
+    const int groups = (int)write_groups(a.tokens);
+    if (kv.format == I8) hipLaunchKernelGGL(write_kernel<I8>, grid, block, 0, s, kv, a, groups);
+    else hipLaunchKernelGGL(write_kernel<E4M3>, grid, block, 0, s, kv, a, groups);
     return hipGetLastError();
 }
 
 hipError_t mz_kv8_read_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) {
     const dim3 grid(mz_kv8_read_grid(kv, a));
-    if (kv.format == I8) hipLaunchKernelGGL(read_kernel<I8>, grid, dim3(64), 0, s, kv, a);
-    else hipLaunchKernelGGL(read_kernel<E4M3>, grid, dim3(64), 0, s, kv, a);
+    const int blocks = (int)spanned(a.tokens);
+    const long units = (long)a.rows * kv.heads * blocks * 2;
+    if (kv.format == I8) hipLaunchKernelGGL(read_kernel<I8>, grid, dim3(256), 0, s, kv, a, blocks, units);
+    else hipLaunchKernelGGL(read_kernel<E4M3>, grid, dim3(256), 0, s, kv, a, blocks, units);
     return hipGetLastError();
 }
 
