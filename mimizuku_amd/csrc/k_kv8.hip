@@ -312,8 +312,9 @@ long write_groups(int tokens) { return 1 + std::max(0L, spanned(tokens) - 1) / 2
 // other in registers, with no exchange between lanes. The values are kept so that one 16-byte load gives a lane
 // both channels 2 p and 2 p + 1 of its eight positions, the keys so that one gives 16 channels of a position.
 //
-// Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' into
-// the block's addition to the state. P is rounded to fp16 (half a step 2^-11 relative, as the output's own rounding); it is
+// Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' (as a
+// multiple of the state's unit, a power of two above every scale so far) into P before its rounding, or, where it is
+// below 2^-7 of the unit, into the block's product after it. P is rounded to fp16 (half a step 2^-11 relative, as the output's own rounding); it is
 // at most 2^8, because the maximum of a state is moved only when a score passes it by more than 8 (in powers of two): most
 // blocks need no exchange between lanes and no rescaling.
 
@@ -340,38 +341,68 @@ struct Seen {
     }
 };
 __device__ __forceinline__ Seen seen_of(const MzKv8& kv, const MzKv8Attn& a, int r) {
+    // (if any array is there all are read, an absent one's place being some other word: the loads go out together, where
+    // a branch around each would wait for one after the other)
+    int slot = 0, first = 0, len = 0, count = 0;
+    if (a.slot || a.first || a.len || a.count) {
+        slot = *(a.slot ? a.slot + r : kv.open);
+        first = *(a.first ? a.first + r : kv.open);
+        len = *(a.len ? a.len + (long)r * a.len_stride : kv.open);
+        count = *(a.count ? a.count + r : kv.open);
+    }
     Seen s;
-    s.slot = a.slot ? a.slot[r] : r;
+    s.slot = a.slot ? slot : r;
     s.cap = kv.blocks * MZ_KV_BLK;
-    s.base = (long)a.len_add + (a.len ? a.len[(long)r * a.len_stride] : 0);
-    s.first = a.first ? max(a.first[r], 0) : 0;
-    s.count = a.count ? min(max(a.count[r], 0), a.tokens) : a.tokens;
+    s.base = (long)a.len_add + (a.len ? len : 0);
+    s.first = a.first ? max(first, 0) : 0;
+    s.count = a.count ? min(max(count, 0), a.tokens) : a.tokens;
     if (s.slot < 0 || s.slot >= kv.slots) s.slot = s.cap = 0;
     return s;
 }
 
-// head h's row of alignment probabilities of (r, i), or null
-__device__ __forceinline__ float* align_row(const MzKv8Attn& a, int r, int i, int h) {
-    const int s = a.head_slot[h];
-    if (s < 0 || s >= a.align_heads) return nullptr;
-    for (int j = 0; j < h; j++)
-        if (a.head_slot[j] == s) return nullptr;
-    return a.align + (((long)r * a.tokens + i) * a.align_heads + s) * a.align_cols;
+// Alignment indices of the query heads h0 .. h0 + n - 1, by all threads of the workgroup: of heads with one index the
+// first has it.
+__device__ __forceinline__ void align_indices(const MzKv8Attn& a, int h0, int n, int (&index)[64]) {
+    const int tid = threadIdx.x;
+    if (tid < n) {
+        const int s = a.head_slot[h0 + tid];
+        index[tid] = s < a.align_heads ? s : -1;
+    }
+    __syncthreads();
+    for (int j = tid; j < h0 + n; j += 256) {
+        const int s = a.head_slot[j];
+        for (int k = 0; k < n; k++)
+            if (h0 + k > j && a.head_slot[h0 + k] == s) index[k] = -1;
+    }
+    __syncthreads();
 }
 
-// scores (in powers of two) to probabilities, by all threads of the workgroup; 0 where nothing is seen
-__device__ __forceinline__ void align_finish(float* row, int cols, int lo, int hi, float lse2) {
-    for (int p = threadIdx.x; p < cols; p += 256)
-        row[p] = p >= lo && p < hi ? __builtin_amdgcn_exp2f(row[p] - lse2) : 0.f;
+// Scores (in powers of two) to probabilities, by all threads of the workgroup; 0 where nothing is seen. get(p) is the score of
+// a position that is; eight of them on their way at a time.
+template <typename Get>
+__device__ __forceinline__ void align_finish(float* row, int cols, int lo, int hi, float lse2, Get get) {
+    for (int p0 = threadIdx.x; p0 < cols; p0 += 2048) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int p = p0 + 256 * k;
+            x[k] = -INFINITY;
+            if (p < cols && p >= lo && p < hi) x[k] = get(p);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (p0 + 256 * k < cols) row[p0 + 256 * k] = x[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[k] - lse2);
+    }
 }
 
 struct Launch {
     int qt, tiles, splits;  // queries a workgroup / 16, such tiles of a (row, cache head), workgroups the blocks are shared by
+    int kept;               // alignment rows: scores that a workgroup keeps in LDS for each query, 0: in their rows
 };
 constexpr int STATE = 66;  // floats of a query's partial state: 64 channels, maximum, sum
 
 template <int FMT, int QT, bool ALIGN>
-__global__ void __launch_bounds__(256) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
+__global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
     __shared__ float red[4][16][68], ms[4][16], ls[4][16];
     __shared__ float* als[16];
     __shared__ float lse2s[16];
@@ -391,12 +422,15 @@ __global__ void __launch_bounds__(256) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch
     const int share = (nb + n.splits - 1) / n.splits, b0 = b_lo + min(split * share, nb), b1 = b_lo + min((split + 1) * share, nb);
 
     const long sh = s.slot * kv.heads + kh;
-    const int open = s.cap ? kv.open[sh] - 1 : -1;
+    const int open_word = kv.open[sh], open = s.cap ? open_word - 1 : -1;
     const unsigned char* kc = kv.k + sh * kv.blocks * MZ_KV_TILE;
     const unsigned char* vc = kv.v + sh * kv.blocks * MZ_KV_TILE;
     const float* ksc = kv.k_scale + sh * kv.blocks;
     const float* vsc = kv.v_scale + sh * kv.blocks;
 
+    extern __shared__ float kept[];  // [query][n.kept]
+    __shared__ int index[ALIGN ? 64 : 1];
+    if constexpr (ALIGN) align_indices(a, kh * grp, grp, index);
     f16x8 qf[QT][2];
     int end[QT];
     float* al[QT];
@@ -408,39 +442,31 @@ __global__ void __launch_bounds__(256) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch
         qf[t][0] = on ? ld8(q) : f16x8{};
         qf[t][1] = on ? ld8(q + 8) : f16x8{};
         end[t] = on ? s.end(a, i) : 0;
-        if (ALIGN) al[t] = on ? align_row(a, r, i, h) : nullptr;
+        if (ALIGN) {
+            const int k = on ? index[x - i * grp] : -1;
+            al[t] = k >= 0 ? a.align + (((long)r * a.tokens + i) * a.align_heads + k) * a.align_cols : nullptr;
+        }
     }
 
-    // a block as it lies: codes in d[0 .. 3], or the open block's fp16
+    // a coded block as it lies
     struct Raw {
-        uint4 d[8];
+        uint4 k[2], v[2];
         float ks, vs;
     };
     const unsigned ktok = 8 * (c >> 2) + (c & 3);  // row c of key tile 0; tile 1 is 4 positions on
     auto fetch = [&](int b, Raw& w) {
-        if (b == open) {
-            const f16* ko = kv.k_open + sh * MZ_KV_TILE;
-            const f16* vo = kv.v_open + sh * MZ_KV_TILE;
+        const unsigned char* k = kc + (long)b * MZ_KV_TILE;
+        const unsigned char* v = vc + (long)b * MZ_KV_TILE;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                w.d[j] = *(const uint4*)(ko + (ktok + 4 * (j >> 1)) * 64 + 16 * g + 8 * (j & 1));
-                w.d[4 + j] = *(const uint4*)(vo + ((16 * (j >> 1) + c) * 4 + g) * 16 + 8 * (j & 1));
-            }
-            w.ks = w.vs = 1.f;
-        } else {
-            const unsigned char* k = kc + (long)b * MZ_KV_TILE;
-            const unsigned char* v = vc + (long)b * MZ_KV_TILE;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                w.d[j] = *(const uint4*)(k + (ktok + 4 * j) * 64 + 16 * g);
-                w.d[2 + j] = *(const uint4*)(v + ((16 * j + c) * 4 + g) * 16);
-            }
-            w.ks = ksc[b];
-            w.vs = vsc[b];
+        for (int j = 0; j < 2; j++) {
+            w.k[j] = *(const uint4*)(k + (ktok + 4 * j) * 64 + 16 * g);
+            w.v[j] = *(const uint4*)(v + ((16 * j + c) * 4 + g) * 16);
         }
+        w.ks = ksc[b];
+        w.vs = vsc[b];
     };
 
-    float m[QT], l[QT];
+    float m[QT], l[QT], unit = 0.f;  // the accumulators are in `unit`s, a power of two that no block's values' scale passes
     f32x4 acc[QT][4];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -450,47 +476,48 @@ __global__ void __launch_bounds__(256) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch
         for (int u = 0; u < 4; u++) acc[t][u] = f32x4{};
     }
     const float scale2 = a.scale * LOG2E;
-    auto block = [&](int b, const Raw& w) {
-        f16x8 kf[2][2], vf[4];
+    auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], float ks, float vs) {
         const int p0 = b * MZ_KV_BLK + 8 * g;  // this lane's positions
-        if (b == open) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                kf[j >> 1][j & 1] = __builtin_bit_cast(f16x8, w.d[j]);
-                vf[j] = __builtin_bit_cast(f16x8, w.d[4 + j]);
-#pragma unroll
-                for (int e = 0; e < 8; e++)  // what no query of the tile sees may be no number
-                    if (p0 + e < s.first || p0 + e >= hi) vf[j][e] = (f16)0.f;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                kf[j][0] = widen<FMT>(w.d[j].x, w.d[j].y);
-                kf[j][1] = widen<FMT>(w.d[j].z, w.d[j].w);
-                vf[2 * j] = widen<FMT>(w.d[2 + j].x, w.d[2 + j].y);
-                vf[2 * j + 1] = widen<FMT>(w.d[2 + j].z, w.d[2 + j].w);
-            }
-        }
-        const float cs = scale2 * w.ks;
+        float cs = scale2 * ks;
+        if (cs == 0.f) cs = 1e-37f;  // (all keys 0; what is not seen is -inf times it)
         const bool whole = b * MZ_KV_BLK >= s.first && (b + 1) * MZ_KV_BLK <= lo_end;  // seen by every query
+        const bool given = b == open;  // fp16 as it was given, any number: vs is 1 and says nothing about the numbers' size
+        if (given && unit == 0.f) unit = 9.5367431640625e-07f;
+        if (!given && vs > unit) {
+            const float to = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, vs) & 0x7f800000u) + 0x00800000u), f = unit / to;
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) acc[t][u] *= f;
+            unit = to;
+        }
+        const float part = vs == 0.f ? 0.f : vs / unit;  // P is multiplied by it, before its rounding if it is not small
+        const bool direct = !given && part >= 0.0078125f;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-            float x[8];
+            f32x4 d[2];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const f32x4 d = mfma16(kf[j][1], qf[t][1], mfma16(kf[j][0], qf[t][0], f32x4{}));
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[4 * j + e] = d[e] * cs;
-            }
+            for (int j = 0; j < 2; j++) d[j] = mfma16(kf[j][1], qf[t][1], mfma16(kf[j][0], qf[t][0], f32x4{}));
             if (!whole)
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    if (p0 + e < s.first || p0 + e >= end[t]) x[e] = -INFINITY;
-            if (ALIGN && al[t])
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (p0 + e >= s.first && p0 + e < min(end[t], a.align_cols)) al[t][p0 + e] = x[e];
-            const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                    if (p0 + e < s.first || p0 + e >= end[t]) d[e >> 2][e & 3] = -INFINITY;
+            if (ALIGN && al[t]) {
+                const f32x4 x[2] = {d[0] * cs, d[1] * cs};
+                if (n.kept) {
+                    f32x4* o = (f32x4*)(kept + (16 * t + c) * n.kept + p0 - b0 * MZ_KV_BLK);
+                    o[0] = x[0];
+                    o[1] = x[1];
+                } else {
+                    for (int e = 0; e < 8; e++)
+                        if (p0 + e >= s.first && p0 + e < min(end[t], a.align_cols)) {
+                            if (n.splits > 1) shared_store(al[t] + p0 + e, x[e >> 2][e & 3]);
+                            else al[t][p0 + e] = x[e >> 2][e & 3];
+                        }
+                }
+            }
+            const float top = cs * fmaxf(fmaxf(fmaxf(d[0][0], d[0][1]), fmaxf(d[0][2], d[0][3])),
+                                         fmaxf(fmaxf(d[1][0], d[1][1]), fmaxf(d[1][2], d[1][3])));
             if (__ballot(top > m[t] + 8.f)) {
                 const float mn = fmaxf(m[t], column_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
@@ -498,58 +525,124 @@ __global__ void __launch_bounds__(256) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch
 #pragma unroll
                 for (int u = 0; u < 4; u++) acc[t][u] *= f;
             }
+            float x[8];
             f16x8 p;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = __builtin_amdgcn_exp2f(x[e] - m[t]);
-                p[e] = (f16)x[e];
-            }
-            l[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            const bool any = whole || b * MZ_KV_BLK < end[t];  // (0 times a scale or a value that is no number is none)
+            for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], cs, -m[t]));
+            // (0 times a scale or a value that is no number is none: a query that does not see the block keeps its sums)
+            const bool any = whole || b * MZ_KV_BLK < end[t];
+            const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            l[t] += any ? sum : 0.f;
+            if (whole && direct) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const f32x4 d = mfma16(vf[u], p, f32x4{});
+                for (int e = 0; e < 8; e++) p[e] = (f16)(x[e] * part);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float y = fmaf(d[e], w.vs, acc[t][u][e]);
-                    acc[t][u][e] = whole || any ? y : acc[t][u][e];
+                for (int u = 0; u < 4; u++) acc[t][u] = mfma16(vf[u], p, acc[t][u]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) p[e] = (f16)x[e];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const f32x4 y = mfma16(vf[u], p, f32x4{});
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[t][u][e] = any ? fmaf(y[e], part, acc[t][u][e]) : acc[t][u][e];
                 }
             }
         }
     };
-    Raw w0, w1;
-    int b = b0 + wave;
-    if (b < b1) fetch(b, w0);
-    for (; b < b1; b += 8) {
-        if (b + 4 < b1) fetch(b + 4, w1);
-        block(b, w0);
-        if (b + 4 < b1) {
-            if (b + 8 < b1) fetch(b + 8, w0);
-            block(b + 4, w1);
+    auto coded = [&](int b, const Raw& w) {
+        f16x8 kf[2][2], vf[4];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            kf[j][0] = widen<FMT>(w.k[j].x, w.k[j].y);
+            kf[j][1] = widen<FMT>(w.k[j].z, w.k[j].w);
+            vf[2 * j] = widen<FMT>(w.v[j].x, w.v[j].y);
+            vf[2 * j + 1] = widen<FMT>(w.v[j].z, w.v[j].w);
+        }
+        products(b, kf, vf, w.ks, w.vs);
+    };
+    // Blocks b0 + wave, + 4, ...: DEPTH of them on their way (no branches around the loads: past the end the last block is
+    // loaded again). The open block, where it is this wave's, comes first; its codes are stale.
+    constexpr int DEPTH = QT == 1 ? 3 : 2;
+    Raw w[DEPTH];
+    if (b0 + wave < b1) {
+        const int tail = b0 + wave + (b1 - 1 - b0 - wave) / 4 * 4;
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) fetch(min(b0 + wave + 4 * i, tail), w[i]);
+        if (open >= b0 && open < b1 && ((open - b0) & 3) == wave) {
+            f16x8 kf[2][2], vf[4];
+            const f16* ko = kv.k_open + sh * MZ_KV_TILE;
+            const f16* vo = kv.v_open + sh * MZ_KV_TILE;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                kf[j >> 1][j & 1] = ld8(ko + (ktok + 4 * (j >> 1)) * 64 + 16 * g + 8 * (j & 1));
+                vf[j] = ld8(vo + ((16 * (j >> 1) + c) * 4 + g) * 16 + 8 * (j & 1));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {  // what no query of the tile sees may be no number
+                    const int p = open * MZ_KV_BLK + 8 * g + e;
+                    if (p < s.first || p >= hi) vf[j][e] = (f16)0.f;
+                }
+            products(open, kf, vf, 1.f, 1.f);
+        }
+        for (int b = b0 + wave; b <= tail; b += 4 * DEPTH) {
+#pragma unroll
+            for (int i = 0; i < DEPTH; i++) {
+                const int bi = b + 4 * i;
+                if (bi <= tail && bi != open) coded(bi, w[i]);
+                fetch(min(bi + 4 * DEPTH, tail), w[i]);
+            }
         }
     }
 
     // the four waves' states joined, 16 queries at a time; accumulator u of lane (c, g) holds channels
     // 32 (u / 2) + 8 g + 2 e + u % 2 of query c
     const int col = tid >> 4, d4 = (tid & 15) * 4;
+    auto emit = [&](int t, float mm, float ll, f32x4 o) {
+        const int x = q0 + 16 * t + col, i = x / grp, h = kh * grp + x - i * grp;
+        const float inv = ll == 0.f ? 0.f : 1.f / ll, lse2 = ll == 0.f ? -INFINITY : mm + __builtin_amdgcn_logf(ll);
+        if (x < nq && i < s.count) {
+            st4(a.out + r * a.out_row + i * a.out_token + h * a.out_head + d4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            if (a.lse && d4 == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
+        }
+        if (ALIGN) {
+            if (tid < 16) als[c] = al[t];
+            if (d4 == 0) lse2s[col] = lse2;
+            __syncthreads();
+            for (int k = 0; k < 16; k++) {
+                if (!als[k]) continue;
+                float* const row = als[k];
+                const int to = s.end(a, (q0 + 16 * t + k) / grp);
+                if (n.splits > 1)
+                    align_finish(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return shared_load(row + p); });
+                else if (n.kept) {
+                    const float* x = kept + (16 * t + k) * n.kept - b0 * MZ_KV_BLK;
+                    align_finish(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return x[p]; });
+                } else align_finish(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return row[p]; });
+            }
+            __syncthreads();
+        }
+    };
+    float* const states = a.work + JOIN_COUNTERS + (pair * n.tiles + tile) * n.splits * (16 * QT) * STATE;
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         const float lt = column_sum(l[t]);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             float* o = &red[wave][c][32 * u + 8 * g];
-            *(f32x4*)o = f32x4{acc[t][2 * u][0], acc[t][2 * u + 1][0], acc[t][2 * u][1], acc[t][2 * u + 1][1]};
-            *(f32x4*)(o + 4) = f32x4{acc[t][2 * u][2], acc[t][2 * u + 1][2], acc[t][2 * u][3], acc[t][2 * u + 1][3]};
+            const f32x4 x = acc[t][2 * u], y = acc[t][2 * u + 1];
+            *(f32x4*)o = f32x4{x[0] * unit, y[0] * unit, x[1] * unit, y[1] * unit};
+            *(f32x4*)(o + 4) = f32x4{x[2] * unit, y[2] * unit, x[3] * unit, y[3] * unit};
         }
         if (g == 0) {
             ms[wave][c] = m[t];
             ls[wave][c] = lt;
-            if (ALIGN && wave == 0) als[c] = al[t];
         }
         __syncthreads();
-        const int x = q0 + 16 * t + col, i = x / grp, h = kh * grp + x - i * grp;
-        const bool on = x < nq && i < s.count;
-        float mm = fmaxf(fmaxf(ms[0][col], ms[1][col]), fmaxf(ms[2][col], ms[3][col])), ll = 0.f;
+        const float mm = fmaxf(fmaxf(ms[0][col], ms[1][col]), fmaxf(ms[2][col], ms[3][col]));
+        float ll = 0.f;
         f32x4 o = {};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -559,86 +652,80 @@ __global__ void __launch_bounds__(256) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = fmaf(f, y[e], o[e]);
         }
-        if (n.splits > 1) {
-            float* w = a.work + (((pair * n.tiles + tile) * n.splits + split) * (16 * QT) + 16 * t + col) * STATE;
-            *(float2*)(w + d4) = float2{o[0], o[1]};
-            *(float2*)(w + d4 + 2) = float2{o[2], o[3]};
-            if (d4 == 0) *(float2*)(w + 64) = float2{mm, ll};
-        } else {
-            const float inv = ll == 0.f ? 0.f : 1.f / ll, lse2 = ll == 0.f ? -INFINITY : mm + __builtin_amdgcn_logf(ll);
-            if (on) {
-                st4(a.out + r * a.out_row + i * a.out_token + h * a.out_head + d4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-                if (a.lse && d4 == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
-            }
-            if (ALIGN) {
-                if (d4 == 0) lse2s[col] = lse2;
-                __syncthreads();
-                for (int k = 0; k < 16; k++)
-                    if (als[k]) align_finish(als[k], a.align_cols, s.first, s.end(a, (q0 + 16 * t + k) / grp), lse2s[k]);
-            }
+        if (n.splits == 1) emit(t, mm, ll, o);
+        else if (q0 + 16 * t + col < nq) {
+            float* w = states + (split * (16 * QT) + 16 * t + col) * STATE;
+            shared_store(w + d4, o[0], o[1]);
+            shared_store(w + d4 + 2, o[2], o[3]);
+            if (d4 == 0) shared_store(w + 64, mm, ll);
         }
-        __syncthreads();
+        if (ALIGN && n.splits > 1 && n.kept) {  // the share's scores to where the last workgroup finds them
+            if (tid < 16) als[c] = al[t];
+            __syncthreads();
+            for (int k = 0; k < 16; k++)
+                if (als[k])
+                    for (int p = b0 * MZ_KV_BLK + tid; p < min(b1 * MZ_KV_BLK, a.align_cols); p += 256)
+                        shared_store(als[k] + p, kept[(16 * t + k) * n.kept + p - b0 * MZ_KV_BLK]);
+        }
+        if (t + 1 < QT) __syncthreads();
     }
-}
-
-// The states of a query's splits joined, a workgroup a query: wave w takes splits w, w + 4, ...
-__global__ void __launch_bounds__(256) attn_join_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
-    __shared__ float red[4][64], ms[4], ls[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, grp = a.heads / kv.heads;
-    const long id = blockIdx.x, ri = id / a.heads;
-    const int h = (int)(id - ri * a.heads), r = (int)(ri / a.tokens), i = (int)(ri - (long)r * a.tokens);
-    const Seen s = seen_of(kv, a, r);
-    if (i >= s.count) return;
-    const int x = i * grp + h % grp, qs = 16 * n.qt, tile = x / qs;
-    const long pair = (long)r * kv.heads + h / grp;
-    const float* w = a.work + ((pair * n.tiles + tile) * n.splits * qs + x - tile * qs) * STATE;
-    float m = NOTHING, l = 0.f, o = 0.f;
-    for (int k = wave; k < n.splits; k += 4) {
-        const float* p = w + (long)k * qs * STATE;
-        const float mk = p[64], lk = p[65], ok = p[lane], mn = fmaxf(m, mk);
-        const float f = __builtin_amdgcn_exp2f(m - mn), fk = __builtin_amdgcn_exp2f(mk - mn);
-        l = fmaf(l, f, lk * fk);
-        o = fmaf(o, f, ok * fk);
-        m = mn;
-    }
-    red[wave][lane] = o;
-    if (lane == 0) {
-        ms[wave] = m;
-        ls[wave] = l;
-    }
-    __syncthreads();
-    const float mm = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-    l = o = 0.f;
+    if (n.splits == 1 || !last_of((unsigned*)a.work + pair * n.tiles + tile, n.splits)) return;
+    // the last of the workgroups that share these queries joins their states
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const float f = __builtin_amdgcn_exp2f(ms[k] - mm);
-        l = fmaf(f, ls[k], l);
-        o = fmaf(f, red[k][lane], o);
+    for (int t = 0; t < QT; t++) {
+        float mm = NOTHING, ll = 0.f;
+        f32x4 o = {};
+        if (q0 + 16 * t + col < nq)
+            for (int k0 = 0; k0 < n.splits; k0 += 4) {
+                float2 x[4][3];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float* w = states + (min(k0 + k, n.splits - 1) * (16 * QT) + 16 * t + col) * STATE;
+                    x[k][0] = shared_load2(w + d4);
+                    x[k][1] = shared_load2(w + d4 + 2);
+                    x[k][2] = shared_load2(w + 64);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (k0 + k >= n.splits) continue;
+                    const float mn = fmaxf(mm, x[k][2].x), f0 = __builtin_amdgcn_exp2f(mm - mn), f1 = __builtin_amdgcn_exp2f(x[k][2].x - mn);
+                    mm = mn;
+                    ll = fmaf(ll, f0, x[k][2].y * f1);
+                    o = f32x4{fmaf(o[0], f0, x[k][0].x * f1), fmaf(o[1], f0, x[k][0].y * f1), fmaf(o[2], f0, x[k][1].x * f1),
+                              fmaf(o[3], f0, x[k][1].y * f1)};
+                }
+            }
+        emit(t, mm, ll, o);
     }
-    const float lse2 = l == 0.f ? -INFINITY : mm + __builtin_amdgcn_logf(l);
-    if (wave == 0) {
-        a.out[r * a.out_row + i * a.out_token + h * a.out_head + lane] = (f16)(l == 0.f ? 0.f : o / l);
-        if (a.lse && lane == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
-    }
-    if (a.head_slot)
-        if (float* row = align_row(a, r, i, h)) align_finish(row, a.align_cols, s.first, s.end(a, i), lse2);
 }
 
+// LDS for the scores of alignment rows: 1504 positions of five queries fit
+constexpr long KEPT_FLOATS = 8192;
+long kept_queries(const Launch& n, long nq) { return std::min(nq, 16L * n.qt); }
+
+// 16 queries a wave where there are no more, else 32 (224-token prompts of 8 rows, 20 heads: 19.4 us with 16 a workgroup, 16.6
+// with 32, 22.9 with 64). The blocks are shared by more workgroups where there are fewer units than CUs, until there
+// are two a CU or a wave has two blocks left: 1500 positions of one row, 20 heads, 10.8 us with one workgroup each, 7.8 with
+// 4 to 6, 8.8 with 11; 16,000 positions of 96 (row, head) pairs 34.1 with 2, 18.7 with 5, 19.1 with 10; 256 pairs 12.9 with
+// one, 14.2 with 2; 640 pairs 28.0 and 30.6.
 Launch attn_shape(const MzKv8& kv, const MzKv8Attn& a) {
-    const long nq = (long)a.tokens * (a.heads / kv.heads), pairs = (long)a.rows * kv.heads;
+    const long nq = (long)a.tokens * (a.heads / kv.heads), cus = mz_cu_count();
     Launch n;
-    n.qt = nq <= 16 ? 1 : nq <= 32 ? 2 : 4;
+    n.qt = nq <= 16 ? 1 : 2;
     n.tiles = (int)((nq + 16 * n.qt - 1) / (16 * n.qt));
-    const long want = 2L * mz_cu_count() / (pairs * n.tiles);
-    n.splits = (int)std::max(1L, std::min(want, (long)kv.blocks / 4));
+    const long units = (long)a.rows * kv.heads * n.tiles, want = units < cus ? 2 * cus / units : 1;
+    n.splits = (int)std::max(1L, std::min(want, (long)kv.blocks / 8));
+    const long keep = ((long)kv.blocks + n.splits - 1) / n.splits * MZ_KV_BLK;
+    n.kept = a.align && keep * kept_queries(n, nq) <= KEPT_FLOATS ? (int)keep : 0;
     return n;
 }
+static_assert(JOIN_COUNTERS >= 1024, "units that are shared have a counter each: fewer than the CUs");
 
 template <int FMT, bool ALIGN>
 void attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a, const Launch& n, long grid) {
-    if (n.qt == 1) hipLaunchKernelGGL((attn_kernel<FMT, 1, ALIGN>), dim3(grid), dim3(256), 0, s, kv, a, n);
-    else if (n.qt == 2) hipLaunchKernelGGL((attn_kernel<FMT, 2, ALIGN>), dim3(grid), dim3(256), 0, s, kv, a, n);
-    else hipLaunchKernelGGL((attn_kernel<FMT, 4, ALIGN>), dim3(grid), dim3(256), 0, s, kv, a, n);
+    const size_t lds = (size_t)n.kept * kept_queries(n, (long)a.tokens * (a.heads / kv.heads)) * 4;
+    if (n.qt == 1) hipLaunchKernelGGL((attn_kernel<FMT, 1, ALIGN>), dim3(grid), dim3(256), lds, s, kv, a, n);
+    else hipLaunchKernelGGL((attn_kernel<FMT, 2, ALIGN>), dim3(grid), dim3(256), lds, s, kv, a, n);
 }
 
 }  // namespace
@@ -647,13 +734,12 @@ long mz_kv8_write_grid(const MzKv8& kv, const MzKv8Io& a) { return (long)a.rows 
 long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a) { return ((long)a.rows * kv.heads * spanned(a.tokens) * 2 + 3) / 4; }
 long mz_kv8_attn_grid(const MzKv8& kv, const MzKv8Attn& a) {
     const Launch n = attn_shape(kv, a);
-    const long main = ((long)a.rows * kv.heads + 7) / 8 * 8 * n.tiles * n.splits, join = (long)a.rows * a.tokens * a.heads;
-    return n.splits > 1 ? std::max(main, join) : main;
+    return ((long)a.rows * kv.heads + 7) / 8 * 8 * n.tiles * n.splits;
 }
 
 size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a) {
     const Launch n = attn_shape(kv, a);
-    return n.splits > 1 ? (size_t)a.rows * kv.heads * n.tiles * n.splits * 16 * n.qt * STATE * 4 : 0;
+    return n.splits > 1 ? ((size_t)a.rows * kv.heads * n.tiles * n.splits * 16 * n.qt * STATE + JOIN_COUNTERS) * 4 : 0;
 }
 
 hipError_t mz_kv8_write_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) {
@@ -675,11 +761,8 @@ hipError_t mz_kv8_read_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) 
 
 hipError_t mz_kv8_attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a) {
     const Launch n = attn_shape(kv, a);
-    const long grid = ((long)a.rows * kv.heads + 7) / 8 * 8 * n.tiles * n.splits;
+    const long grid = mz_kv8_attn_grid(kv, a);
     if (kv.format == I8) a.align ? attn_launch<I8, true>(s, kv, a, n, grid) : attn_launch<I8, false>(s, kv, a, n, grid);
     else a.align ? attn_launch<E4M3, true>(s, kv, a, n, grid) : attn_launch<E4M3, false>(s, kv, a, n, grid);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || n.splits == 1) return e;
-    hipLaunchKernelGGL(attn_join_kernel, dim3((long)a.rows * a.tokens * a.heads), dim3(256), 0, s, kv, a, n);
     return hipGetLastError();
 }

@@ -169,3 +169,33 @@ __device__ __forceinline__ void st4(f16* p, float a, float b, float c, float d) 
     f16x4 v = {(f16)a, (f16)b, (f16)c, (f16)d};
     *(f16x4*)p = v;
 }
+
+// ---- Several workgroups' results joined by the last of them to end, without another launch. Workgroups of one launch run on
+// different XCDs, whose L2 caches do not see each other's lines: what is handed on is written through to memory and read
+// past the caches (agent scope), and it has arrived (vmcnt 0 in every wave, then a barrier) before the workgroup counts
+// itself in. The counter is 0 before and after.
+constexpr int JOIN_COUNTERS = 4096;  // words at the head of a workspace, whatever the call: always 0 between launches
+__device__ __forceinline__ void shared_store(float* p, float x) {
+    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void shared_store(float* p, float x, float y) {  // p a multiple of 8 bytes
+    __hip_atomic_store((unsigned long long*)p, __builtin_bit_cast(unsigned long long, float2{x, y}), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float shared_load(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 shared_load2(const float* p) {
+    return __builtin_bit_cast(float2, __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+// whether this workgroup (every thread of which calls) is the last of `n` to count itself in
+__device__ __forceinline__ bool last_of(unsigned* counter, int n) {
+    __shared__ unsigned before;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (before != (unsigned)n - 1) return false;
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}

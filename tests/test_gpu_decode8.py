@@ -430,11 +430,16 @@ def test_what_is_not_seen_is_not_looked_at(ctx, dev, fmt):
     for n in (90, 96):  # the block open, and coded
         k, v = f16(rng, (1, n, 1, 64)), f16(rng, (1, n, 1, 64))
         v[0, 70, 0, 9] = np.nan
-        b.write(dev, k, v)
-        q = f16(rng, (1, 30, 1, 64), 1.5)
-        out, lse, _ = run_attention(ctx, dev, b, q, True, [50])  # token i sees 50 + i
-        assert np.isfinite(out[0, :15]).all() and np.isfinite(lse[0, :15]).all()
-        assert np.isnan(out[0, 21:, :, 9]).all()
+        for kbad in (False, True):
+            if kbad:
+                k[0, 71, 0, 5] = np.inf
+            b.write(dev, k, v)
+            q = f16(rng, (1, 30, 1, 64), 1.5)
+            out, lse, _ = run_attention(ctx, dev, b, q, True, [50])  # token i sees 50 + i
+            assert np.isfinite(out[0, :15]).all() and np.isfinite(lse[0, :15]).all()
+            assert np.isnan(out[0, 22:, :, 9]).all()
+            # (in an open block an infinite key alone: a score of -inf where the query's channel is negative)
+            assert not kbad or np.isnan(lse[0, 22:][(q[0, 22:, :, 5] > 0) | (n == 96)]).all()
     b.free()
 
 
