@@ -45,10 +45,6 @@ __device__ __forceinline__ f16x8 stand_for(f16x8 code, float scale) {
     for (int e = 0; e < 8; e++) r[e] = stands_for(code[e], scale);
     return r;
 }
-template <int FMT>
-__device__ __forceinline__ f16 one_stands_for(unsigned char code, float scale) {
-    return stands_for(widen<FMT>(code, 0)[0], scale);
-}
 
 // T x / top rounded as the real quotient would be. y = T x is exact in 32 bits (an fp16 value times 127 or 7 * 64), and
 // the quotient of two such numbers is either halfway between two codes, and then a number of 32 bits, or at least 2^-19
@@ -121,7 +117,7 @@ struct Writer {
 
     int off, end;
     bool full, old;
-    f16x8 x[4];  // keys: position lane / 8 + 8 i; values: channel 4 c + i, positions 8 g .. 8 g + 7
+    f16x8 x[4] = {};  // keys: position lane / 8 + 8 i; values: channel 4 c + i, positions 8 g .. 8 g + 7
 
     __device__ __forceinline__ void load(int b) {
         off = max(p - b * MZ_KV_BLK, 0);
@@ -147,20 +143,31 @@ struct Writer {
             }
         } else {
             const int d = (lane & 15) * 4, t0 = (lane >> 4) * 8;
+            f16x4 y[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int t = t0 + j;
-                f16x4 y = {};
-                if (t >= off && t < end) y = __builtin_nontemporal_load((const f16x4*)(s + t * a.token_stride + d));
-                else if (old && t < off) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        y[e] = open == b ? kv.v_open[sh * MZ_KV_TILE + v_at(t, d + e)]
-                                         : one_stands_for<FMT>(kv.v[blk * MZ_KV_TILE + v_at(t, d + e)], kv.v_scale[blk]);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e][j] = y[e];
+                y[j] = f16x4{};
+                if (t >= off && t < end) y[j] = __builtin_nontemporal_load((const f16x4*)(s + t * a.token_stride + d));
             }
+            if (old) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int at = ((lane & 15) * 2 + e) * 64 + (lane >> 4) * 16;
+                    if (open == b) {
+                        x[2 * e] = ld8(kv.v_open + sh * MZ_KV_TILE + at);
+                        x[2 * e + 1] = ld8(kv.v_open + sh * MZ_KV_TILE + at + 8);
+                    } else {
+                        const uint4 u = *(const uint4*)(kv.v + blk * MZ_KV_TILE + at);
+                        x[2 * e] = stand_for(widen<FMT>(u.x, u.y), kv.v_scale[blk]);
+                        x[2 * e + 1] = stand_for(widen<FMT>(u.z, u.w), kv.v_scale[blk]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e][j] = t0 + j < off ? x[e][j] : y[j][e];
         }
     }
 
@@ -361,18 +368,19 @@ __device__ __forceinline__ Seen seen_of(const MzKv8& kv, const MzKv8Attn& a, int
 }
 
 // Alignment indices of the query heads h0 .. h0 + n - 1, by all threads of the workgroup: of heads with one index the
-// first has it.
-__device__ __forceinline__ void align_indices(const MzKv8Attn& a, int h0, int n, int (&index)[64]) {
+// first has it. mine: head_slot[threadIdx.x], requested earlier.
+__device__ __forceinline__ void align_indices(const MzKv8Attn& a, int h0, int n, int mine, int (&index)[64]) {
+    __shared__ int slots[64];
     const int tid = threadIdx.x;
-    if (tid < n) {
-        const int s = a.head_slot[h0 + tid];
-        index[tid] = s < a.align_heads ? s : -1;
+    for (int j = tid; j < h0 + n; j += 256) {
+        const int s = j == tid ? mine : a.head_slot[j];
+        if (j >= h0) slots[j - h0] = index[j - h0] = s < a.align_heads ? s : -1;
     }
     __syncthreads();
     for (int j = tid; j < h0 + n; j += 256) {
-        const int s = a.head_slot[j];
-        for (int k = 0; k < n; k++)
-            if (h0 + k > j && a.head_slot[h0 + k] == s) index[k] = -1;
+        const int s = j == tid ? mine : a.head_slot[j];
+        for (int k = max(0, j - h0 + 1); k < n; k++)
+            if (slots[k] == s) index[k] = -1;
     }
     __syncthreads();
 }
@@ -430,10 +438,16 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
 
     extern __shared__ float kept[];  // [query][n.kept]
     __shared__ int index[ALIGN ? 64 : 1];
-    if constexpr (ALIGN) align_indices(a, kh * grp, grp, index);
+    const int mine = ALIGN && tid < a.heads ? a.head_slot[tid] : -1;
+    if constexpr (ALIGN)
+        if (!n.kept) align_indices(a, kh * grp, grp, mine, index);
     f16x8 qf[QT][2];
     int end[QT];
     float* al[QT];
+    auto align_row = [&](int t) -> float* {
+        const int x = q0 + 16 * t + c, i = x / grp, k = x < nq && i < s.count ? index[x - i * grp] : -1;
+        return k >= 0 ? a.align + (((long)r * a.tokens + i) * a.align_heads + k) * a.align_cols : nullptr;
+    };
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         const int x = q0 + 16 * t + c, i = x / grp, h = kh * grp + x - i * grp;
@@ -442,10 +456,7 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
         qf[t][0] = on ? ld8(q) : f16x8{};
         qf[t][1] = on ? ld8(q + 8) : f16x8{};
         end[t] = on ? s.end(a, i) : 0;
-        if (ALIGN) {
-            const int k = on ? index[x - i * grp] : -1;
-            al[t] = k >= 0 ? a.align + (((long)r * a.tokens + i) * a.align_heads + k) * a.align_cols : nullptr;
-        }
+        al[t] = ALIGN && !n.kept ? align_row(t) : nullptr;
     }
 
     // a coded block as it lies
@@ -502,7 +513,7 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
 #pragma unroll
                 for (int e = 0; e < 8; e++)
                     if (p0 + e < s.first || p0 + e >= end[t]) d[e >> 2][e & 3] = -INFINITY;
-            if (ALIGN && al[t]) {
+            if (ALIGN && (n.kept ? 16 * t + c < qn - q0 : al[t] != nullptr)) {
                 const f32x4 x[2] = {d[0] * cs, d[1] * cs};
                 if (n.kept) {
                     f32x4* o = (f32x4*)(kept + (16 * t + c) * n.kept + p0 - b0 * MZ_KV_BLK);
@@ -597,6 +608,12 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
         }
     }
 
+    if constexpr (ALIGN)
+        if (n.kept) {
+            align_indices(a, kh * grp, grp, mine, index);
+#pragma unroll
+            for (int t = 0; t < QT; t++) al[t] = align_row(t);
+        }
     // the four waves' states joined, 16 queries at a time; accumulator u of lane (c, g) holds channels
     // 32 (u / 2) + 8 g + 2 e + u % 2 of query c
     const int col = tid >> 4, d4 = (tid & 15) * 4;

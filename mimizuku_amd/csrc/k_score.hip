@@ -16,12 +16,8 @@ constexpr int PARTS = 64;                            // most waves that share a 
 constexpr int NONE = 0x7fffffff;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// what one wave knows of its elements
-struct Part {
-    float m, s, u, pad;
-    float v[MZ_SCORE_ALTS];  // its best alternatives, best first
-    int id[MZ_SCORE_ALTS];
-};
+// What one wave knows of its elements: m, s, u, then its alternatives' keys, best first.
+constexpr int HEAD = 4, MOST = HEAD + 2 * MZ_SCORE_ALTS;
 
 // d = x - m to exp(d) and exp(d) d, 0 and 0 for -inf
 __device__ __forceinline__ void add(float x, float m, float& s, float& u) {
@@ -30,14 +26,106 @@ __device__ __forceinline__ void add(float x, float m, float& s, float& u) {
     u = fmaf(e, fmaxf(d, -200.f), u);
 }
 
-// Lane i < parts holds part i: the row's results. The alternatives are taken one after the other from the parts' lists.
-template <typename T>
-__device__ __forceinline__ void finish(const MzScores& p, int r, const Part* part, int parts, int lane) {
-    const long n = p.at ? (long)*p.at + p.at_add : 0;
-    if (n < 0 || n >= p.out_stride) return;
+// A value and an id as one number: the larger the better, of equal values the lowest id; 0: none (below -inf with any id).
+// 62 bits, so that as a number of 64 bits it is positive, finite and in the same order, and v_max_f64 takes the larger one.
+typedef unsigned long long Key;
+constexpr unsigned IDS = 1u << 30;
+__device__ __forceinline__ Key key_of(float v, int id) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    return (Key)(u ^ ((unsigned)((int)u >> 31) | 0x80000000u)) << 30 | (IDS - 1 - (unsigned)id);
+}
+__device__ __forceinline__ float value_of(Key k) {
+    const unsigned u = (unsigned)(k >> 30);
+    return k ? __builtin_bit_cast(float, u ^ (~(unsigned)((int)u >> 31) | 0x80000000u)) : -INFINITY;
+}
+__device__ __forceinline__ int id_of(Key k) { return (int)(IDS - 1 - ((unsigned)k & (IDS - 1))); }
+__device__ __forceinline__ Key larger(Key a, Key b) {
+    Key r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ Key smaller(Key a, Key b) {
+    Key r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ Key lane_key(Key k, int i) {
+    return (Key)(unsigned)__builtin_amdgcn_readlane((int)(k >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)k, i);
+}
+// ---- keys in order: networks of compare-and-exchange steps across lanes, best first within each row of 16 lanes. A step is
+// six instructions or so; finding the best of 64 lanes k times over takes about 70 dependent ones each time.
+template <int CTRL>
+__device__ __forceinline__ Key moved(Key k) {
+    return (Key)(unsigned)dpp_i<CTRL>((int)(k >> 32)) << 32 | (unsigned)dpp_i<CTRL>((int)k);
+}
+__device__ __forceinline__ int xor4(int v) {  // lanes with bit 2 clear read 4 on, the others 4 back
+    const int t = __builtin_amdgcn_update_dpp(0, v, 0x104, 0xF, 0x5, false);
+    return __builtin_amdgcn_update_dpp(t, v, 0x114, 0xF, 0xA, false);
+}
+// the better of k and p where `first` is set, the other one elsewhere
+__device__ __forceinline__ Key step(Key k, Key p, bool first) {
+    const Key a = larger(k, p), b = smaller(k, p);  // (both, where a branch would be taken)
+    return first ? a : b;
+}
+// a row whose better half is anywhere in bitonic order, best first
+__device__ __forceinline__ Key cleaned(Key k, int lane) {
+    k = step(k, moved<0x128>(k), !(lane & 8));
+    k = step(k, (Key)(unsigned)xor4((int)(k >> 32)) << 32 | (unsigned)xor4((int)k), !(lane & 4));
+    k = step(k, moved<0x4E>(k), !(lane & 2));
+    return step(k, moved<0xB1>(k), !(lane & 1));
+}
+// the best 16 of two sorted rows: the better of every pair of opposite places, put in order
+__device__ __forceinline__ Key joined(Key a, Key b, int lane) {
+    return cleaned(larger(a, moved<0x140>(b)), lane);
+}
+__device__ __forceinline__ Key other_row(Key k, int lane) {
+    const auto h = __builtin_amdgcn_permlane16_swap((unsigned)(k >> 32), (unsigned)(k >> 32), false, false);
+    const auto l = __builtin_amdgcn_permlane16_swap((unsigned)k, (unsigned)k, false, false);
+    return lane & 16 ? (Key)(unsigned)h[0] << 32 | (unsigned)l[0] : (Key)(unsigned)h[1] << 32 | (unsigned)l[1];
+}
+__device__ __forceinline__ Key other_half(Key k, int lane) {
+    const auto h = __builtin_amdgcn_permlane32_swap((unsigned)(k >> 32), (unsigned)(k >> 32), false, false);
+    const auto l = __builtin_amdgcn_permlane32_swap((unsigned)k, (unsigned)k, false, false);
+    return lane & 32 ? (Key)(unsigned)h[0] << 32 | (unsigned)l[0] : (Key)(unsigned)h[1] << 32 | (unsigned)l[1];
+}
+// the best 16 of the wave's 64 keys, best first, in every row
+__device__ __forceinline__ Key best16(Key k, int lane) {
+    k = step(k, moved<0xB1>(k), !(lane & 1));
+    k = step(k, moved<0x1B>(k), !(lane & 2));
+    k = step(k, moved<0xB1>(k), !(lane & 1));
+    k = step(k, moved<0x141>(k), !(lane & 4));
+    k = step(k, moved<0x4E>(k), !(lane & 2));
+    k = step(k, moved<0xB1>(k), !(lane & 1));
+    k = step(k, moved<0x140>(k), !(lane & 8));
+    k = step(k, (Key)(unsigned)xor4((int)(k >> 32)) << 32 | (unsigned)xor4((int)k), !(lane & 4));
+    k = step(k, moved<0x4E>(k), !(lane & 2));
+    k = step(k, moved<0xB1>(k), !(lane & 1));
+    k = joined(k, other_row(k, lane), lane);
+    return joined(k, other_half(k, lane), lane);
+}
+// LDS written by other lanes of the wave is read behind this (a wave's LDS operations run in order; the compiler is told so)
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// the lane with the largest of the wave's keys (v: their values), at least one of them not 0
+__device__ __forceinline__ int best_lane(float v, Key k) {
+    unsigned long long has = __ballot(v == wave_max(v));
+    int lane = __ffsll(has) - 1;
+    for (has &= has - 1; has; has &= has - 1) {  // (hardly ever)
+        const int other = __ffsll(has) - 1;
+        if (lane_key(k, other) > lane_key(k, lane)) lane = other;
+    }
+    return lane;
+}
+
+// The row's results from its parts (words as above, one lane each). The alternatives are taken one after the other from the
+// parts' lists. tok, xt: the given token and its logit.
+__device__ __forceinline__ void finish(const MzScores& p, long o, const float* part, int parts, int lane, int tok, float xt, Key (&pick)[64]) {
     const bool on = lane < parts;
-    float mi = on ? part[lane].m : -INFINITY;
-    const float si = on ? part[lane].s : 0.f, ui = on ? part[lane].u : 0.f;
+    const int words = HEAD + 2 * p.alts;
+    const float* mine = part + (on ? lane * words : 0);
+    const float mi = on ? mine[0] : -INFINITY, si = on ? mine[1] : 0.f, ui = on ? mine[2] : 0.f;
     const float m = wave_max(mi);
     // one of the parts with the row's maximum holds the element that S leaves out; the others' maxima count in it
     const bool owner = lane == __ffsll((unsigned long long)__ballot(mi == m)) - 1;
@@ -47,87 +135,123 @@ __device__ __forceinline__ void finish(const MzScores& p, int r, const Part* par
     const float S = wave_sum(owner || si != si ? si : t * e), U = wave_sum(owner ? ui : e == 0.f ? 0.f : e * fmaf(t, d, ui));
     const bool bad = S != S || m == INFINITY;
     const float z = log1pf(S);
-    const long o = r * p.out_stride + n;
-    if (lane == 0 && p.logp) {
-        const int tok = n < p.token_stride ? p.tokens[r * p.token_stride + n] : -1;
-        float lp = 0.f;
-        if (tok >= 0) {
-            if (bad || tok >= p.vocab) lp = NAN;
-            else if (m == -INFINITY || (p.mask && p.mask[tok])) lp = -INFINITY;
-            else lp = ((float)((const T*)p.logits)[r * p.ld + tok] - m) - z;
-        }
-        p.logp[o] = lp;
-    }
+    if (lane == 0 && p.logp)
+        p.logp[o] = tok < 0 ? 0.f : bad || tok >= p.vocab ? NAN : m == -INFINITY || xt == -INFINITY ? -INFINITY : (xt - m) - z;
     if (lane == 0 && p.entropy) p.entropy[o] = bad ? NAN : m == -INFINITY ? 0.f : z - U / (1.f + S);
-    float v = on && p.alts ? part[lane].v[0] : -INFINITY;
-    int id = on && p.alts ? part[lane].id[0] : NONE, at = 0;
-    for (int k = 0; k < p.alts; k++) {
-        float bv = v;
-        int bi = id;
-        wave_argmax(bv, bi);
-        if (lane == 0) {
-            if (p.alt_ids) p.alt_ids[o * p.alts + k] = bad || bv == -INFINITY ? -1 : bi;
-            if (p.alt_logp) p.alt_logp[o * p.alts + k] = bad ? NAN : bv == -INFINITY ? -INFINITY : (bv - m) - z;
+    if (!p.alts) return;
+    auto entry = [&](int k) -> Key {  // of the lane's list
+        return on && k < p.alts ? *(const Key*)(mine + HEAD + 2 * k) : 0;
+    };
+    Key x = entry(0), list = 0;
+    if (p.alts <= 10) {
+        // the part whose best is q-th has no more than alts - q of the row's: 55 at most
+        const Key firsts = best16(x, lane);
+        int q = x ? 0 : 64;
+        for (int k = 0; k < p.alts; k++) q += lane_key(firsts, k) > x;
+        pick[lane] = 0;
+        wave_lds();
+        if (q < p.alts)
+            for (int k = 0; k + q < p.alts; k++) pick[q * p.alts - q * (q - 1) / 2 + k] = entry(k);
+        wave_lds();
+        list = best16(pick[lane], lane);
+    } else
+        for (int k = 0, at = 0; k < p.alts; k++) {
+            const int l = best_lane(value_of(x), x);
+            if (lane == k) list = lane_key(x, l);
+            if (lane == l) x = entry(++at);
         }
-        if (id == bi && v == bv && v > -INFINITY) {
-            at++;
-            v = at < p.alts ? part[lane].v[at] : -INFINITY;
-            id = at < p.alts ? part[lane].id[at] : NONE;
-        }
-    }
+    if (lane >= p.alts) return;
+    if (p.alt_ids) p.alt_ids[o * p.alts + lane] = bad || !list ? -1 : id_of(list);
+    if (p.alt_logp) p.alt_logp[o * p.alts + lane] = bad ? NAN : list ? (value_of(list) - m) - z : -INFINITY;
 }
 
-// A workgroup's share of a row, four waves taking chunks of 1024 elements in turn. `splits` workgroups share a row, each
-// wave writing its part to the workspace (to LDS and the row finished here where there is one).
+// A workgroup's share of a row, four waves taking chunks of 1024 elements in turn. Where `splits` workgroups share a row the
+// last of them to end has the parts of all.
 template <typename T, bool MASK>
 __global__ void __launch_bounds__(256) score_kernel(MzScores p, int splits) {
     constexpr int V = 16 / sizeof(T), G = PER_LANE / V;  // elements of a 16-byte load, loads of a chunk
     typedef T TV __attribute__((ext_vector_type(V)));
-    __shared__ Part lds[4];
+    __shared__ __attribute__((aligned(8))) float lds[PARTS * MOST];
+    __shared__ Key pick[64];
+    __shared__ Key bound;  // no element with a smaller key is an alternative of the row
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = blockIdx.x / splits, split = blockIdx.x - r * splits;
     const T* row = (const T*)p.logits + r * p.ld;
+    const long n = p.at ? (long)*p.at + p.at_add : 0;
+    if (n < 0 || n >= p.out_stride) return;
+    if (tid == 0) bound = 0;
+    __syncthreads();
     // the row's 16-byte pieces, the first of which begins `off` elements before it
     const int off = (int)((uintptr_t)row % 16 / sizeof(T));
     const int chunks = (p.vocab + off + CHUNK - 1) / CHUNK, share = (chunks + splits - 1) / splits;
     const int c0 = split * share, c1 = min(c0 + share, chunks);
 
-    struct Raw {
-        TV x[G];
-        unsigned char mask[PER_LANE];
-    };
-    auto first = [&](int c, int j) { return (c * G + j) * 64 * V + lane * V - off; };  // id of lane's element 0 of load j
-    auto fetch = [&](int c, Raw& w) {
-#pragma unroll
-        for (int j = 0; j < G; j++) {
-            const int e = first(c, j);
-            if (e >= 0 && e + V <= p.vocab) {
-                w.x[j] = __builtin_nontemporal_load((const TV*)(row + e));
-                if (MASK) __builtin_memcpy(w.mask + j * V, p.mask + e, V);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; k++) {
-                    const bool in = e + k >= 0 && e + k < p.vocab;
-                    w.x[j][k] = in ? row[e + k] : (T)-INFINITY;
-                    if (MASK) w.mask[j * V + k] = in ? p.mask[e + k] : 0;
-                }
-            }
-        }
-    };
+    // Lane's element 0 of load j, a piece's first; the loads at the row's ends are moved into the row (`from`: where they
+    // are then), and what they have of other pieces is left out.
+    auto piece = [&](int c, int j) { return (c * G + j) * 64 * V + lane * V - off; };
+    auto from = [&](int e) { return max(min(e, p.vocab - V), 0); };
 
     float m = -INFINITY, S = 0.f, U = 0.f;  // m of the wave, the sums of the lane
-    float lv = -INFINITY, thr = -INFINITY;  // lane k: alternative k; thr: the last one's value
-    int li = NONE;
-    auto chunk = [&](int c, const Raw& w) {
-        float x[PER_LANE], top = -INFINITY;
+    Key list = 0, least = 0;  // lane k of each row: alternative k; the last one, or a larger bound that another wave found
+    // the given token and its logit, which each wait for a load
+    const int tok = p.logp && n < p.token_stride ? p.tokens[r * p.token_stride + n] : -1;
+    const bool known = tok >= 0 && tok < p.vocab;
+    const float xt = (float)row[known ? tok : 0];
+    const bool left_out = MASK && p.mask[known ? tok : 0];
+    typedef TV __attribute__((aligned(sizeof(T)))) Piece;
+    typedef unsigned Bits __attribute__((aligned(1)));
+    TV raw[G];
+    unsigned masks[PER_LANE / 4];
+    auto fetch = [&](int c) {
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            const int e = from(piece(c, j));
+            raw[j] = __builtin_nontemporal_load((const Piece*)(row + e));
+            if (MASK)
+#pragma unroll
+                for (int k = 0; k < V / 4; k++) masks[j * V / 4 + k] = *(const Bits*)(p.mask + e + 4 * k);
+        }
+    };
+    int c = c0 + wave;
+    if (p.vocab < V) {  // a row shorter than a piece: lane 0's
 #pragma unroll
         for (int j = 0; j < PER_LANE; j++) {
-            x[j] = (float)w.x[j / V][j % V];
-            if (MASK) x[j] = w.mask[j] ? -INFINITY : x[j];
-            top = fmaxf(top, x[j]);
+            raw[j / V][j % V] = row[min(j, p.vocab - 1)];
+            if (MASK) {
+                const unsigned bit = (p.mask[min(j, p.vocab - 1)] != 0) << (j % 4 * 8);
+                masks[j / 4] = j % 4 ? masks[j / 4] | bit : bit;
+            }
         }
-        const unsigned long long up = __ballot(top > m);
-        if (up) {  // a new maximum: the sums so far, the old maximum among them, become multiples of it
+    } else if (c < c1) fetch(c);
+    for (; c < c1; c += 4) {
+        float x[PER_LANE];
+#pragma unroll
+        for (int j = 0; j < PER_LANE; j++) {
+            x[j] = (float)raw[j / V][j % V];
+            if (MASK) x[j] = masks[j / 4] & 0xffu << (j % 4 * 8) ? -INFINITY : x[j];
+        }
+        if (c + 4 < c1) fetch(c + 4);  // on its way while this one is taken
+        if (c == 0 || c == chunks - 1)
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+                const int e = piece(c, j), at = from(e);
+#pragma unroll
+                for (int k = 0; k < V; k++) {
+                    const bool in = at + k >= e && at + k < min(e + V, p.vocab);
+                    x[j * V + k] = in ? x[j * V + k] : -INFINITY;
+                }
+            }
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < PER_LANE; j++) top = fmaxf(top, x[j]);
+        int at;  // the lane's best element, the first one of equal ones
+        auto find = [&]() {
+            at = 0;
+#pragma unroll
+            for (int j = PER_LANE - 1; j >= 0; j--) at = x[j] == top ? j : at;
+        };
+        if (__ballot(top > m)) {  // a new maximum: the sums so far, the old maximum among them, become multiples of it
+            find();
             const float mn = wave_max(top);
             const bool own = lane == __ffsll((unsigned long long)__ballot(top == mn)) - 1;
             if (m > -INFINITY) {
@@ -137,81 +261,88 @@ __global__ void __launch_bounds__(256) score_kernel(MzScores p, int splits) {
                 S = t * f;
             }
             m = mn;
-            bool left = own;  // one element of the maximum is left out
+            const int out = own ? at : -1;  // one element of the maximum is left out
 #pragma unroll
-            for (int j = 0; j < PER_LANE; j++) {
-                const bool out = left && x[j] == mn;
-                left = left && !out;
-                if (!out) add(x[j], m, S, U);
-            }
+            for (int j = 0; j < PER_LANE; j++) add(j == out ? -INFINITY : x[j], m, S, U);
         } else {
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int j = 0; j < PER_LANE; j++) add(x[j], ref, S, U);
         }
-        if (p.alts)
-            while (__ballot(top > thr)) {
-                // the chunk's best, lowest id first, into its place of the list
-                int bi = NONE;
-#pragma unroll
-                for (int j = PER_LANE - 1; j >= 0; j--)
-                    if (x[j] == top) bi = first(c, j / V) + j % V;
-                float bv = top;
-                int id = bi;
-                wave_argmax(bv, id);
-                const int at = __popcll(__ballot(lane < p.alts && (lv > bv || (lv == bv && li < id))));
-                const float pv = dpp_f<0x111>(lv);  // the lane before
-                const int pi = dpp_i<0x111>(li);
-                if (lane < p.alts && lane >= at) {
-                    lv = lane == at ? bv : pv;
-                    li = lane == at ? id : pi;
-                }
-                thr = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lv), p.alts - 1));
-                if (bi == id) {
-                    top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < PER_LANE; j++) {
-                        if (first(c, j / V) + j % V == id) x[j] = -INFINITY;
-                        top = fmaxf(top, x[j]);
-                    }
-                }
+        if (!p.alts) continue;
+        least = max(least, *(volatile Key*)&bound);
+        if (!__ballot(top >= value_of(least) && top > -INFINITY)) continue;
+        // Elements above the list's last one are put in their places: the lanes' best ones, then the next ones of the
+        // lanes that had one.
+        find();
+        auto best = [&]() {
+            const Key k = key_of(top, from(piece(c, 0) + at / V * (64 * V)) + at % V);
+            return top > -INFINITY ? k : 0;
+        };
+        Key mine = best();
+        for (;;) {
+            const unsigned long long can = __ballot(mine > least);
+            if (!can) break;
+            bool next;  // the lane's best is in the list, or not as good as what is
+            if (p.alts > 1 && (can & (can - 1))) {
+                list = joined(list, best16(mine, lane), lane);
+                const Key last = lane_key(list, p.alts - 1);
+                next = mine && mine >= last;
+                least = max(least, last);
+            } else {
+                const int l = best_lane(mine > least ? top : -INFINITY, mine);
+                const Key in = lane_key(mine, l), before = moved<0x111>(list);
+                const int row16 = lane & 15, place = __popcll(__ballot(lane < 16 && list > in));
+                list = row16 < place ? list : row16 == place ? in : before;
+                least = max(least, lane_key(list, p.alts - 1));
+                next = lane == l;
             }
-    };
-    Raw w0, w1;
-    int c = c0 + wave;
-    if (c < c1) fetch(c, w0);
-    for (; c < c1; c += 8) {
-        if (c + 4 < c1) fetch(c + 4, w1);
-        chunk(c, w0);
-        if (c + 4 < c1) {
-            if (c + 8 < c1) fetch(c + 8, w0);
-            chunk(c + 4, w1);
+            float second = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < PER_LANE; j++) {
+                x[j] = next && j == at ? -INFINITY : x[j];
+                second = fmaxf(second, x[j]);
+            }
+            top = next ? second : top;
+            if (!__ballot(next && top >= value_of(least))) break;
+            find();
+            const Key k = best();
+            mine = next ? k : mine;
         }
+        if (lane == 0 && least > *(volatile Key*)&bound) bound = least;
     }
     S = wave_sum(S);
     U = wave_sum(U);
-    Part* part = splits > 1 ? (Part*)p.work + ((long)r * splits + split) * 4 + wave : lds + wave;
-    if (lane == 0) {
-        part->m = m;
-        part->s = S;
-        part->u = U;
+    const int words = HEAD + 2 * p.alts;
+    // lane i: word i of the wave's part
+    const float head = lane == 0 ? m : lane == 1 ? S : U;  // (and an unused word)
+    if (splits == 1) {
+        float* const part = lds + wave * words;
+        if (lane < HEAD) part[lane] = head;
+        if (lane < p.alts) *(Key*)(part + HEAD + 2 * lane) = list;
+        __syncthreads();
+    } else {
+        float* const parts = p.work + JOIN_COUNTERS + (long)r * splits * 4 * words;
+        float* const part = parts + (split * 4 + wave) * words;
+        if (lane < HEAD) shared_store(part + lane, head);
+        if (lane < p.alts)
+            shared_store(part + HEAD + 2 * lane, __builtin_bit_cast(float, (unsigned)list), __builtin_bit_cast(float, (unsigned)(list >> 32)));
+        if (!last_of((unsigned*)p.work + r, splits)) return;
+        const int all = splits * 4 * words;
+        for (int i0 = tid; i0 < all; i0 += 1024) {
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = shared_load(parts + min(i0 + 256 * k, all - 1));
+#pragma unroll
+            for (int k = 0; k < 4; k++) lds[min(i0 + 256 * k, all - 1)] = x[k];
+        }
+        __syncthreads();
     }
-    if (lane < p.alts) {
-        part->v[lane] = lv;
-        part->id[lane] = li;
-    }
-    if (splits > 1) return;
-    __syncthreads();
-    if (wave == 0) finish<T>(p, r, lds, 4, lane);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(64) score_join_kernel(MzScores p, int parts) {
-    finish<T>(p, blockIdx.x, (const Part*)p.work + (long)blockIdx.x * parts, parts, threadIdx.x);
+    if (wave == 0) finish(p, r * p.out_stride + n, lds, 4 * splits, lane, tok, left_out ? -INFINITY : xt, pick);
 }
 
 int score_splits(const MzScores& p) {
-    const long chunks = (p.vocab + CHUNK - 1) / CHUNK, want = 4L * mz_cu_count() / p.rows;
+    const long chunks = (p.vocab + CHUNK - 1) / CHUNK, want = p.rows <= JOIN_COUNTERS ? 4L * mz_cu_count() / p.rows : 1;
     return (int)std::max(1L, std::min({want, (chunks + 3) / 4, (long)PARTS / 4}));
 }
 
@@ -221,9 +352,6 @@ hipError_t launch(hipStream_t s, const MzScores& p) {
     const dim3 grid((long)p.rows * splits);
     if (p.mask) hipLaunchKernelGGL((score_kernel<T, true>), grid, dim3(256), 0, s, p, splits);
     else hipLaunchKernelGGL((score_kernel<T, false>), grid, dim3(256), 0, s, p, splits);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || splits == 1) return e;
-    hipLaunchKernelGGL(score_join_kernel<T>, dim3(p.rows), dim3(64), 0, s, p, 4 * splits);
     return hipGetLastError();
 }
 
@@ -231,7 +359,7 @@ hipError_t launch(hipStream_t s, const MzScores& p) {
 
 size_t mz_scores_work(const MzScores& p) {
     const int splits = score_splits(p);
-    return splits > 1 ? (size_t)p.rows * splits * 4 * sizeof(Part) : 0;
+    return splits > 1 ? ((size_t)p.rows * splits * 4 * (HEAD + 2 * p.alts) + JOIN_COUNTERS) * 4 : 0;
 }
 
 hipError_t mz_scores_launch(hipStream_t s, const MzScores& p) { return p.half ? launch<f16>(s, p) : launch<float>(s, p); }
