@@ -122,7 +122,7 @@ int mz_mel_transpose(mz_ctx* c, uint64_t mel, uint64_t melT, int clips, int n_me
  * capturable (no allocation, no host synchronisation). Positions, lengths and slots are read on the device, so that a
  * captured graph can be replayed while they change; one that lies outside a cache touches nothing, as stated below.
  *
- * A cache holds `slots` sequences of up to blocks * 32 positions. Each block of 32 positions x 64 channels of a (slot,
+ * A cache holds `slots` sequences of up to blocks * 32 positions (blocks < 2^20). Each block of 32 positions x 64 channels of a (slot,
  * head) has one scale for its keys and one for its values; code c stands for c * scale, with
  *   MZ_KV8_I8:   c a signed whole number, scale = f32(top / 127), c = 127 x / top to the nearest, halves to even
  *   MZ_KV8_E4M3: c an OCP e4m3 number,    scale = f32(top / 448), c = 448 x / top to the nearest, halves to even

@@ -36,11 +36,12 @@ bool aligned(uint64_t p, uint64_t n) { return p % n == 0; }
 
 // Elements of each tensor stay below this, so that no 64-bit byte offset of a kernel can wrap.
 constexpr int64_t MOST = (int64_t)1 << 46;
+constexpr int MAX_BLOCKS = (1 << 20) - 1;  // of a slot: its codes lie within 2^31 bytes, as far as a buffer descriptor reaches
 constexpr int64_t MAX_WORKGROUPS = ((int64_t)1 << 31) - 1;
 
 int check_cache(const char* who, const mz_kv8* kv, MzKv8* out) {
     if (kv->format != MZ_KV8_I8 && kv->format != MZ_KV8_E4M3) return mz_fail(MZ_ERR_ARG, "%s: bad cache format %d", who, kv->format);
-    if (kv->slots <= 0 || kv->heads <= 0 || kv->blocks <= 0 || kv->blocks > (1 << 24) ||
+    if (kv->slots <= 0 || kv->heads <= 0 || kv->blocks <= 0 || kv->blocks > MAX_BLOCKS ||
         (int64_t)kv->slots * kv->heads > MOST / MZ_KV_TILE / kv->blocks)
         return mz_fail(MZ_ERR_ARG, "%s: bad cache of %d slots, %d heads, %d blocks", who, kv->slots, kv->heads, kv->blocks);
     for (uint64_t p : {kv->k, kv->v, kv->k_open, kv->v_open})
@@ -106,6 +107,10 @@ int check_attention(const char* who, const mz_kv8* kv, const mz_kv8_attention_ar
     if ((int64_t)a->rows * std::max(a->tokens, 1) > MOST / a->heads ||
         (a->align && (int64_t)a->rows * std::max(a->tokens, 1) > MOST / a->align_heads / a->align_cols))
         return mz_fail(MZ_ERR_ARG, "%s: too large", who);
+    out->rows = a->rows;
+    out->tokens = a->tokens;
+    out->heads = a->heads;
+    if (!mz_kv8_attn_fits(*cache, *out)) return mz_fail(MZ_ERR_ARG, "%s: too large for one call", who);
     *out = {DP(const f16, a->q), DP(f16, a->out), (long)a->q_row, (long)a->q_token, (long)a->q_head, (long)a->out_row,
             (long)a->out_token, (long)a->out_head, a->rows, a->tokens, a->heads, a->causal != 0, a->scale, DP(int, a->slot),
             DP(int, a->count), DP(int, a->len), a->len_stride, a->len_add, DP(int, a->first), DP(float, a->lse),
@@ -146,7 +151,7 @@ extern "C" int mz_kv8_place(int format, int slots, int heads, int max_tokens, ui
     if (bytes) *bytes = 0;
     if (format != MZ_KV8_I8 && format != MZ_KV8_E4M3) return mz_fail(MZ_ERR_ARG, "mz_kv8_place: bad format %d", format);
     const int64_t blocks = ((int64_t)max_tokens + MZ_KV8_BLOCK - 1) / MZ_KV8_BLOCK;
-    if (slots <= 0 || heads <= 0 || max_tokens <= 0 || blocks > (1 << 24) || (int64_t)slots * heads > MOST / MZ_KV_TILE / blocks)
+    if (slots <= 0 || heads <= 0 || max_tokens <= 0 || blocks > MAX_BLOCKS || (int64_t)slots * heads > MOST / MZ_KV_TILE / blocks)
         return mz_fail(MZ_ERR_ARG, "mz_kv8_place: %d slots, %d heads, %d tokens", slots, heads, max_tokens);
     if (!aligned(base, 256)) return mz_fail(MZ_ERR_ARG, "mz_kv8_place: base must be a multiple of 256 bytes");
     const uint64_t sh = (uint64_t)slots * heads;
@@ -219,7 +224,6 @@ extern "C" int mz_kv8_attention(mz_ctx* c, const mz_kv8* kv, const mz_kv8_attent
     if (!a->rows || !a->tokens) return MZ_OK;
     OnDevice on(c->device);
     if (on.status()) return on.status();
-    if (mz_kv8_attn_grid(cache, p) > MAX_WORKGROUPS) return mz_fail(MZ_ERR_ARG, "mz_kv8_attention: too large for one call");
     if (int r = check_work("mz_kv8_attention", a->work, a->work_bytes, mz_kv8_attn_work(cache, p))) return r;
     p.work = DP(float, a->work);
     return mz_hip(mz_kv8_attn_launch(c->stream, cache, p), "mz_kv8_attention");

@@ -8,6 +8,7 @@
 namespace {
 
 enum { I8 = 0, E4M3 = 1 };
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // element of position t (of its block) and channel d in a block of values
 __device__ __forceinline__ int v_at(int t, int d) { return ((d >> 1) * 4 + (t >> 3)) * 16 + (d & 1) * 8 + (t & 7); }
@@ -339,6 +340,10 @@ __device__ __forceinline__ float column_sum(float v) {
     return pair32_sum(__builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]));
 }
 
+__device__ __forceinline__ float lane_value(float v, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
 // what a row's queries see: token i positions first .. min(base + (causal ? i : 0), cap) - 1 of its slot
 struct Seen {
     long slot, base;
@@ -369,15 +374,16 @@ __device__ __forceinline__ Seen seen_of(const MzKv8& kv, const MzKv8Attn& a, int
 
 // Alignment indices of the query heads h0 .. h0 + n - 1, by all threads of the workgroup: of heads with one index the
 // first has it. mine: head_slot[threadIdx.x], requested earlier.
+template <int THREADS>
 __device__ __forceinline__ void align_indices(const MzKv8Attn& a, int h0, int n, int mine, int (&index)[64]) {
     __shared__ int slots[64];
     const int tid = threadIdx.x;
-    for (int j = tid; j < h0 + n; j += 256) {
+    for (int j = tid; j < h0 + n; j += THREADS) {
         const int s = j == tid ? mine : a.head_slot[j];
         if (j >= h0) slots[j - h0] = index[j - h0] = s < a.align_heads ? s : -1;
     }
     __syncthreads();
-    for (int j = tid; j < h0 + n; j += 256) {
+    for (int j = tid; j < h0 + n; j += THREADS) {
         const int s = j == tid ? mine : a.head_slot[j];
         for (int k = max(0, j - h0 + 1); k < n; k++)
             if (slots[k] == s) index[k] = -1;
@@ -387,47 +393,61 @@ __device__ __forceinline__ void align_indices(const MzKv8Attn& a, int h0, int n,
 
 // Scores (in powers of two) to probabilities, by all threads of the workgroup; 0 where nothing is seen. get(p) is the score of
 // a position that is; eight of them on their way at a time.
-template <typename Get>
+template <int THREADS, typename Get>
 __device__ __forceinline__ void align_finish(float* row, int cols, int lo, int hi, float lse2, Get get) {
-    for (int p0 = threadIdx.x; p0 < cols; p0 += 2048) {
+    for (int p0 = threadIdx.x; p0 < cols; p0 += 8 * THREADS) {
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const int p = p0 + 256 * k;
+            const int p = p0 + THREADS * k;
             x[k] = -INFINITY;
             if (p < cols && p >= lo && p < hi) x[k] = get(p);
         }
 #pragma unroll
         for (int k = 0; k < 8; k++)
-            if (p0 + 256 * k < cols) row[p0 + 256 * k] = x[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[k] - lse2);
+            if (p0 + THREADS * k < cols) row[p0 + THREADS * k] = x[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[k] - lse2);
     }
 }
 
 struct Launch {
-    int qt, tiles, splits;  // queries a workgroup / 16, such tiles of a (row, cache head), workgroups the blocks are shared by
+    int qt, tiles, splits;  // queries a workgroup / 16 (where its waves take the blocks in turn), such tiles of a (row, cache head), workgroups the blocks are shared by
     int kept;               // alignment rows: scores that a workgroup keeps in LDS for each query, 0: in their rows
+    int group;                    // query heads of a cache head
+    int waves, own;               // waves of a workgroup; whether each has queries of its own
+    unsigned by_heads, by_group, by_splits;  // for dividing by the cache's heads, group and splits (see divided)
 };
+// x / d for x below 2^31 by r = min(2^32 / d, 2^32 - 1): no more than one too small before the correction (a division by a
+// number not known beforehand takes about twenty dependent instructions)
+__device__ __forceinline__ int divided(int x, int d, unsigned r) {
+    const int q = (int)__umulhi((unsigned)x, r);
+    return q + ((q + 1) * (long)d <= x);
+}
 constexpr int STATE = 66;  // floats of a query's partial state: 64 channels, maximum, sum
 
-template <int FMT, int QT, bool ALIGN>
-__global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
-    __shared__ float red[4][16][68], ms[4][16], ls[4][16];
+// NW waves, which take the blocks in turn, or, with OWN, each 16 QT queries of its own and every block (no alignment rows).
+template <int FMT, int QT, bool ALIGN, int NW, bool OWN>
+__global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
+    static_assert(!(OWN && ALIGN));
+    __shared__ float red[OWN ? 1 : NW][16][68], ms[NW][16], ls[NW][16];
     __shared__ float* als[16];
     __shared__ float lse2s[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    // workgroups of one (row, cache head) on one XCD (they share its keys and values where there are several tiles), the
-    // tiles that see most first
-    const unsigned per = 8u * n.tiles * n.splits, id = blockIdx.x, rem = id % per;
-    const long pair = (long)(id / per) * 8 + (rem & 7);
-    if (pair >= (long)a.rows * kv.heads) return;
-    const int tile = n.tiles - 1 - (int)(rem >> 3) / n.splits, split = (int)(rem >> 3) % n.splits;
-    const int r = (int)(pair / kv.heads), kh = (int)(pair - (long)r * kv.heads), grp = a.heads / kv.heads;
+    // x: (row, cache head), padded to a multiple of the XCDs, so that what shares keys and values shares an XCD; y: the tiles,
+    // those that see most first; z: the shares of the blocks
+    const int pair = blockIdx.x;
+    if (pair >= a.rows * (long)kv.heads) return;
+    const int tile = n.tiles - 1 - (int)blockIdx.y, split = blockIdx.z, grp = n.group;
+    const int r = divided(pair, kv.heads, n.by_heads), kh = pair - r * kv.heads;
     const Seen s = seen_of(kv, a, r);
-    const int q0 = tile * 16 * QT, nq = a.tokens * grp, qn = min(q0 + 16 * QT, nq);  // this tile's queries
-    if (q0 / grp >= s.count) return;  // none of its tokens is there
-    const int hi = s.end(a, min((qn - 1) / grp, s.count - 1)), lo_end = s.end(a, q0 / grp);
+    const int q0 = (OWN ? tile * NW + wave : tile) * 16 * QT, nq = a.tokens * grp, qn = min(q0 + 16 * QT, nq);  // these queries
+    if (OWN && q0 >= nq) return;
+    auto token_of = [&](int x) { return divided(x, grp, n.by_group); };
+    if (token_of(q0) >= s.count) return;  // none of its tokens is there
+    const int hi = s.end(a, min(token_of(qn - 1), s.count - 1)), lo_end = s.end(a, token_of(q0));
     const int b_lo = s.first / MZ_KV_BLK, nb = max((hi + MZ_KV_BLK - 1) / MZ_KV_BLK - b_lo, 0);
-    const int share = (nb + n.splits - 1) / n.splits, b0 = b_lo + min(split * share, nb), b1 = b_lo + min((split + 1) * share, nb);
+    // (splits is at most 256, nb below 2^20)
+    const int b0 = b_lo + (OWN || n.splits == 1 ? 0 : divided(nb * split, n.splits, n.by_splits));
+    const int b1 = b_lo + (OWN || n.splits == 1 ? nb : divided(nb * (split + 1), n.splits, n.by_splits));
 
     const long sh = s.slot * kv.heads + kh;
     const int open_word = kv.open[sh], open = s.cap ? open_word - 1 : -1;
@@ -440,17 +460,17 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
     __shared__ int index[ALIGN ? 64 : 1];
     const int mine = ALIGN && tid < a.heads ? a.head_slot[tid] : -1;
     if constexpr (ALIGN)
-        if (!n.kept) align_indices(a, kh * grp, grp, mine, index);
+        if (!n.kept) align_indices<64 * NW>(a, kh * grp, grp, mine, index);
     f16x8 qf[QT][2];
     int end[QT];
     float* al[QT];
     auto align_row = [&](int t) -> float* {
-        const int x = q0 + 16 * t + c, i = x / grp, k = x < nq && i < s.count ? index[x - i * grp] : -1;
+        const int x = q0 + 16 * t + c, i = token_of(x), k = x < nq && i < s.count ? index[x - i * grp] : -1;
         return k >= 0 ? a.align + (((long)r * a.tokens + i) * a.align_heads + k) * a.align_cols : nullptr;
     };
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        const int x = q0 + 16 * t + c, i = x / grp, h = kh * grp + x - i * grp;
+        const int x = q0 + 16 * t + c, i = token_of(x), h = kh * grp + x - i * grp;
         const bool on = x < nq && i < s.count;
         const f16* q = a.q + r * a.q_row + (on ? i * a.q_token + h * a.q_head : 0) + 16 * g;
         qf[t][0] = on ? ld8(q) : f16x8{};
@@ -459,25 +479,27 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
         al[t] = ALIGN && !n.kept ? align_row(t) : nullptr;
     }
 
-    // a coded block as it lies
+    // A coded block as it lies. Blocks past this workgroup's share read as zeros, without a memory access: the loads need no
+    // branches, around which the compiler would wait for all that is on its way.
     struct Raw {
-        uint4 k[2], v[2];
-        float ks, vs;
+        u32x4 k[2], v[2];
     };
     const unsigned ktok = 8 * (c >> 2) + (c & 3);  // row c of key tile 0; tile 1 is 4 positions on
+    const __amdgpu_buffer_rsrc_t rk = rsrc(kc + (long)b0 * MZ_KV_TILE, (b1 - b0) * MZ_KV_TILE);
+    const __amdgpu_buffer_rsrc_t rv = rsrc(vc + (long)b0 * MZ_KV_TILE, (b1 - b0) * MZ_KV_TILE);
+    const unsigned kat = ktok * 64 + 16 * g, vat = (c * 4 + g) * 16;
+    constexpr int POLICY = QT == 1 && !OWN ? 2 : 0;  // nontemporal where no other workgroup reads the same
     auto fetch = [&](int b, Raw& w) {
-        const unsigned char* k = kc + (long)b * MZ_KV_TILE;
-        const unsigned char* v = vc + (long)b * MZ_KV_TILE;
+        const unsigned o = (unsigned)(b - b0) * MZ_KV_TILE;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            w.k[j] = *(const uint4*)(k + (ktok + 4 * j) * 64 + 16 * g);
-            w.v[j] = *(const uint4*)(v + ((16 * j + c) * 4 + g) * 16);
+            w.k[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, kat + o + 256 * j, 0, POLICY);
+            w.v[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, vat + o + 1024 * j, 0, POLICY);
         }
-        w.ks = ksc[b];
-        w.vs = vsc[b];
     };
 
-    float m[QT], l[QT], unit = 0.f;  // the accumulators are in `unit`s, a power of two that no block's values' scale passes
+    float m[QT], l[QT];
+    float unit = 0.f, per_unit = 0.f;  // the accumulators are in `unit`s, a power of two that no block's values' scale passes
     f32x4 acc[QT][4];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -493,17 +515,21 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
         if (cs == 0.f) cs = 1e-37f;  // (all keys 0; what is not seen is -inf times it)
         const bool whole = b * MZ_KV_BLK >= s.first && (b + 1) * MZ_KV_BLK <= lo_end;  // seen by every query
         const bool given = b == open;  // fp16 as it was given, any number: vs is 1 and says nothing about the numbers' size
-        if (given && unit == 0.f) unit = 9.5367431640625e-07f;
-        if (!given && vs > unit) {
-            const float to = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, vs) & 0x7f800000u) + 0x00800000u), f = unit / to;
+        if (given ? unit == 0.f : vs > unit) {
+            const float to = given ? 9.5367431640625e-07f
+                                   : __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, vs) & 0x7f800000u) + 0x00800000u);
+            per_unit = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(unsigned, to));  // 1 / to
+            const float f = unit * per_unit;
 #pragma unroll
             for (int t = 0; t < QT; t++)
 #pragma unroll
                 for (int u = 0; u < 4; u++) acc[t][u] *= f;
             unit = to;
         }
-        const float part = vs == 0.f ? 0.f : vs / unit;  // P is multiplied by it, before its rounding if it is not small
+        // P is multiplied by `part`, before its rounding (in the exponent) if it is not small
+        const float part = vs * per_unit;
         const bool direct = !given && part >= 0.0078125f;
+        const float up = direct ? __builtin_amdgcn_logf(part) : 0.f, down = direct ? __builtin_amdgcn_rcpf(part) : 1.f;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             f32x4 d[2];
@@ -539,48 +565,57 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
             float x[8];
             f16x8 p;
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], cs, -m[t]));
+            for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], cs, up - m[t]));
             // (0 times a scale or a value that is no number is none: a query that does not see the block keeps its sums)
             const bool any = whole || b * MZ_KV_BLK < end[t];
             const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            l[t] += any ? sum : 0.f;
-            if (whole && direct) {
+            l[t] += any ? sum * down : 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = (f16)(x[e] * part);
+            for (int e = 0; e < 8; e++) p[e] = (f16)x[e];
+            if (whole && direct) {
 #pragma unroll
                 for (int u = 0; u < 4; u++) acc[t][u] = mfma16(vf[u], p, acc[t][u]);
             } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = (f16)x[e];
+                const float f = direct ? 1.f : part;
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const f32x4 y = mfma16(vf[u], p, f32x4{});
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[t][u][e] = any ? fmaf(y[e], part, acc[t][u][e]) : acc[t][u][e];
+                    for (int e = 0; e < 4; e++) acc[t][u][e] = any ? fmaf(y[e], f, acc[t][u][e]) : acc[t][u][e];
                 }
             }
         }
     };
-    auto coded = [&](int b, const Raw& w) {
+    auto coded = [&](int b, const Raw& w, float ks, float vs) {
         f16x8 kf[2][2], vf[4];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            kf[j][0] = widen<FMT>(w.k[j].x, w.k[j].y);
-            kf[j][1] = widen<FMT>(w.k[j].z, w.k[j].w);
-            vf[2 * j] = widen<FMT>(w.v[j].x, w.v[j].y);
-            vf[2 * j + 1] = widen<FMT>(w.v[j].z, w.v[j].w);
+            kf[j][0] = widen<FMT>(w.k[j][0], w.k[j][1]);
+            kf[j][1] = widen<FMT>(w.k[j][2], w.k[j][3]);
+            vf[2 * j] = widen<FMT>(w.v[j][0], w.v[j][1]);
+            vf[2 * j + 1] = widen<FMT>(w.v[j][2], w.v[j][3]);
         }
-        products(b, kf, vf, w.ks, w.vs);
+        products(b, kf, vf, ks, vs);
     };
-    // Blocks b0 + wave, + 4, ...: DEPTH of them on their way (no branches around the loads: past the end the last block is
-    // loaded again). The open block, where it is this wave's, comes first; its codes are stale.
-    constexpr int DEPTH = QT == 1 ? 3 : 2;
+    // Blocks b0 + wave, + 4, ...: DEPTH of them on their way. The open block, where it is this wave's, comes first; its codes
+    // are stale.
+    // The scales of 60 of them lie in the lanes of two registers: scalar loads, which come back in any order, would have
+    // every block wait for the newest of them.
+    constexpr int DEPTH = 2, WINDOW = 60, STEP = OWN ? 1 : NW;
     Raw w[DEPTH];
-    if (b0 + wave < b1) {
-        const int tail = b0 + wave + (b1 - 1 - b0 - wave) / 4 * 4;
+    const int head = b0 + (OWN ? 0 : wave);
+    if (head < b1) {
+        const int tail = head + (b1 - 1 - head) / STEP * STEP;
+        float ks, vs;
+        auto scales = [&](int b) {
+            const int at = min(b + STEP * lane, tail);
+            ks = ksc[at];
+            vs = vsc[at];
+        };
 #pragma unroll
-        for (int i = 0; i < DEPTH; i++) fetch(min(b0 + wave + 4 * i, tail), w[i]);
-        if (open >= b0 && open < b1 && ((open - b0) & 3) == wave) {
+        for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
+        scales(head);
+        if (open >= b0 && open < b1 && (open - head) % STEP == 0) {
             f16x8 kf[2][2], vf[4];
             const f16* ko = kv.k_open + sh * MZ_KV_TILE;
             const f16* vo = kv.v_open + sh * MZ_KV_TILE;
@@ -598,51 +633,73 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
                 }
             products(open, kf, vf, 1.f, 1.f);
         }
-        for (int b = b0 + wave; b <= tail; b += 4 * DEPTH) {
+        for (int b = head, at = 0; b <= tail; b += STEP * DEPTH, at += DEPTH) {
+            if (at == WINDOW) {
+                scales(b);
+                at = 0;
+            }
 #pragma unroll
             for (int i = 0; i < DEPTH; i++) {
-                const int bi = b + 4 * i;
-                if (bi <= tail && bi != open) coded(bi, w[i]);
-                fetch(min(bi + 4 * DEPTH, tail), w[i]);
+                const int bi = b + STEP * i;
+                if (bi <= tail && bi != open) coded(bi, w[i], lane_value(ks, at + i), lane_value(vs, at + i));
+                fetch(bi + STEP * DEPTH, w[i]);
             }
         }
     }
 
+    // accumulator u of lane (c, g) holds channels 32 (u / 2) + 8 g + 2 e + u % 2 of query c
+    if constexpr (OWN) {
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const int x = q0 + 16 * t + c, i = token_of(x), h = kh * grp + x - i * grp;
+            const float ll = column_sum(l[t]), f = ll == 0.f ? 0.f : unit / ll;
+            if (x >= nq || i >= s.count) continue;
+            f16* o = a.out + r * a.out_row + i * a.out_token + h * a.out_head + 8 * g;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const f32x4 y = acc[t][2 * u] * f, z = acc[t][2 * u + 1] * f;
+                *(f16x8*)(o + 32 * u) = f16x8{(f16)y[0], (f16)z[0], (f16)y[1], (f16)z[1], (f16)y[2], (f16)z[2], (f16)y[3], (f16)z[3]};
+            }
+            if (a.lse && g == 0)
+                a.lse[((long)r * a.tokens + i) * a.heads + h] = ll == 0.f ? -INFINITY : (m[t] + __builtin_amdgcn_logf(ll)) * LN2;
+        }
+        return;
+    }
     if constexpr (ALIGN)
         if (n.kept) {
-            align_indices(a, kh * grp, grp, mine, index);
+            align_indices<64 * NW>(a, kh * grp, grp, mine, index);
 #pragma unroll
             for (int t = 0; t < QT; t++) al[t] = align_row(t);
         }
-    // the four waves' states joined, 16 queries at a time; accumulator u of lane (c, g) holds channels
-    // 32 (u / 2) + 8 g + 2 e + u % 2 of query c
-    const int col = tid >> 4, d4 = (tid & 15) * 4;
+    // the waves' states joined, 16 queries at a time, by the first 256 threads
+    const int col = tid >> 4 & 15, d4 = (tid & 15) * 4;
+    const bool mine256 = NW == 4 || tid < 256;
     auto emit = [&](int t, float mm, float ll, f32x4 o) {
-        const int x = q0 + 16 * t + col, i = x / grp, h = kh * grp + x - i * grp;
+        const int x = q0 + 16 * t + col, i = token_of(x), h = kh * grp + x - i * grp;
         const float inv = ll == 0.f ? 0.f : 1.f / ll, lse2 = ll == 0.f ? -INFINITY : mm + __builtin_amdgcn_logf(ll);
-        if (x < nq && i < s.count) {
+        if (mine256 && x < nq && i < s.count) {
             st4(a.out + r * a.out_row + i * a.out_token + h * a.out_head + d4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
             if (a.lse && d4 == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
         }
         if (ALIGN) {
             if (tid < 16) als[c] = al[t];
-            if (d4 == 0) lse2s[col] = lse2;
+            if (mine256 && d4 == 0) lse2s[col] = lse2;
             __syncthreads();
             for (int k = 0; k < 16; k++) {
                 if (!als[k]) continue;
                 float* const row = als[k];
-                const int to = s.end(a, (q0 + 16 * t + k) / grp);
+                const int to = s.end(a, token_of(q0 + 16 * t + k));
                 if (n.splits > 1)
-                    align_finish(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return shared_load(row + p); });
+                    align_finish<64 * NW>(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return shared_load(row + p); });
                 else if (n.kept) {
                     const float* x = kept + (16 * t + k) * n.kept - b0 * MZ_KV_BLK;
-                    align_finish(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return x[p]; });
-                } else align_finish(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return row[p]; });
+                    align_finish<64 * NW>(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return x[p]; });
+                } else align_finish<64 * NW>(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return row[p]; });
             }
             __syncthreads();
         }
     };
-    float* const states = a.work + JOIN_COUNTERS + (pair * n.tiles + tile) * n.splits * (16 * QT) * STATE;
+    float* const states = a.work + JOIN_COUNTERS + ((long)pair * n.tiles + tile) * n.splits * (16 * QT) * STATE;
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         const float lt = column_sum(l[t]);
@@ -658,11 +715,12 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
             ls[wave][c] = lt;
         }
         __syncthreads();
-        const float mm = fmaxf(fmaxf(ms[0][col], ms[1][col]), fmaxf(ms[2][col], ms[3][col]));
-        float ll = 0.f;
+        float mm = ms[0][col], ll = 0.f;
+#pragma unroll
+        for (int k = 1; k < NW; k++) mm = fmaxf(mm, ms[k][col]);
         f32x4 o = {};
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < NW; k++) {
             const float f = __builtin_amdgcn_exp2f(ms[k][col] - mm);
             ll = fmaf(f, ls[k][col], ll);
             const f32x4 y = *(const f32x4*)&red[k][col][d4];
@@ -670,7 +728,7 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
             for (int e = 0; e < 4; e++) o[e] = fmaf(f, y[e], o[e]);
         }
         if (n.splits == 1) emit(t, mm, ll, o);
-        else if (q0 + 16 * t + col < nq) {
+        else if (mine256 && q0 + 16 * t + col < nq) {
             float* w = states + (split * (16 * QT) + 16 * t + col) * STATE;
             shared_store(w + d4, o[0], o[1]);
             shared_store(w + d4 + 2, o[2], o[3]);
@@ -681,18 +739,18 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
             __syncthreads();
             for (int k = 0; k < 16; k++)
                 if (als[k])
-                    for (int p = b0 * MZ_KV_BLK + tid; p < min(b1 * MZ_KV_BLK, a.align_cols); p += 256)
+                    for (int p = b0 * MZ_KV_BLK + tid; p < min(b1 * MZ_KV_BLK, a.align_cols); p += 64 * NW)
                         shared_store(als[k] + p, kept[(16 * t + k) * n.kept + p - b0 * MZ_KV_BLK]);
         }
         if (t + 1 < QT) __syncthreads();
     }
-    if (n.splits == 1 || !last_of((unsigned*)a.work + pair * n.tiles + tile, n.splits)) return;
+    if (n.splits == 1 || !last_of((unsigned*)a.work + (long)pair * n.tiles + tile, n.splits)) return;
     // the last of the workgroups that share these queries joins their states
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         float mm = NOTHING, ll = 0.f;
         f32x4 o = {};
-        if (q0 + 16 * t + col < nq)
+        if (mine256 && q0 + 16 * t + col < nq)
             for (int k0 = 0; k0 < n.splits; k0 += 4) {
                 float2 x[4][3];
 #pragma unroll
@@ -720,18 +778,35 @@ __global__ void __launch_bounds__(256, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, Mz
 constexpr long KEPT_FLOATS = 8192;
 long kept_queries(const Launch& n, long nq) { return std::min(nq, 16L * n.qt); }
 
-// 16 queries a wave where there are no more, else 32 (224-token prompts of 8 rows, 20 heads: 19.4 us with 16 a workgroup, 16.6
-// with 32, 22.9 with 64). The blocks are shared by more workgroups where there are fewer units than CUs, until there
-// are two a CU or a wave has two blocks left: 1500 positions of one row, 20 heads, 10.8 us with one workgroup each, 7.8 with
-// 4 to 6, 8.8 with 11; 16,000 positions of 96 (row, head) pairs 34.1 with 2, 18.7 with 5, 19.1 with 10; 256 pairs 12.9 with
-// one, 14.2 with 2; 640 pairs 28.0 and 30.6.
+// Measured, us, 20 heads unless stated; a unit is a tile of a (row, cache head).
+// Up to 16 queries: a tile of 16, and no more units than CUs: eight waves each instead of four (1500 positions, 160 units
+// 11.2 / 13.1, five beams of 256 units 12.1 / 13.7, but 260 units 16.8 / 15.9, 640 units 26.1 / 24.8), and with fewer
+// than half as many, the blocks shared by more workgroups until there is one a CU or a wave has about a block left (1500
+// positions of one row 10.6 with one workgroup, 8.8 with 2, 7.9 with 4, 8.2 with 6; 80 units 10.1, 9.4 with 2, 10.3 with 4;
+// 16,000 positions of 48 units 53 with one, 18.9 with 5, 20.6 with 8).
+// More queries: each wave 16 of its own, where that gives every CU a workgroup (40-token prompts of 8 rows 7.8, the waves taking
+// blocks in turn 8.9; 224 tokens 15.6 / 16.7), else tiles of 32 whose waves take the blocks in turn (224 tokens of one row
+// 8.3 / 10.7, of 3 rows 9.9 / 11.2).
 Launch attn_shape(const MzKv8& kv, const MzKv8Attn& a) {
-    const long nq = (long)a.tokens * (a.heads / kv.heads), cus = mz_cu_count();
-    Launch n;
+    const long nq = (long)a.tokens * (a.heads / kv.heads), cus = mz_cu_count(), pairs = (long)a.rows * kv.heads;
+    auto inverse = [](int d) { return (unsigned)std::min((1ULL << 32) / d, 0xffffffffULL); };
+    Launch n{};
+    n.group = a.heads / kv.heads;
+    n.by_heads = inverse(kv.heads);
+    n.by_group = inverse(n.group);
+    n.waves = 4;
+    n.splits = 1;
+    n.own = !a.align && nq > 16 && pairs * ((nq + 63) / 64) >= cus;
+    if (n.own) {
+        n.tiles = (int)((nq + 63) / 64);
+        return n;
+    }
     n.qt = nq <= 16 ? 1 : 2;
     n.tiles = (int)((nq + 16 * n.qt - 1) / (16 * n.qt));
-    const long units = (long)a.rows * kv.heads * n.tiles, want = units < cus ? 2 * cus / units : 1;
-    n.splits = (int)std::max(1L, std::min(want, (long)kv.blocks / 8));
+    const long units = pairs * n.tiles;
+    if (units <= cus && n.qt == 1) n.waves = 8;
+    n.splits = (int)std::max(1L, std::min({cus / units, (long)kv.blocks / 10, 256L}));
+    n.by_splits = inverse(n.splits);
     const long keep = ((long)kv.blocks + n.splits - 1) / n.splits * MZ_KV_BLK;
     n.kept = a.align && keep * kept_queries(n, nq) <= KEPT_FLOATS ? (int)keep : 0;
     return n;
@@ -739,19 +814,26 @@ Launch attn_shape(const MzKv8& kv, const MzKv8Attn& a) {
 static_assert(JOIN_COUNTERS >= 1024, "units that are shared have a counter each: fewer than the CUs");
 
 template <int FMT, bool ALIGN>
-void attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a, const Launch& n, long grid) {
-    const size_t lds = (size_t)n.kept * kept_queries(n, (long)a.tokens * (a.heads / kv.heads)) * 4;
-    if (n.qt == 1) hipLaunchKernelGGL((attn_kernel<FMT, 1, ALIGN>), dim3(grid), dim3(256), lds, s, kv, a, n);
-    else hipLaunchKernelGGL((attn_kernel<FMT, 2, ALIGN>), dim3(grid), dim3(256), lds, s, kv, a, n);
+void attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a, const Launch& n) {
+    const size_t lds = (size_t)n.kept * kept_queries(n, (long)a.tokens * n.group) * 4;
+    const dim3 grid(((long)a.rows * kv.heads + 7) / 8 * 8, n.tiles, n.splits);
+    if constexpr (!ALIGN)
+        if (n.own) {
+            hipLaunchKernelGGL((attn_kernel<FMT, 1, false, 4, true>), grid, dim3(256), 0, s, kv, a, n);
+            return;
+        }
+    if (n.qt == 2) hipLaunchKernelGGL((attn_kernel<FMT, 2, ALIGN, 4, false>), grid, dim3(256), lds, s, kv, a, n);
+    else if (n.waves == 4) hipLaunchKernelGGL((attn_kernel<FMT, 1, ALIGN, 4, false>), grid, dim3(256), lds, s, kv, a, n);
+    else hipLaunchKernelGGL((attn_kernel<FMT, 1, ALIGN, 8, false>), grid, dim3(512), lds, s, kv, a, n);
 }
 
 }  // namespace
 
 long mz_kv8_write_grid(const MzKv8& kv, const MzKv8Io& a) { return (long)a.rows * kv.heads * write_groups(a.tokens); }
 long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a) { return ((long)a.rows * kv.heads * spanned(a.tokens) * 2 + 3) / 4; }
-long mz_kv8_attn_grid(const MzKv8& kv, const MzKv8Attn& a) {
-    const Launch n = attn_shape(kv, a);
-    return ((long)a.rows * kv.heads + 7) / 8 * 8 * n.tiles * n.splits;
+bool mz_kv8_attn_fits(const MzKv8& kv, const MzKv8Attn& a) {
+    const long nq = (long)a.tokens * (a.heads / kv.heads);
+    return (long)a.rows * kv.heads < 1L << 24 && nq <= 32L * 65535;
 }
 
 size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a) {
@@ -778,8 +860,7 @@ hipError_t mz_kv8_read_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) 
 
 hipError_t mz_kv8_attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a) {
     const Launch n = attn_shape(kv, a);
-    const long grid = mz_kv8_attn_grid(kv, a);
-    if (kv.format == I8) a.align ? attn_launch<I8, true>(s, kv, a, n, grid) : attn_launch<I8, false>(s, kv, a, n, grid);
-    else a.align ? attn_launch<E4M3, true>(s, kv, a, n, grid) : attn_launch<E4M3, false>(s, kv, a, n, grid);
+    if (kv.format == I8) a.align ? attn_launch<I8, true>(s, kv, a, n) : attn_launch<I8, false>(s, kv, a, n);
+    else a.align ? attn_launch<E4M3, true>(s, kv, a, n) : attn_launch<E4M3, false>(s, kv, a, n);
     return hipGetLastError();
 }

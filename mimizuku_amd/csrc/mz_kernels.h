@@ -294,7 +294,8 @@ struct MzKv8Attn {
     int align_heads, align_cols;
     float* work;
 };
-long mz_kv8_attn_grid(const MzKv8& kv, const MzKv8Attn& a);
+// whether one launch takes it: rows x cache heads below 2^24, tokens x query heads of each at most 32 x 65535
+bool mz_kv8_attn_fits(const MzKv8& kv, const MzKv8Attn& a);
 size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a);
 hipError_t mz_kv8_attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a);
 
