@@ -37,7 +37,7 @@ bool aligned(uint64_t p, uint64_t n) { return p % n == 0; }
 // Elements of each tensor stay below this, so that no 64-bit byte offset of a kernel can wrap.
 constexpr int64_t MOST = (int64_t)1 << 46;
 constexpr int MAX_BLOCKS = (1 << 20) - 1;  // of a slot: its codes lie within 2^31 bytes, as far as a buffer descriptor reaches
-constexpr int64_t MAX_WORKGROUPS = ((int64_t)1 << 31) - 1;
+constexpr int64_t MAX_WORKGROUPS = ((int64_t)1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32 along x
 
 int check_cache(const char* who, const mz_kv8* kv, MzKv8* out) {
     if (kv->format != MZ_KV8_I8 && kv->format != MZ_KV8_E4M3) return mz_fail(MZ_ERR_ARG, "%s: bad cache format %d", who, kv->format);
@@ -120,7 +120,7 @@ int check_attention(const char* who, const mz_kv8* kv, const mz_kv8_attention_ar
 
 int check_scores(const char* who, const mz_score_args* a, MzScores* out) {
     if (a->dtype != MZ_DT_F16 && a->dtype != MZ_DT_F32) return mz_fail(MZ_ERR_ARG, "%s: bad dtype %d", who, a->dtype);
-    if (a->rows < 0 || a->vocab <= 0 || a->vocab > (1 << 30) || a->ld < a->vocab || a->ld > MOST / std::max(a->rows, 1))
+    if (a->rows < 0 || a->rows > MAX_WORKGROUPS || a->vocab <= 0 || a->vocab > (1 << 30) || a->ld < a->vocab || a->ld > MOST / std::max(a->rows, 1))
         return mz_fail(MZ_ERR_ARG, "%s: %d rows of %d logits, ld %lld", who, a->rows, a->vocab, (long long)a->ld);
     if (a->alts < 0 || a->alts > MZ_SCORE_ALTS) return mz_fail(MZ_ERR_ARG, "%s: %d alternatives (0 .. %d)", who, a->alts, MZ_SCORE_ALTS);
     if (!a->logits || !aligned(a->logits, a->dtype == MZ_DT_F32 ? 4 : 2))
@@ -182,7 +182,7 @@ extern "C" int mz_kv8_write(mz_ctx* c, const mz_kv8* kv, const mz_kv8_io* a) {
     if (int r = check_io("mz_kv8_write", kv, a, &io)) return r;
     if (!a->rows || !a->tokens) return MZ_OK;
     if (!a->k || !a->v) return mz_fail(MZ_ERR_ARG, "mz_kv8_write: null k or v");
-    if (mz_kv8_write_grid(cache, io) > MAX_WORKGROUPS) return mz_fail(MZ_ERR_ARG, "mz_kv8_write: too large for one call");
+    if (!mz_kv8_write_fits(cache, io)) return mz_fail(MZ_ERR_ARG, "mz_kv8_write: too large for one call");
     OnDevice on(c->device);
     if (on.status()) return on.status();
     return mz_hip(mz_kv8_write_launch(c->stream, cache, io), "mz_kv8_write");

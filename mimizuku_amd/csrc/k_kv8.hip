@@ -8,6 +8,7 @@
 namespace {
 
 enum { I8 = 0, E4M3 = 1 };
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // element of position t (of its block) and channel d in a block of values
@@ -96,9 +97,16 @@ struct Row {
     int p, n;
 };
 __device__ __forceinline__ bool row_of(const MzKv8& kv, const MzKv8Io& a, int r, Row& o) {
-    o.slot = a.slot ? a.slot[r] : r;
-    const long p = (long)a.pos_add + (a.pos ? a.pos[(long)r * a.pos_stride] : 0);
-    o.n = a.count ? min(max(a.count[r], 0), a.tokens) : a.tokens;
+    // (if any array is there all are read, an absent one's place being some other word: the loads go out together)
+    int slot = 0, pos = 0, count = 0;
+    if (a.slot || a.pos || a.count) {
+        slot = *(a.slot ? a.slot + r : kv.open);
+        pos = *(a.pos ? a.pos + (long)r * a.pos_stride : kv.open);
+        count = *(a.count ? a.count + r : kv.open);
+    }
+    o.slot = a.slot ? slot : r;
+    const long p = (long)a.pos_add + (a.pos ? pos : 0);
+    o.n = a.count ? min(max(count, 0), a.tokens) : a.tokens;
     o.p = (int)p;
     return o.n > 0 && o.slot >= 0 && o.slot < kv.slots && p >= 0 && p < (long)kv.blocks * MZ_KV_BLK;
 }
@@ -119,6 +127,34 @@ struct Writer {
     int off, end;
     bool full, old;
     f16x8 x[4] = {};  // keys: position lane / 8 + 8 i; values: channel 4 c + i, positions 8 g .. 8 g + 7
+
+    // a block all of whose positions are new
+    __device__ __forceinline__ void fetch(int b, u32x4 (&raw)[4]) const {
+        const f16* s = src + (long)(b * MZ_KV_BLK - p) * a.token_stride;
+        if (side == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                raw[i] = __builtin_nontemporal_load((const u32x4*)(s + ((lane >> 3) + 8 * i) * a.token_stride + (lane & 7) * 8));
+        else
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const u32x2 y = __builtin_nontemporal_load((const u32x2*)(s + ((lane >> 4) * 8 + j) * a.token_stride + (lane & 15) * 4));
+                raw[j >> 1][(j & 1) * 2] = y[0];
+                raw[j >> 1][(j & 1) * 2 + 1] = y[1];
+            }
+    }
+    __device__ __forceinline__ void take(const u32x4 (&raw)[4]) {
+        if (side == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = __builtin_bit_cast(f16x8, raw[i]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const f16x4 y = __builtin_bit_cast(f16x4, u32x2{raw[j >> 1][(j & 1) * 2], raw[j >> 1][(j & 1) * 2 + 1]});
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e][j] = y[e];
+            }
+    }
 
     __device__ __forceinline__ void load(int b) {
         off = max(p - b * MZ_KV_BLK, 0);
@@ -172,33 +208,37 @@ struct Writer {
         }
     }
 
-    __device__ __forceinline__ void store(int b) {
+    __device__ __forceinline__ void code(int b) const {
         const long blk = sh * kv.blocks + b;
+        u16x2 m = {};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 u = __builtin_bit_cast(uint4, x[i]);
+            m = larger(larger(larger(larger(m, u.x), u.y), u.z), u.w);
+        }
+        float top, rc;
+        const float scale = block_scale<FMT>(m, top, rc);
+        uint2 c[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            c[i] = uint2{codes4<FMT>(x[i][0], x[i][1], x[i][2], x[i][3], top, rc), codes4<FMT>(x[i][4], x[i][5], x[i][6], x[i][7], top, rc)};
+            if (top == 0.f) c[i] = uint2{0, 0};
+        }
+        if (side == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) *(uint2*)(kv.k + blk * MZ_KV_TILE + lane * 8 + 512 * i) = c[i];
+            if (lane == 0) kv.k_scale[blk] = scale;
+        } else {
+            unsigned char* v = kv.v + blk * MZ_KV_TILE + (lane & 15) * 128 + (lane >> 4) * 16;
+            *(uint4*)v = uint4{c[0].x, c[0].y, c[1].x, c[1].y};
+            *(uint4*)(v + 64) = uint4{c[2].x, c[2].y, c[3].x, c[3].y};
+            if (lane == 0) kv.v_scale[blk] = scale;
+        }
+    }
+
+    __device__ __forceinline__ void store(int b) const {
         if (full) {
-            u16x2 m = {};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint4 u = __builtin_bit_cast(uint4, x[i]);
-                m = larger(larger(larger(larger(m, u.x), u.y), u.z), u.w);
-            }
-            float top, rc;
-            const float scale = block_scale<FMT>(m, top, rc);
-            uint2 c[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                c[i] = uint2{codes4<FMT>(x[i][0], x[i][1], x[i][2], x[i][3], top, rc), codes4<FMT>(x[i][4], x[i][5], x[i][6], x[i][7], top, rc)};
-                if (top == 0.f) c[i] = uint2{0, 0};
-            }
-            if (side == 0) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) *(uint2*)(kv.k + blk * MZ_KV_TILE + lane * 8 + 512 * i) = c[i];
-                if (lane == 0) kv.k_scale[blk] = scale;
-            } else {
-                unsigned char* v = kv.v + blk * MZ_KV_TILE + (lane & 15) * 128 + (lane >> 4) * 16;
-                *(uint4*)v = uint4{c[0].x, c[0].y, c[1].x, c[1].y};
-                *(uint4*)(v + 64) = uint4{c[2].x, c[2].y, c[3].x, c[3].y};
-                if (lane == 0) kv.v_scale[blk] = scale;
-            }
+            code(b);
             return;
         }
         const int lo = old ? 0 : off;
@@ -220,28 +260,41 @@ struct Writer {
     }
 };
 
-// Workgroup 0 of a (row, head) takes its first and its last block, which may want the open block and may leave one; the
-// others two of those between each. Waves: keys and values of the one, keys and values of the other.
+// Workgroup 0 of a (row, head) takes its first and its last block, which may want the open block and may leave one: a wave
+// for the keys and one for the values of each. The others take the blocks between, 2 * per each, whose positions are all new:
+// every wave `per` of keys or of values, the next one's on their way while one is coded.
 template <int FMT>
-__global__ void __launch_bounds__(256) write_kernel(MzKv8 kv, MzKv8Io a, int groups) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = blockIdx.x % groups;
-    const int rh = blockIdx.x / groups, r = rh / kv.heads, h = rh - r * kv.heads;
+__global__ void __launch_bounds__(256) write_kernel(MzKv8 kv, MzKv8Io a, int per) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = blockIdx.x;
+    const int r = blockIdx.z, h = blockIdx.y;
     Row w;
     if (!row_of(kv, a, r, w) || w.p + (long)w.n > (long)kv.blocks * MZ_KV_BLK) return;
     const int first = w.p / MZ_KV_BLK, last = (w.p + w.n - 1) / MZ_KV_BLK;
-    const int b = grp ? first + 2 * grp - 1 + (wave >> 1) : wave < 2 ? first : last;
-    if (grp && first + 2 * grp - 1 >= last) return;
+    if (grp && first + 1 + 2 * per * (grp - 1) >= last) return;
     if (a.slot)  // the last row of a slot counts
         for (int i = r + 1; i < a.rows; i += 64)
             if (__ballot(i + lane < a.rows && a.slot[i + lane < a.rows ? i + lane : i] == w.slot)) return;
     const long sh = w.slot * kv.heads + h;
     const int side = wave & 1;
     Writer<FMT> x{kv, a, sh, (side ? a.v : a.k) + r * a.row_stride + h * a.head_stride, side, lane, w.p, w.n, grp ? -1 : kv.open[sh] - 1};
-    const bool mine = grp ? b < last : wave < 2 || last > first;
+    if (grp) {
+        const int end = min(first + 1 + 2 * per * grp, last);
+        int b = first + 1 + 2 * per * (grp - 1) + (wave >> 1);
+        u32x4 raw[4];
+        if (b < end) x.fetch(b, raw);
+        for (; b < end; b += 2) {
+            x.take(raw);
+            if (b + 2 < end) x.fetch(b + 2, raw);
+            x.code(b);
+        }
+        return;
+    }
+    const int b = wave < 2 ? first : last;
+    const bool mine = wave < 2 || last > first;
     if (mine) x.load(b);
-    if (grp == 0) __syncthreads();  // the open block is read before it is written
+    __syncthreads();  // the open block is read before it is written
     if (mine) x.store(b);
-    if (grp == 0 && threadIdx.x == 0) kv.open[sh] = (w.p + w.n) % MZ_KV_BLK ? last + 1 : 0;
+    if (threadIdx.x == 0) kv.open[sh] = (w.p + w.n) % MZ_KV_BLK ? last + 1 : 0;
 }
 
 // a wave: one side of one block of a (row, head)
@@ -305,8 +358,13 @@ __global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a, int bloc
 
 // the most blocks that `tokens` positions of a row can lie in
 long spanned(int tokens) { return ((long)tokens + MZ_KV_BLK - 2) / MZ_KV_BLK + 1; }
-// workgroups of a (row, head): the first and the last block, and two of the others each
-long write_groups(int tokens) { return 1 + std::max(0L, spanned(tokens) - 1) / 2; }
+// Blocks between the first and the last that a wave takes (write_kernel): two where that leaves every CU four workgroups (8 x
+// 1500 positions of 20 heads 19.8 us, 25.8 with one, 22.0 with four; 32 x 224 positions 15.6 / 22.5 / 16.2; but 1500 positions
+// of one row 6.8 / 6.5 / 8.3).
+int write_per(const MzKv8& kv, const MzKv8Io& a) {
+    return (long)a.rows * kv.heads * std::max(0L, spanned(a.tokens) - 2) >= 16L * mz_cu_count() ? 2 : 1;
+}
+long write_groups(int tokens, int per) { return 1 + (std::max(0L, spanned(tokens) - 2) + 2 * per - 1) / (2 * per); }
 
 // ---------------------------------------------------------------- attention
 //
@@ -410,10 +468,10 @@ __device__ __forceinline__ void align_finish(float* row, int cols, int lo, int h
 }
 
 struct Launch {
-    int qt, tiles, splits;  // queries a workgroup / 16 (where its waves take the blocks in turn), such tiles of a (row, cache head), workgroups the blocks are shared by
+    int qt, tiles, splits;  // queries of a workgroup / 16, such tiles of a (row, cache head), workgroups that share the blocks
+    int waves, own;         // waves of a workgroup; whether each has 16 queries of its own (qt is not used then)
     int kept;               // alignment rows: scores that a workgroup keeps in LDS for each query, 0: in their rows
-    int group;                    // query heads of a cache head
-    int waves, own;               // waves of a workgroup; whether each has queries of its own
+    int group;              // query heads of a cache head
     unsigned by_heads, by_group, by_splits;  // for dividing by the cache's heads, group and splits (see divided)
 };
 // x / d for x below 2^31 by r = min(2^32 / d, 2^32 - 1): no more than one too small before the correction (a division by a
@@ -829,11 +887,12 @@ void attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a, const Launc
 
 }  // namespace
 
-long mz_kv8_write_grid(const MzKv8& kv, const MzKv8Io& a) { return (long)a.rows * kv.heads * write_groups(a.tokens); }
+// (a launch has fewer than 2^32 threads along x, and 2^16 workgroups along y and z)
+bool mz_kv8_write_fits(const MzKv8& kv, const MzKv8Io& a) { return a.rows <= 65535 && kv.heads <= 65535; }
 long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a) { return ((long)a.rows * kv.heads * spanned(a.tokens) * 2 + 3) / 4; }
 bool mz_kv8_attn_fits(const MzKv8& kv, const MzKv8Attn& a) {
     const long nq = (long)a.tokens * (a.heads / kv.heads);
-    return (long)a.rows * kv.heads < 1L << 24 && nq <= 32L * 65535;
+    return (long)a.rows * kv.heads < (1L << 23) - 8 && nq <= 16L * 65535;
 }
 
 size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a) {
@@ -842,10 +901,10 @@ size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a) {
 }
 
 hipError_t mz_kv8_write_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) {
-    const dim3 grid(mz_kv8_write_grid(kv, a)), block(a.tokens == 1 ? 128 : 256);  // (one token: one block)
-    const int groups = (int)write_groups(a.tokens);
-    if (kv.format == I8) hipLaunchKernelGGL(write_kernel<I8>, grid, block, 0, s, kv, a, groups);
-    else hipLaunchKernelGGL(write_kernel<E4M3>, grid, block, 0, s, kv, a, groups);
+    const int per = write_per(kv, a);
+    const dim3 grid(write_groups(a.tokens, per), kv.heads, a.rows), block(a.tokens == 1 ? 128 : 256);  // (one token: one block)
+    if (kv.format == I8) hipLaunchKernelGGL(write_kernel<I8>, grid, block, 0, s, kv, a, per);
+    else hipLaunchKernelGGL(write_kernel<E4M3>, grid, block, 0, s, kv, a, per);
     return hipGetLastError();
 }
 

@@ -273,8 +273,9 @@ struct MzKv8Io {
     int pos_stride, pos_add;
     const int* count;
 };
-// workgroups of a launch; the caller keeps them below 2^31
-long mz_kv8_write_grid(const MzKv8& kv, const MzKv8Io& a);
+// whether one launch takes it: rows and heads at most 65535
+bool mz_kv8_write_fits(const MzKv8& kv, const MzKv8Io& a);
+// workgroups of 256 threads of a launch; the caller keeps them below 2^24
 long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a);
 hipError_t mz_kv8_write_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a);
 hipError_t mz_kv8_read_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a);
@@ -294,7 +295,7 @@ struct MzKv8Attn {
     int align_heads, align_cols;
     float* work;
 };
-// whether one launch takes it: rows x cache heads below 2^24, tokens x query heads of each at most 32 x 65535
+// whether one launch takes it: rows x cache heads below 2^23 - 8, tokens x query heads of each at most 16 x 65535
 bool mz_kv8_attn_fits(const MzKv8& kv, const MzKv8Attn& a);
 size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a);
 hipError_t mz_kv8_attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a);

@@ -89,6 +89,8 @@ def test_write_and_read_refuse(fn):
     for args in ((None, 1, 1), (1, None, 1), (1, 1, None)):
         ctx, kv, a = (x and y for x, y in zip(args, (C.byref(NOBODY), C.byref(place()[0]), C.byref(L.Kv8Io(**IO)))))
         assert getattr(L.lib(), fn)(ctx, kv, a) == 2
+    with pytest.raises(L.MzError, match="too large"):
+        io_call(fn, dict(slots=1 << 24), rows=1 << 24)
     # nothing to do is no error
     io_call(fn, rows=0)
     io_call(fn, tokens=0)
@@ -132,7 +134,7 @@ def test_attention_refuses(fn):
                 dict(out_row=0), dict(out_head=32), dict(out_token=64, tokens=2, out_row=4096),
                 dict(align=SOME), dict(align=SOME, head_slot=SOME, align_heads=0, align_cols=4),
                 dict(align=SOME, head_slot=SOME, align_heads=2, align_cols=0), dict(align=SOME + 1),
-                dict(out_row=1 << 47), dict(tokens=1 << 30, rows=1 << 30)):
+                dict(out_row=1 << 47), dict(tokens=1 << 30, rows=1 << 30), dict(rows=1 << 21), dict(tokens=1 << 20)):
         with pytest.raises(L.MzError, match=fn):
             att_call(None, fn, **bad)
     att_call(None, fn, rows=0)
@@ -147,7 +149,7 @@ SC = dict(dtype=L.DT_F32, rows=2, vocab=100, alts=3, logits=SOME, ld=100, tokens
                                  dict(logits=0), dict(logits=SOME + 2), dict(dtype=L.DT_F16, logits=SOME + 1),
                                  dict(tokens=0), dict(tokens=SOME + 2), dict(out_stride=0), dict(token_stride=-1),
                                  dict(logp=SOME + 1), dict(entropy=SOME + 2), dict(alt_ids=SOME + 1), dict(at=SOME + 1),
-                                 dict(alt_logp=SOME + 3), dict(ld=1 << 50), dict(vocab=(1 << 30) + 1, ld=1 << 31)])
+                                 dict(rows=1 << 24), dict(alt_logp=SOME + 3), dict(ld=1 << 50), dict(vocab=(1 << 30) + 1, ld=1 << 31)])
 def test_scores_refuse(bad):
     a = L.ScoreArgs(**{**SC, **bad})
     n = C.c_size_t()

@@ -142,6 +142,20 @@ def test_write_in_pieces_is_write_at_once(ctx, dev, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("rows,heads,tokens", [(24, 20, 500), (3, 20, 333)])
+def test_write_of_many_blocks(ctx, dev, fmt, rows, heads, tokens):
+    """Rows at every place of a block, with one block a wave and with two; read back whole."""
+    rng = np.random.default_rng(tokens)
+    b = Both(ctx, rows, heads, 640, fmt)
+    pos, cnt = [(11 * r) % 35 for r in range(rows)], [tokens - 17 * (r % 7) for r in range(rows)]
+    b.end = pos
+    b.write(dev, *(f16(rng, (rows, 35, heads, 64)) for _ in "kv"), count=pos)
+    b.end = [p + c for p, c in zip(pos, cnt)]
+    b.write(dev, *(f16(rng, (rows, tokens, heads, 64)) for _ in "kv"), pos=pos, count=cnt)
+    b.check().free()
+
+
+@pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("back", [5, 32, 33, 50, 63, 64, 70])
 def test_write_behind_the_end_opens_a_block_again(ctx, dev, fmt, back):
     rng = np.random.default_rng(back)
@@ -500,6 +514,38 @@ def test_alignment_rows(ctx, dev, fmt, tokens, heads, kvh, cols):
     for causal in (False, True):
         got = run_attention(ctx, dev, b, q, causal, length, first=first, count=cnt, head_slot=head_slot, align_heads=3, align_cols=cols)
         check_attention(b, q, got, causal, length, first=first, count=cnt, head_slot=head_slot)
+    b.free()
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("rows,heads,tokens", [(10, 16, 5), (3, 7, 1), (20, 16, 1), (17, 16, 3)])
+def test_alignment_rows_of_long_caches(ctx, dev, fmt, rows, heads, tokens):
+    """The encoder's 1500 positions: scores kept by a workgroup (the most that are), by several that share a row, by
+    workgroups of four and of eight waves."""
+    rng = np.random.default_rng(rows)
+    lens = [1500 - 7 * (r % 5) for r in range(rows)]
+    b = filled(ctx, dev, rng, rows, heads, lens, fmt)
+    q = f16(rng, (rows, tokens, heads, 64), 1.5)
+    head_slot = [(5 * h) % heads if h % 3 == 0 else -1 for h in range(heads)]
+    n = max(head_slot) + 1
+    got = run_attention(ctx, dev, b, q, False, lens, head_slot=head_slot, align_heads=n, align_cols=1500)
+    check_attention(b, q, got, False, lens, head_slot=head_slot)
+    b.free()
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("rows,heads,kvh,tokens", [(16, 16, 16, 17), (13, 20, 20, 40), (16, 32, 16, 33), (17, 16, 16, 1),
+                                                   (4, 8, 4, 130)])
+def test_attention_of_many_rows(ctx, dev, fmt, rows, heads, kvh, tokens):
+    """Workgroups enough for every CU: queries of a wave's own (more than 16 of a cache head), or four waves a tile."""
+    rng = np.random.default_rng(rows + tokens)
+    past = [(13 * r) % 60 for r in range(rows)]
+    cnt = [max(1, tokens - r % 4) for r in range(rows)]
+    b = filled(ctx, dev, rng, rows, kvh, [p + c for p, c in zip(past, cnt)], fmt, cap=200)
+    q = f16(rng, (rows, tokens, heads, 64), 1.5)
+    length, first = [p + 1 for p in past], [r % 3 for r in range(rows)]
+    for causal in (True, False):
+        check_attention(b, q, run_attention(ctx, dev, b, q, causal, length, first=first, count=cnt), causal, length, first=first, count=cnt)
     b.free()
 
 
