@@ -380,9 +380,11 @@ long write_groups(int tokens, int per) { return 1 + (std::max(0L, spanned(tokens
 //
 // Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' (as a
 // multiple of the state's unit, a power of two above every scale so far) into P before its rounding, or, where it is
-// below 2^-7 of the unit, into the block's product after it. P is rounded to fp16 (half a step 2^-11 relative, as the output's own rounding); it is
-// at most 2^8, because the maximum of a state is moved only when a score passes it by more than 8 (in powers of two): most
-// blocks need no exchange between lanes and no rescaling.
+// below 2^-7 of the unit, into the block's product after it. With up to 16 queries, where the kernel waits for memory, P goes
+// into its product as the sum of two fp16 numbers (22 bits: the error is the output's own rounding; 32 rows of 1500 27.4 us
+// with one, 27.9 with two). With more it is rounded to one, half a step 2^-11 relative, as the output is (prompts of 224
+// tokens 16.0 us, 19.5 with two). P is at most 2^8: the maximum of a state is moved only when a score passes it by more than
+// 8 (in powers of two), so that most blocks need no exchange between lanes and no rescaling.
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
 
@@ -567,6 +569,9 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
         for (int u = 0; u < 4; u++) acc[t][u] = f32x4{};
     }
     const float scale2 = a.scale * LOG2E;
+    // P as one fp16 number, or as the sum of two where the products wait for memory anyway
+    constexpr bool FINE = QT == 1 && !OWN;
+    auto weighted = [&](f16x8 v, f16x8 p, f16x8 rest, f32x4 to) { return mfma16(v, p, FINE ? mfma16(v, rest, to) : to); };
     auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], float ks, float vs) {
         const int p0 = b * MZ_KV_BLK + 8 * g;  // this lane's positions
         float cs = scale2 * ks;
@@ -628,16 +633,21 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             const bool any = whole || b * MZ_KV_BLK < end[t];
             const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             l[t] += any ? sum * down : 0.f;
+            f16x8 rest = {};
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[e] = (f16)x[e];
+            for (int e = 0; e < 8; e++) {
+                const float hi = FINE ? __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x[e]) & 0xffffe000u) : x[e];
+                p[e] = (f16)hi;
+                if (FINE) rest[e] = (f16)(x[e] - hi);
+            }
             if (whole && direct) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) acc[t][u] = mfma16(vf[u], p, acc[t][u]);
+                for (int u = 0; u < 4; u++) acc[t][u] = weighted(vf[u], p, rest, acc[t][u]);
             } else {
                 const float f = direct ? 1.f : part;
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                    const f32x4 y = mfma16(vf[u], p, f32x4{});
+                    const f32x4 y = weighted(vf[u], p, rest, f32x4{});
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[t][u][e] = any ? fmaf(y[e], f, acc[t][u][e]) : acc[t][u][e];
                 }
