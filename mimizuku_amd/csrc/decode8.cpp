@@ -37,7 +37,7 @@ bool aligned(uint64_t p, uint64_t n) { return p % n == 0; }
 // Elements of each tensor stay below this, so that no 64-bit byte offset of a kernel can wrap.
 constexpr int64_t MOST = (int64_t)1 << 46;
 constexpr int MAX_BLOCKS = (1 << 20) - 1;  // of a slot: its codes lie within 2^31 bytes, as far as a buffer descriptor reaches
-constexpr int64_t MAX_WORKGROUPS = ((int64_t)1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32 along x
+constexpr int MAX_SCORE_ROWS = (1 << 24) - 1;  // a workgroup of 256 threads each: a launch has fewer than 2^32 along x
 
 int check_cache(const char* who, const mz_kv8* kv, MzKv8* out) {
     if (kv->format != MZ_KV8_I8 && kv->format != MZ_KV8_E4M3) return mz_fail(MZ_ERR_ARG, "%s: bad cache format %d", who, kv->format);
@@ -73,7 +73,7 @@ bool apart(const int64_t (&stride)[3], const int64_t (&n)[3]) {
     return true;
 }
 
-int check_io(const char* who, const mz_kv8* kv, const mz_kv8_io* a, MzKv8Io* out) {
+int check_io(const char* who, const mz_kv8* kv, const mz_kv8_io* a, const MzKv8* cache, MzKv8Io* out) {
     if (a->rows < 0 || a->tokens < 0) return mz_fail(MZ_ERR_ARG, "%s: %d rows, %d tokens", who, a->rows, a->tokens);
     if (a->pos_stride < 0) return mz_fail(MZ_ERR_ARG, "%s: pos_stride %d", who, a->pos_stride);
     if (!aligned(a->k, 16) || !aligned(a->v, 16)) return mz_fail(MZ_ERR_ARG, "%s: k and v must be multiples of 16 bytes", who);
@@ -83,6 +83,7 @@ int check_io(const char* who, const mz_kv8* kv, const mz_kv8_io* a, MzKv8Io* out
     if (!strides_ok(stride, n)) return mz_fail(MZ_ERR_ARG, "%s: strides must be multiples of 8 elements, none negative", who);
     *out = {DP(f16, a->k), DP(f16, a->v), (long)a->row_stride, (long)a->token_stride, (long)a->head_stride, a->rows,
             a->tokens, DP(int, a->slot), DP(int, a->pos), a->pos_stride, a->pos_add, DP(int, a->count)};
+    if (!mz_kv8_io_fits(*cache, *out)) return mz_fail(MZ_ERR_ARG, "%s: too large for one call", who);
     return MZ_OK;
 }
 
@@ -120,7 +121,7 @@ int check_attention(const char* who, const mz_kv8* kv, const mz_kv8_attention_ar
 
 int check_scores(const char* who, const mz_score_args* a, MzScores* out) {
     if (a->dtype != MZ_DT_F16 && a->dtype != MZ_DT_F32) return mz_fail(MZ_ERR_ARG, "%s: bad dtype %d", who, a->dtype);
-    if (a->rows < 0 || a->rows > MAX_WORKGROUPS || a->vocab <= 0 || a->vocab > (1 << 30) || a->ld < a->vocab || a->ld > MOST / std::max(a->rows, 1))
+    if (a->rows < 0 || a->rows > MAX_SCORE_ROWS || a->vocab <= 0 || a->vocab > (1 << 30) || a->ld < a->vocab || a->ld > MOST / std::max(a->rows, 1))
         return mz_fail(MZ_ERR_ARG, "%s: %d rows of %d logits, ld %lld", who, a->rows, a->vocab, (long long)a->ld);
     if (a->alts < 0 || a->alts > MZ_SCORE_ALTS) return mz_fail(MZ_ERR_ARG, "%s: %d alternatives (0 .. %d)", who, a->alts, MZ_SCORE_ALTS);
     if (!a->logits || !aligned(a->logits, a->dtype == MZ_DT_F32 ? 4 : 2))
@@ -179,10 +180,9 @@ extern "C" int mz_kv8_write(mz_ctx* c, const mz_kv8* kv, const mz_kv8_io* a) {
     MzKv8 cache;
     MzKv8Io io;
     if (int r = check_cache("mz_kv8_write", kv, &cache)) return r;
-    if (int r = check_io("mz_kv8_write", kv, a, &io)) return r;
+    if (int r = check_io("mz_kv8_write", kv, a, &cache, &io)) return r;
     if (!a->rows || !a->tokens) return MZ_OK;
     if (!a->k || !a->v) return mz_fail(MZ_ERR_ARG, "mz_kv8_write: null k or v");
-    if (!mz_kv8_write_fits(cache, io)) return mz_fail(MZ_ERR_ARG, "mz_kv8_write: too large for one call");
     OnDevice on(c->device);
     if (on.status()) return on.status();
     return mz_hip(mz_kv8_write_launch(c->stream, cache, io), "mz_kv8_write");
@@ -193,11 +193,10 @@ extern "C" int mz_kv8_read(mz_ctx* c, const mz_kv8* kv, const mz_kv8_io* a) {
     MzKv8 cache;
     MzKv8Io io;
     if (int r = check_cache("mz_kv8_read", kv, &cache)) return r;
-    if (int r = check_io("mz_kv8_read", kv, a, &io)) return r;
+    if (int r = check_io("mz_kv8_read", kv, a, &cache, &io)) return r;
     const int64_t stride[3] = {a->row_stride, a->token_stride, a->head_stride}, n[3] = {a->rows, a->tokens, kv->heads};
     if (!apart(stride, n)) return mz_fail(MZ_ERR_ARG, "mz_kv8_read: the rows read into overlap");
     if (!a->rows || !a->tokens || (!a->k && !a->v)) return MZ_OK;
-    if (mz_kv8_read_grid(cache, io) > MAX_WORKGROUPS) return mz_fail(MZ_ERR_ARG, "mz_kv8_read: too large for one call");
     OnDevice on(c->device);
     if (on.status()) return on.status();
     return mz_hip(mz_kv8_read_launch(c->stream, cache, io), "mz_kv8_read");

@@ -125,7 +125,7 @@ struct Writer {
     int side, lane, p, n, open;
 
     int off, end;
-    bool full, old;
+    bool full, old;  // the block is whole now; its earlier positions are wanted
     f16x8 x[4] = {};  // keys: position lane / 8 + 8 i; values: channel 4 c + i, positions 8 g .. 8 g + 7
 
     // a block all of whose positions are new
@@ -160,7 +160,6 @@ struct Writer {
         off = max(p - b * MZ_KV_BLK, 0);
         end = min(p + n - b * MZ_KV_BLK, MZ_KV_BLK);
         full = end == MZ_KV_BLK;
-        old = off > 0 && (full || open != b);  // earlier positions are wanted
         const f16* s = src + (long)(b * MZ_KV_BLK - p) * a.token_stride;
         const long blk = sh * kv.blocks + b;
         if (side == 0) {
@@ -170,14 +169,19 @@ struct Writer {
                 const int t = (lane >> 3) + 8 * i;
                 x[i] = f16x8{};
                 if (t >= off && t < end) x[i] = __builtin_nontemporal_load((const f16x8*)(s + t * a.token_stride + d));
-                else if (old && t < off) {
+            }
+            old = off > 0 && (full || open != b);  // (the new ones are on their way before it is known which block is open)
+            if (old)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = (lane >> 3) + 8 * i;
+                    if (t >= off) continue;
                     if (open == b) x[i] = ld8(kv.k_open + sh * MZ_KV_TILE + t * 64 + d);
                     else {
                         const uint2 c = *(const uint2*)(kv.k + blk * MZ_KV_TILE + t * 64 + d);
                         x[i] = stand_for(widen<FMT>(c.x, c.y), kv.k_scale[blk]);
                     }
                 }
-            }
         } else {
             const int d = (lane & 15) * 4, t0 = (lane >> 4) * 8;
             f16x4 y[8];
@@ -187,6 +191,7 @@ struct Writer {
                 y[j] = f16x4{};
                 if (t >= off && t < end) y[j] = __builtin_nontemporal_load((const f16x4*)(s + t * a.token_stride + d));
             }
+            old = off > 0 && (full || open != b);
             if (old) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -297,19 +302,16 @@ __global__ void __launch_bounds__(256) write_kernel(MzKv8 kv, MzKv8Io a, int per
     if (threadIdx.x == 0) kv.open[sh] = (w.p + w.n) % MZ_KV_BLK ? last + 1 : 0;
 }
 
-// a wave: one side of one block of a (row, head)
+// a workgroup: keys and values of two blocks of a (row, head), a wave each
 template <int FMT>
-__global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a, int blocks, long units) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long unit = (long)blockIdx.x * 4 + wave, bh = unit / 2;
-    const int side = (int)(unit & 1);
+__global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), side = wave & 1;
+    const int r = blockIdx.z, h = blockIdx.y;
     f16* const base = side ? a.v : a.k;
-    if (unit >= units || !base) return;
-    const long rh = bh / blocks;
-    const int r = (int)(rh / kv.heads), h = (int)(rh - (long)r * kv.heads);
+    if (!base) return;
     Row w;
     if (!row_of(kv, a, r, w)) return;
-    const int b = w.p / MZ_KV_BLK + (int)(bh - rh * blocks);
+    const int b = w.p / MZ_KV_BLK + (int)blockIdx.x * 2 + (wave >> 1);
     const int lo = max(w.p - b * MZ_KV_BLK, 0), hi = min((int)min((long)w.p + w.n, (long)kv.blocks * MZ_KV_BLK) - b * MZ_KV_BLK, MZ_KV_BLK);
     if (hi <= lo) return;
     const long sh = w.slot * kv.heads + h, blk = sh * kv.blocks + b;
@@ -356,15 +358,15 @@ __global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a, int bloc
     }
 }
 
-// the most blocks that `tokens` positions of a row can lie in
-long spanned(int tokens) { return ((long)tokens + MZ_KV_BLK - 2) / MZ_KV_BLK + 1; }
+// the most blocks that a row's positions can lie in
+long spanned(const MzKv8& kv, const MzKv8Io& a) { return std::min(((long)a.tokens + MZ_KV_BLK - 2) / MZ_KV_BLK + 1, (long)kv.blocks); }
 // Blocks between the first and the last that a wave takes (write_kernel): two where that leaves every CU four workgroups (8 x
 // 1500 positions of 20 heads 19.8 us, 25.8 with one, 22.0 with four; 32 x 224 positions 15.6 / 22.5 / 16.2; but 1500 positions
 // of one row 6.8 / 6.5 / 8.3).
 int write_per(const MzKv8& kv, const MzKv8Io& a) {
-    return (long)a.rows * kv.heads * std::max(0L, spanned(a.tokens) - 2) >= 16L * mz_cu_count() ? 2 : 1;
+    return (long)a.rows * kv.heads * std::max(0L, spanned(kv, a) - 2) >= 16L * mz_cu_count() ? 2 : 1;
 }
-long write_groups(int tokens, int per) { return 1 + (std::max(0L, spanned(tokens) - 2) + 2 * per - 1) / (2 * per); }
+long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std::max(0L, spanned(kv, a) - 2) + 2 * per - 1) / (2 * per); }
 
 // ---------------------------------------------------------------- attention
 //
@@ -898,8 +900,8 @@ void attn_launch(hipStream_t s, const MzKv8& kv, const MzKv8Attn& a, const Launc
 }  // namespace
 
 // (a launch has fewer than 2^32 threads along x, and 2^16 workgroups along y and z)
-bool mz_kv8_write_fits(const MzKv8& kv, const MzKv8Io& a) { return a.rows <= 65535 && kv.heads <= 65535; }
-long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a) { return ((long)a.rows * kv.heads * spanned(a.tokens) * 2 + 3) / 4; }
+bool mz_kv8_io_fits(const MzKv8& kv, const MzKv8Io& a) { return a.rows <= 65535 && kv.heads <= 65535; }
+
 bool mz_kv8_attn_fits(const MzKv8& kv, const MzKv8Attn& a) {
     const long nq = (long)a.tokens * (a.heads / kv.heads);
     return (long)a.rows * kv.heads < (1L << 23) - 8 && nq <= 16L * 65535;
@@ -912,18 +914,16 @@ size_t mz_kv8_attn_work(const MzKv8& kv, const MzKv8Attn& a) {
 
 hipError_t mz_kv8_write_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) {
     const int per = write_per(kv, a);
-    const dim3 grid(write_groups(a.tokens, per), kv.heads, a.rows), block(a.tokens == 1 ? 128 : 256);  // (one token: one block)
+    const dim3 grid(write_groups(kv, a, per), kv.heads, a.rows), block(a.tokens == 1 ? 128 : 256);  // (one token: one block)
     if (kv.format == I8) hipLaunchKernelGGL(write_kernel<I8>, grid, block, 0, s, kv, a, per);
     else hipLaunchKernelGGL(write_kernel<E4M3>, grid, block, 0, s, kv, a, per);
     return hipGetLastError();
 }
 
 hipError_t mz_kv8_read_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a) {
-    const dim3 grid(mz_kv8_read_grid(kv, a));
-    const int blocks = (int)spanned(a.tokens);
-    const long units = (long)a.rows * kv.heads * blocks * 2;
-    if (kv.format == I8) hipLaunchKernelGGL(read_kernel<I8>, grid, dim3(256), 0, s, kv, a, blocks, units);
-    else hipLaunchKernelGGL(read_kernel<E4M3>, grid, dim3(256), 0, s, kv, a, blocks, units);
+    const dim3 grid((spanned(kv, a) + 1) / 2, kv.heads, a.rows);
+    if (kv.format == I8) hipLaunchKernelGGL(read_kernel<I8>, grid, dim3(256), 0, s, kv, a);
+    else hipLaunchKernelGGL(read_kernel<E4M3>, grid, dim3(256), 0, s, kv, a);
     return hipGetLastError();
 }
 

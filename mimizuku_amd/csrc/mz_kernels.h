@@ -274,9 +274,7 @@ struct MzKv8Io {
     const int* count;
 };
 // whether one launch takes it: rows and heads at most 65535
-bool mz_kv8_write_fits(const MzKv8& kv, const MzKv8Io& a);
-// workgroups of 256 threads of a launch; the caller keeps them below 2^24
-long mz_kv8_read_grid(const MzKv8& kv, const MzKv8Io& a);
+bool mz_kv8_io_fits(const MzKv8& kv, const MzKv8Io& a);
 hipError_t mz_kv8_write_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a);
 hipError_t mz_kv8_read_launch(hipStream_t s, const MzKv8& kv, const MzKv8Io& a);
 

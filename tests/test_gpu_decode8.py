@@ -233,6 +233,14 @@ def test_rows_outside_the_cache_write_nothing(ctx, dev):
     huge = [2 ** 31 - 1] * 9
     b.write(dev, k, v, slot=slot, pos=huge, count=cnt)
     b.check()
+    # more tokens than a slot has positions, of which a few are there
+    b.d.write(dev(k), dev(v), 1, 2 ** 31 - 1, strides=(0, 128, 64), pos=dev(i32([3])), count=dev(i32([17])))
+    b.r.write(k[:1, :17], v[:1, :17], pos=[3])
+    b.end[0] = 20
+    b.check()
+    out = dev(np.zeros((64, 2, 64), np.float16))
+    b.d.read(out, 0, 1, 2 ** 31 - 1, strides=(0, 128, 64), slot=dev(i32([4])), count=dev(i32([2 ** 31 - 1])))
+    np.testing.assert_array_equal(ctx.download(out, (64, 2, 64), np.float16)[:40], b.r.stands_for(0)[4, :, :40].transpose(1, 0, 2))
     b.free()
 
 
@@ -518,10 +526,11 @@ def test_alignment_rows(ctx, dev, fmt, tokens, heads, kvh, cols):
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("rows,heads,tokens", [(10, 16, 5), (3, 7, 1), (20, 16, 1), (17, 16, 3)])
+@pytest.mark.parametrize("rows,heads,tokens", [(10, 16, 5), (3, 7, 1), (20, 16, 1), (17, 16, 3), (10, 16, 6), (1, 2, 30),
+                                               (9, 15, 33)])
 def test_alignment_rows_of_long_caches(ctx, dev, fmt, rows, heads, tokens):
-    """The encoder's 1500 positions: scores kept by a workgroup (the most that are), by several that share a row, by
-    workgroups of four and of eight waves."""
+    """The encoder's 1500 positions: scores kept by a workgroup (the most that are) or in their rows, by one workgroup or
+    several that share the blocks, of four and of eight waves."""
     rng = np.random.default_rng(rows)
     lens = [1500 - 7 * (r % 5) for r in range(rows)]
     b = filled(ctx, dev, rng, rows, heads, lens, fmt)
