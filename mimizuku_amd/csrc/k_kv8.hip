@@ -406,6 +406,8 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
 // what a row's queries see: token i positions first .. min(base + (causal ? i : 0), cap) - 1 of its slot
 struct Seen {
     long slot, base;
@@ -561,7 +563,8 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     };
 
     float m[QT], l[QT];
-    float unit = 0.f, per_unit = 0.f;  // the accumulators are in `unit`s, a power of two that no block's values' scale passes
+    // the accumulators are in `unit`s, a power of two that no block's values' scale passes (lg_unit: its logarithm)
+    float unit = 0.f, per_unit = 0.f, lg_unit = -INFINITY;
     f32x4 acc[QT][4];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -574,16 +577,20 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     // P as one fp16 number, or as the sum of two where the products wait for memory anyway
     constexpr bool FINE = QT == 1 && !OWN;
     auto weighted = [&](f16x8 v, f16x8 p, f16x8 rest, f32x4 to) { return mfma16(v, p, FINE ? mfma16(v, rest, to) : to); };
-    auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], float ks, float vs) {
+    // A block's scales: cs the keys' in the exponent (of two), vs the values', with its logarithm and reciprocal.
+    struct Scales {
+        float cs, vs, lg, rc;
+    };
+    auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], const Scales& sc) {
         const int p0 = b * MZ_KV_BLK + 8 * g;  // this lane's positions
-        float cs = scale2 * ks;
-        if (cs == 0.f) cs = 1e-37f;  // (all keys 0; what is not seen is -inf times it)
+        const float cs = sc.cs;
         const bool whole = b * MZ_KV_BLK >= s.first && (b + 1) * MZ_KV_BLK <= lo_end;  // seen by every query
         const bool given = b == open;  // fp16 as it was given, any number: vs is 1 and says nothing about the numbers' size
-        if (given ? unit == 0.f : vs > unit) {
+        if (given ? unit == 0.f : sc.vs > unit) {
             const float to = given ? 9.5367431640625e-07f
-                                   : __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, vs) & 0x7f800000u) + 0x00800000u);
+                                   : __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, sc.vs) & 0x7f800000u) + 0x00800000u);
             per_unit = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(unsigned, to));  // 1 / to
+            lg_unit = (float)((int)(__builtin_bit_cast(unsigned, to) >> 23) - 127);
             const float f = unit * per_unit;
 #pragma unroll
             for (int t = 0; t < QT; t++)
@@ -591,10 +598,9 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
                 for (int u = 0; u < 4; u++) acc[t][u] *= f;
             unit = to;
         }
-        // P is multiplied by `part`, before its rounding (in the exponent) if it is not small
-        const float part = vs * per_unit;
-        const bool direct = !given && part >= 0.0078125f;
-        const float up = direct ? __builtin_amdgcn_logf(part) : 0.f, down = direct ? __builtin_amdgcn_rcpf(part) : 1.f;
+        // P is multiplied by vs / unit, in the exponent, if that is not small
+        const bool direct = !given && sc.lg - lg_unit >= -7.f;
+        const float up = direct ? sc.lg - lg_unit : 0.f, down = direct ? sc.rc * unit : 1.f;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             f32x4 d[2];
@@ -618,8 +624,9 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
                         }
                 }
             }
-            const float top = cs * fmaxf(fmaxf(fmaxf(d[0][0], d[0][1]), fmaxf(d[0][2], d[0][3])),
-                                         fmaxf(fmaxf(d[1][0], d[1][1]), fmaxf(d[1][2], d[1][3])));
+            // (the median of two numbers and infinity is the larger one; a maximum would make its operands quiet first)
+            const float top = cs * fmaxf(fmaxf(larger(d[0][0], d[0][1]), larger(d[0][2], d[0][3])),
+                                         fmaxf(larger(d[1][0], d[1][1]), larger(d[1][2], d[1][3])));
             if (__ballot(top > m[t] + 8.f)) {
                 const float mn = fmaxf(m[t], column_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
@@ -646,7 +653,7 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
 #pragma unroll
                 for (int u = 0; u < 4; u++) acc[t][u] = weighted(vf[u], p, rest, acc[t][u]);
             } else {
-                const float f = direct ? 1.f : part;
+                const float f = direct ? 1.f : sc.vs * per_unit;
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const f32x4 y = weighted(vf[u], p, rest, f32x4{});
@@ -656,7 +663,7 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             }
         }
     };
-    auto coded = [&](int b, const Raw& w, float ks, float vs) {
+    auto coded = [&](int b, const Raw& w, const Scales& sc) {
         f16x8 kf[2][2], vf[4];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
@@ -665,7 +672,7 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             vf[2 * j] = widen<FMT>(w.v[j][0], w.v[j][1]);
             vf[2 * j + 1] = widen<FMT>(w.v[j][2], w.v[j][3]);
         }
-        products(b, kf, vf, ks, vs);
+        products(b, kf, vf, sc);
     };
     // Blocks b0 + wave, + 4, ...: DEPTH of them on their way. The open block, where it is this wave's, comes first; its codes
     // are stale.
@@ -676,11 +683,17 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     const int head = b0 + (OWN ? 0 : wave);
     if (head < b1) {
         const int tail = head + (b1 - 1 - head) / STEP * STEP;
-        float ks, vs;
+        Scales lanes;
         auto scales = [&](int b) {
             const int at = min(b + STEP * lane, tail);
-            ks = ksc[at];
-            vs = vsc[at];
+            const float ks = ksc[at], vs = vsc[at], cs = scale2 * ks;
+            lanes.cs = cs == 0.f ? 1e-37f : cs;  // (all keys 0; what is not seen is -inf times it)
+            lanes.vs = vs;
+            lanes.lg = __builtin_amdgcn_logf(vs);
+            lanes.rc = __builtin_amdgcn_rcpf(vs);
+        };
+        auto scales_of = [&](int i) {
+            return Scales{lane_value(lanes.cs, i), lane_value(lanes.vs, i), lane_value(lanes.lg, i), lane_value(lanes.rc, i)};
         };
 #pragma unroll
         for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
@@ -701,7 +714,7 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
                     const int p = open * MZ_KV_BLK + 8 * g + e;
                     if (p < s.first || p >= hi) vf[j][e] = (f16)0.f;
                 }
-            products(open, kf, vf, 1.f, 1.f);
+            products(open, kf, vf, Scales{scale2, 1.f, 0.f, 1.f});
         }
         for (int b = head, at = 0; b <= tail; b += STEP * DEPTH, at += DEPTH) {
             if (at == WINDOW) {
@@ -711,7 +724,7 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
 #pragma unroll
             for (int i = 0; i < DEPTH; i++) {
                 const int bi = b + STEP * i;
-                if (bi <= tail && bi != open) coded(bi, w[i], lane_value(ks, at + i), lane_value(vs, at + i));
+                if (bi <= tail && bi != open) coded(bi, w[i], scales_of(at + i));
                 fetch(bi + STEP * DEPTH, w[i]);
             }
         }

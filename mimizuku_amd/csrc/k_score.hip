@@ -39,14 +39,16 @@ __device__ __forceinline__ float value_of(Key k) {
     return k ? __builtin_bit_cast(float, u ^ (~(unsigned)((int)u >> 31) | 0x80000000u)) : -INFINITY;
 }
 __device__ __forceinline__ int id_of(Key k) { return (int)(IDS - 1 - ((unsigned)k & (IDS - 1))); }
+// (through the compiler each operand would be made quiet first, another such instruction each; the two wait states are those
+// that a DPP or lane-swap reader of a vector result needs, which the compiler does not see here)
 __device__ __forceinline__ Key larger(Key a, Key b) {
     Key r;
-    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    asm("v_max_f64 %0, %1, %2\n\ts_nop 1" : "=v"(r) : "v"(a), "v"(b));
     return r;
 }
 __device__ __forceinline__ Key smaller(Key a, Key b) {
     Key r;
-    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    asm("v_min_f64 %0, %1, %2\n\ts_nop 1" : "=v"(r) : "v"(a), "v"(b));
     return r;
 }
 __device__ __forceinline__ Key lane_key(Key k, int i) {
