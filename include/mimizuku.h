@@ -122,8 +122,8 @@ int mz_mel_transpose(mz_ctx* c, uint64_t mel, uint64_t melT, int clips, int n_me
  * capturable (no allocation, no host synchronisation). Positions, lengths and slots are read on the device, so that a
  * captured graph can be replayed while they change; one that lies outside a cache touches nothing, as stated below.
  *
- * A cache holds `slots` sequences of up to blocks * 32 positions (blocks < 2^20). Each block of 32 positions x 64 channels of a (slot,
- * head) has one scale for its keys and one for its values; code c stands for c * scale, with
+ * A cache holds `slots` sequences of up to blocks * 32 positions (blocks < 2^20). Each block of 32 positions x 64
+ * channels of a (slot, head) has one scale for its keys and one for its values; code c stands for c * scale, with
  *   MZ_KV8_I8:   c a signed whole number, scale = f32(top / 127), c = 127 x / top to the nearest, halves to even
  *   MZ_KV8_E4M3: c an OCP e4m3 number,    scale = f32(top / 448), c = 448 x / top to the nearest, halves to even
  * where top is the block's largest magnitude (0: scale 0 and codes 0). A block is coded when its last position is
@@ -185,7 +185,10 @@ typedef struct {
     uint64_t count; /* i32 [rows]: tokens of row r that are there (0: all); the others' outputs are left as they were */
     /* token i sees positions from first[r] (first 0: from 0) to below len[r * len_stride] + len_add (len 0: len_add),
      * and with `causal` i more; never past the cache. A query that sees nothing, or whose row's slot lies outside the
-     * cache, gets out 0 and lse -inf. What lies outside the positions seen is never looked at, NaN or not. */
+     * cache, gets out 0 and lse -inf. Blocks of which a query sees nothing do not touch it, NaN or not; neither do
+     * positions of the open block that no token of the call sees. (A NaN or infinity at a position of the open block
+     * that later tokens of the call see can reach the earlier tokens that see the block: it is none as a whole, as it
+     * will be when it is coded.) */
     uint64_t len; /* i32 */
     int len_stride, len_add;
     uint64_t first; /* i32 [rows] */
@@ -195,8 +198,10 @@ typedef struct {
      * counts), 0 at positions not seen. align 0: not wanted. */
     uint64_t head_slot, align;
     int align_heads, align_cols;
-    uint64_t work; /* mz_kv8_attention_bytes bytes of device memory (256-byte aligned), not shared with calls that may
-                    * run at the same time */
+    /* mz_kv8_attention_bytes bytes of device memory (256-byte aligned), zero before its first use (mz_alloc's is) and
+     * written by nothing but these calls and mz_token_scores, whatever their sizes: its first 16 KB are zero again when
+     * a call has run. Calls that may run at the same time need one each. */
+    uint64_t work;
     size_t work_bytes;
 } mz_kv8_attention_args;
 int mz_kv8_attention(mz_ctx* c, const mz_kv8* kv, const mz_kv8_attention_args* a);

@@ -76,7 +76,8 @@ class Kv8:
                   len_stride: int = 1, len_add: int = 0, first: int = 0, lse: int = 0, head_slot: int = 0,
                   align: int = 0, align_heads: int = 0, align_cols: int = 0, work: tuple[int, int] | None = None):
         """Attention of rows x tokens queries f16 over the cache (mz_kv8_attention). Strides as of write, over `heads`
-        query heads. work: (address, bytes) of a workspace; None: the context's (Context.workspace)."""
+        query heads. work: (address, bytes) of a workspace, zero before its first use; None: the context's
+        (Context.workspace)."""
         dense = (tokens * heads * HD, heads * HD, HD)
         a = L.Kv8Attention(q, out, *(q_strides or dense), *(out_strides or dense), rows, tokens, heads, int(causal), scale,
                            slot, count, len, len_stride, len_add, first, lse, head_slot, align, align_heads, align_cols)

@@ -591,6 +591,42 @@ def test_attention_needs_its_workspace(ctx, dev):
     b.free()
 
 
+def test_one_workspace_for_calls_of_every_size(ctx, dev):
+    """Attention and scores of different sizes one after the other in one workspace, twice: the same bits as each in one of
+    its own, which is zero before and whose head is zero afterwards."""
+    rng = np.random.default_rng(19)
+    caches = [filled(ctx, dev, rng, r, h, [n] * r, "i8") for r, h, n in ((1, 2, 1500), (5, 7, 1400), (2, 20, 700))]
+    qs = [f16(rng, (b.r.slots, 1, b.r.heads, 64), 1.5) for b in caches]
+    xs = [logits(rng, n, v, np.float32) for n, v in ((1, 51865), (30, 20000), (200, 9000))]
+    size = 32 << 20
+    shared = ctx.alloc(size)
+
+    def attend(i, work):
+        b, q = caches[i], qs[i]
+        return run_attention(ctx, dev, b, q, False, [b.end[0]] * len(q), head_slot=[0] + [-1] * (b.r.heads - 1), align_heads=1,
+                             align_cols=1500, work=work)
+
+    def score(i, work):
+        x = xs[i]
+        o = [dev(np.zeros((len(x), 3), t)) for t in (np.float32, np.int32)]
+        decode8.token_scores(ctx, dev(x), *x.shape, entropy=o[0], alts=3, alt_ids=o[1], work=work)
+        return ctx.download(o[0], (len(x),), np.float32), ctx.download(o[1], (len(x), 3), np.int32)
+
+    calls = [(attend, 0), (score, 0), (attend, 1), (score, 1), (attend, 2), (score, 2), (attend, 0), (score, 0)]
+    for _ in range(2):
+        for f, i in calls:
+            own = ctx.alloc(size)
+            want, got = f(i, (own, size)), f(i, (shared, size))
+            for a, b in zip(want, got):
+                np.testing.assert_array_equal(a, b)
+            for p in (own, shared):
+                assert not ctx.download(p, (4096,), np.uint32).any()
+            ctx.free(own)
+    ctx.free(shared)
+    for b in caches:
+        b.free()
+
+
 @pytest.mark.parametrize("fmt", FMT)
 def test_offsets_past_32_bits(ctx, dev, fmt):
     """A cache whose codes alone are 5 GB for the keys and as much for the values: the last slot's last blocks written,
