@@ -163,8 +163,8 @@ typedef struct {
 /* Writes the rows' tokens at their positions. Sequences are written in order: a row's first position is at most the
  * number of positions its slot holds, and what a slot held behind the last position written is gone. A write that
  * begins inside a coded block opens it again: its earlier positions become what their codes stand for, in fp16. A row
- * whose slot or positions lie outside the cache writes nothing, and neither does one whose slot a later row names
- * too. */
+ * without tokens, or whose slot or positions lie outside the cache, writes nothing, and of rows that would write to one
+ * slot the last one does. */
 int mz_kv8_write(mz_ctx* c, const mz_kv8* kv, const mz_kv8_io* a);
 /* Reads positions back: f16(f32(code * scale)), or an open block's fp16. Here k and v are written (either may be 0: not
  * wanted); rows whose slot lies outside the cache, tokens whose position does and tokens from count[r] on are left as

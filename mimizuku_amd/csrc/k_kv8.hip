@@ -111,6 +111,11 @@ __device__ __forceinline__ bool row_of(const MzKv8& kv, const MzKv8Io& a, int r,
     return o.n > 0 && o.slot >= 0 && o.slot < kv.slots && p >= 0 && p < (long)kv.blocks * MZ_KV_BLK;
 }
 
+// the same for a write, whose positions are all in the cache or not written
+__device__ __forceinline__ bool write_row(const MzKv8& kv, const MzKv8Io& a, int r, Row& o) {
+    return row_of(kv, a, r, o) && o.p + (long)o.n <= (long)kv.blocks * MZ_KV_BLK;
+}
+
 // Lanes over a block, keys: 8 channels of positions lane / 8 + 8 i; values: 4 channels of 8 positions, so that whole
 // 16-byte pieces of the order of v are a lane's own.
 //
@@ -273,12 +278,18 @@ __global__ void __launch_bounds__(256) write_kernel(MzKv8 kv, MzKv8Io a, int per
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = blockIdx.x;
     const int r = blockIdx.z, h = blockIdx.y;
     Row w;
-    if (!row_of(kv, a, r, w) || w.p + (long)w.n > (long)kv.blocks * MZ_KV_BLK) return;
+    if (!write_row(kv, a, r, w)) return;
     const int first = w.p / MZ_KV_BLK, last = (w.p + w.n - 1) / MZ_KV_BLK;
     if (grp && first + 1 + 2 * per * (grp - 1) >= last) return;
-    if (a.slot)  // the last row of a slot counts
-        for (int i = r + 1; i < a.rows; i += 64)
-            if (__ballot(i + lane < a.rows && a.slot[i + lane < a.rows ? i + lane : i] == w.slot)) return;
+    if (a.slot)  // of rows that write to a slot the last one does
+        for (int i = r + 1; i < a.rows; i += 64) {
+            bool later = i + lane < a.rows && a.slot[i + lane < a.rows ? i + lane : i] == w.slot;
+            if (__ballot(later)) {
+                Row o;
+                later = later && write_row(kv, a, i + lane, o);
+                if (__ballot(later)) return;
+            }
+        }
     const long sh = w.slot * kv.heads + h;
     const int side = wave & 1;
     Writer<FMT> x{kv, a, sh, (side ? a.v : a.k) + r * a.row_stride + h * a.head_stride, side, lane, w.p, w.n, grp ? -1 : kv.open[sh] - 1};

@@ -68,8 +68,9 @@ class Context:
 
     def workspace(self, nbytes: int) -> tuple[int, int]:
         """(address, bytes) of a scratch buffer of at least nbytes, zero at first, for calls on this context's stream
-        (Kv8.attention, token_scores), which run one after the other and share it. Grown by a new buffer; the smaller one stays allocated until the context is
-        closed, for graphs captured with it. It allocates: the first call of a size comes before a capture."""
+        (Kv8.attention, token_scores), which run one after the other and share it. Grown by a new buffer; the smaller
+        one stays allocated until the context is closed, for graphs captured with it. It allocates: the first call of a
+        size comes before a capture."""
         if nbytes > self.work[1]:
             n = max(2 * self.work[1], nbytes, 1 << 20)
             self.work = (self.alloc(n), n)

@@ -78,14 +78,14 @@ class Cache:
     def write(self, k, v, slot=None, pos=None, count=None):
         """k, v f16 [rows][tokens][heads][64]."""
         rows, tokens = k.shape[:2]
+        todo = {}  # slot: its row, position and tokens
         for r in range(rows):
             s = r if slot is None else int(slot[r])
             p = 0 if pos is None else int(pos[r])
             n = tokens if count is None else min(max(int(count[r]), 0), tokens)
-            if not 0 <= s < self.slots or n <= 0 or p < 0 or p + n > self.cap:
-                continue
-            if slot is not None and any(int(x) == s for x in slot[r + 1:]):
-                continue
+            if 0 <= s < self.slots and n > 0 and p >= 0 and p + n <= self.cap:
+                todo[s] = r, p, n
+        for s, (r, p, n) in todo.items():
             for h in range(self.heads):
                 was, last = int(self.open[s, h]) - 1, (p + n - 1) // BLK
                 for side, src in enumerate((k, v)):

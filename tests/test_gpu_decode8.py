@@ -244,6 +244,28 @@ def test_rows_outside_the_cache_write_nothing(ctx, dev):
     b.free()
 
 
+def test_padding_rows_do_not_take_a_slot(ctx, dev):
+    """Rows behind the last sequence name slot 0 and have no tokens, or tokens outside the cache: slot 0's own row writes.
+    More rows than a wave looks at in one go."""
+    rng = np.random.default_rng(7)
+    n = 200
+    b = Both(ctx, 3, 2, 96, "e4m3")
+    slot, pos, cnt = [0, 1, 2, 1] + [0] * (n - 4), [0] * n, [40, 33, 10, 64] + [0] * (n - 4)
+    cnt[150], pos[150] = 40, 57
+    cnt[180], pos[180] = -3, 5
+    k, v = f16(rng, (n, 64, 2, 64)), f16(rng, (n, 64, 2, 64))
+    b.end = [40, 64, 10]
+    b.write(dev, k, v, slot=slot, pos=pos, count=cnt)
+    b.check()
+    assert b.r.open[:, 0].tolist() == [2, 0, 1]
+    # one of them writes after all
+    cnt[150], pos[150] = 7, 40
+    b.end = [47, 64, 10]
+    b.write(dev, k, v, slot=slot, pos=pos, count=cnt)
+    b.check()
+    b.free()
+
+
 @pytest.mark.parametrize("fmt", FMT)
 def test_source_layouts(ctx, dev, fmt):
     """Rows of a fused projection, per-head tiles as the engine's cross keys and values, a broadcast row."""
@@ -888,6 +910,66 @@ def test_a_captured_decoding_step(ctx, dev, fmt):
         p.kv.free()
     cross_kv.free()
     assert np.isfinite(last[0]).all() or (last[0] == -np.inf).any()
+
+
+def test_captured_calls_that_share_rows_and_a_workspace(ctx, dev):
+    """Two graphs, each of an attention and scores whose work is shared by workgroups, in one workspace, replayed in turn with
+    eager calls between them while a second context runs the same on its own stream with its own: always the bits of the
+    eager calls."""
+    import ctypes as C
+    rng = np.random.default_rng(23)
+    lens = (1500, 1311)
+    caches = [filled(ctx, dev, rng, 1, 2, [n], "i8") for n in lens]
+    qs = [dev(f16(rng, (1, 2, 64), 1.5)) for _ in lens]
+    xs = [dev(logits(rng, 1, 51866, np.float32)) for _ in lens]
+    other = model.Context(0)
+    work = other.alloc(4 << 20)
+
+    class Calls:
+        def __init__(self, c, i, work=None):
+            self.c, self.i, self.work = c, i, work
+            self.o, self.l, self.e = dev(np.zeros((2, 64), np.float16)), dev(np.zeros(2, np.float32)), dev(np.zeros(1, np.float32))
+            self.ids = dev(np.zeros((1, 5), np.int32))
+            self.kv = decode8.Kv8.__new__(decode8.Kv8)
+            self.kv.ctx, self.kv.kv = c, caches[i].d.kv
+
+        def run(self):
+            self.kv.attention(qs[self.i], self.o, 1, 1, 2, causal=False, len_add=lens[self.i], lse=self.l, work=self.work)
+            decode8.token_scores(self.c, xs[self.i], 1, 51866, entropy=self.e, alts=5, alt_ids=self.ids, work=self.work)
+
+        def results(self):
+            self.c.sync()
+            return [ctx.download(*x) for x in ((self.o, (2, 64), np.float16), (self.l, (2,), np.float32),
+                                               (self.e, (1,), np.float32), (self.ids, (1, 5), np.int32))]
+
+    want, graphs = [], []
+    for i in range(2):
+        eager = Calls(ctx, i)
+        eager.run()
+        want.append(eager.results())
+        held = Calls(ctx, i)
+        L.check(L.lib().mz_graph_begin(ctx.h))
+        held.run()
+        g = C.c_void_p()
+        L.check(L.lib().mz_graph_end(ctx.h, C.byref(g)))
+        graphs.append((held, g))
+    for n in range(6):
+        beside = Calls(other, n % 2, (work, 4 << 20))
+        between = Calls(ctx, 1 - n % 2)
+        for _ in range(3):
+            beside.run()
+            for held, g in graphs:
+                L.check(L.lib().mz_graph_launch(ctx.h, g))
+            between.run()
+        for c in (graphs[0][0], graphs[1][0], between, beside):
+            for a, b in zip(c.results(), want[c.i]):
+                np.testing.assert_array_equal(a, b, err_msg=f"replay {n}")
+    for _, g in graphs:
+        L.check(L.lib().mz_graph_free(g))
+    other.free(work)
+    other.close()
+    for b in caches:
+        b.free()
 
 
 def test_engine_buffers(ctx, dev):
