@@ -466,24 +466,6 @@ __device__ __forceinline__ void align_indices(const MzKv8Attn& a, int h0, int n,
     __syncthreads();
 }
 
-// Scores (in powers of two) to probabilities, by all threads of the workgroup; 0 where nothing is seen. get(p) is the score of
-// a position that is; eight of them on their way at a time.
-template <int THREADS, typename Get>
-__device__ __forceinline__ void align_finish(float* row, int cols, int lo, int hi, float lse2, Get get) {
-    for (int p0 = threadIdx.x; p0 < cols; p0 += 8 * THREADS) {
-        float x[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int p = p0 + THREADS * k;
-            x[k] = -INFINITY;
-            if (p < cols && p >= lo && p < hi) x[k] = get(p);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (p0 + THREADS * k < cols) row[p0 + THREADS * k] = x[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[k] - lse2);
-    }
-}
-
 struct Launch {
     int qt, tiles, splits;  // queries of a workgroup / 16, such tiles of a (row, cache head), workgroups that share the blocks
     int waves, own;         // waves of a workgroup; whether each has 16 queries of its own (qt is not used then)
@@ -504,7 +486,6 @@ template <int FMT, int QT, bool ALIGN, int NW, bool OWN>
 __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
     static_assert(!(OWN && ALIGN));
     __shared__ float red[OWN ? 1 : NW][16][68], ms[NW][16], ls[NW][16];
-    __shared__ float* als[16];
     __shared__ float lse2s[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     // x: (row, cache head), padded to a multiple of the XCDs, so that what shares keys and values shares an XCD; y: the tiles,
@@ -768,7 +749,61 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     // the waves' states joined, 16 queries at a time, by the first 256 threads
     const int col = tid >> 4 & 15, d4 = (tid & 15) * 4;
     const bool mine256 = NW == 4 || tid < 256;
-    auto emit = [&](int t, float mm, float ll, f32x4 o) {
+    // Alignment rows of 16 queries: their scores (in powers of two, get(query, row, position)) to probabilities, 0 where nothing
+    // is seen, by all threads, eight of a row's scores a thread at a time and the first ones of four rows.
+    constexpr int STRIDE = 64 * NW;
+    auto rows = [&](int t) { return (unsigned)__ballot(al[t] != nullptr) & 0xffff; };
+    auto row_of_query = [&](int t, int k) {
+        const unsigned long at = (unsigned long)al[t];
+        return (float*)((unsigned long)(unsigned)__builtin_amdgcn_readlane((int)(at >> 32), k) << 32 |
+                        (unsigned)__builtin_amdgcn_readlane((int)at, k));
+    };
+    auto scores = [&](int t, int k, int p0, float (&x)[8], auto get) {
+        const float* row = row_of_query(t, k);
+        const int to = min(s.end(a, token_of(q0 + 16 * t + k)), a.align_cols);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int p = p0 + STRIDE * j;
+            x[j] = -INFINITY;
+            if (p >= s.first && p < to) x[j] = get(16 * t + k, row, p);
+        }
+    };
+    // of the first FEW of the rows `has`
+    constexpr int FEW = 4;
+    typedef float Few[FEW][8];
+    auto few_scores = [&](int t, unsigned has, Few& x, auto get) {
+#pragma unroll
+        for (int u = 0; u < FEW; u++) {
+            if (!has) break;
+            scores(t, __ffs(has) - 1, tid, x[u], get);
+            has &= has - 1;
+        }
+    };
+    // (x: those of the first rows are on their way)
+    auto probabilities = [&](int t, Few& x, auto get) {
+        for (unsigned has = rows(t); has;) {
+#pragma unroll
+            for (int u = 0; u < FEW; u++) {
+                if (!has) break;
+                const int k = __ffs(has) - 1;
+                has &= has - 1;
+                float* const row = row_of_query(t, k);
+                const float lse2 = lse2s[k];
+                for (int p0 = tid; p0 < a.align_cols; p0 += 8 * STRIDE) {
+                    if (p0 != tid) scores(t, k, p0, x[u], get);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (p0 + STRIDE * j < a.align_cols)
+                            row[p0 + STRIDE * j] = x[u][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[u][j] - lse2);
+                }
+            }
+            few_scores(t, has, x, get);
+        }
+    };
+    auto in_lds = [&](int q, const float*, int p) { return kept[q * n.kept + p - b0 * MZ_KV_BLK]; };
+    auto in_place = [&](int, const float* row, int p) { return row[p]; };
+    auto in_memory = [&](int, const float* row, int p) { return shared_load(row + p); };
+    auto emit = [&](int t, float mm, float ll, f32x4 o, Few& scores, auto get) {
         const int x = q0 + 16 * t + col, i = token_of(x), h = kh * grp + x - i * grp;
         const float inv = ll == 0.f ? 0.f : 1.f / ll, lse2 = ll == 0.f ? -INFINITY : mm + __builtin_amdgcn_logf(ll);
         if (mine256 && x < nq && i < s.count) {
@@ -776,20 +811,9 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             if (a.lse && d4 == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
         }
         if (ALIGN) {
-            if (tid < 16) als[c] = al[t];
             if (mine256 && d4 == 0) lse2s[col] = lse2;
             __syncthreads();
-            for (int k = 0; k < 16; k++) {
-                if (!als[k]) continue;
-                float* const row = als[k];
-                const int to = s.end(a, token_of(q0 + 16 * t + k));
-                if (n.splits > 1)
-                    align_finish<64 * NW>(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return shared_load(row + p); });
-                else if (n.kept) {
-                    const float* x = kept + (16 * t + k) * n.kept - b0 * MZ_KV_BLK;
-                    align_finish<64 * NW>(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return x[p]; });
-                } else align_finish<64 * NW>(row, a.align_cols, s.first, to, lse2s[k], [&](int p) { return row[p]; });
-            }
+            probabilities(t, scores, get);
             __syncthreads();
         }
     };
@@ -821,21 +845,28 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = fmaf(f, y[e], o[e]);
         }
-        if (n.splits == 1) emit(t, mm, ll, o);
+        if (n.splits == 1) {
+            Few x;
+            if (n.kept) {
+                few_scores(t, ALIGN ? rows(t) : 0, x, in_lds);
+                emit(t, mm, ll, o, x, in_lds);
+            } else {
+                few_scores(t, ALIGN ? rows(t) : 0, x, in_place);
+                emit(t, mm, ll, o, x, in_place);
+            }
+        }
         else if (mine256 && q0 + 16 * t + col < nq) {
             float* w = states + (split * (16 * QT) + 16 * t + col) * STATE;
             shared_store(w + d4, o[0], o[1]);
             shared_store(w + d4 + 2, o[2], o[3]);
             if (d4 == 0) shared_store(w + 64, mm, ll);
         }
-        if (ALIGN && n.splits > 1 && n.kept) {  // the share's scores to where the last workgroup finds them
-            if (tid < 16) als[c] = al[t];
-            __syncthreads();
-            for (int k = 0; k < 16; k++)
-                if (als[k])
-                    for (int p = b0 * MZ_KV_BLK + tid; p < min(b1 * MZ_KV_BLK, a.align_cols); p += 64 * NW)
-                        shared_store(als[k] + p, kept[(16 * t + k) * n.kept + p - b0 * MZ_KV_BLK]);
-        }
+        if (ALIGN && n.splits > 1 && n.kept)  // the share's scores to where the last workgroup finds them
+            for (unsigned has = rows(t); has; has &= has - 1) {
+                const int k = __ffs(has) - 1;
+                float* const row = row_of_query(t, k);
+                for (int p = b0 * MZ_KV_BLK + tid; p < min(b1 * MZ_KV_BLK, a.align_cols); p += STRIDE) shared_store(row + p, in_lds(16 * t + k, row, p));
+            }
         if (t + 1 < QT) __syncthreads();
     }
     if (n.splits == 1 || !last_of((unsigned*)a.work + (long)pair * n.tiles + tile, n.splits)) return;
@@ -844,32 +875,35 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     for (int t = 0; t < QT; t++) {
         float mm = NOTHING, ll = 0.f;
         f32x4 o = {};
+        Few x;
+        few_scores(t, ALIGN ? rows(t) : 0, x, in_memory);  // (they come with the states)
         if (mine256 && q0 + 16 * t + col < nq)
             for (int k0 = 0; k0 < n.splits; k0 += 4) {
-                float2 x[4][3];
+                float2 y[4][3];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const float* w = states + (min(k0 + k, n.splits - 1) * (16 * QT) + 16 * t + col) * STATE;
-                    x[k][0] = shared_load2(w + d4);
-                    x[k][1] = shared_load2(w + d4 + 2);
-                    x[k][2] = shared_load2(w + 64);
+                    y[k][0] = shared_load2(w + d4);
+                    y[k][1] = shared_load2(w + d4 + 2);
+                    y[k][2] = shared_load2(w + 64);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     if (k0 + k >= n.splits) continue;
-                    const float mn = fmaxf(mm, x[k][2].x), f0 = __builtin_amdgcn_exp2f(mm - mn), f1 = __builtin_amdgcn_exp2f(x[k][2].x - mn);
+                    const float mn = fmaxf(mm, y[k][2].x), f0 = __builtin_amdgcn_exp2f(mm - mn), f1 = __builtin_amdgcn_exp2f(y[k][2].x - mn);
                     mm = mn;
-                    ll = fmaf(ll, f0, x[k][2].y * f1);
-                    o = f32x4{fmaf(o[0], f0, x[k][0].x * f1), fmaf(o[1], f0, x[k][0].y * f1), fmaf(o[2], f0, x[k][1].x * f1),
-                              fmaf(o[3], f0, x[k][1].y * f1)};
+                    ll = fmaf(ll, f0, y[k][2].y * f1);
+                    o = f32x4{fmaf(o[0], f0, y[k][0].x * f1), fmaf(o[1], f0, y[k][0].y * f1), fmaf(o[2], f0, y[k][1].x * f1),
+                              fmaf(o[3], f0, y[k][1].y * f1)};
                 }
             }
-        emit(t, mm, ll, o);
+        emit(t, mm, ll, o, x, in_memory);
     }
 }
 
-// LDS for the scores of alignment rows: 1504 positions of five queries fit
-constexpr long KEPT_FLOATS = 8192;
+// LDS for the scores of alignment rows: 1504 positions of five queries fit, so that three workgroups share a CU, or of sixteen
+// where each has one to itself
+constexpr long KEPT_FLOATS = 8192, KEPT_FLOATS_ALONE = 24576;
 long kept_queries(const Launch& n, long nq) { return std::min(nq, 16L * n.qt); }
 
 // Measured, us, 20 heads unless stated; a unit is a tile of a (row, cache head).
@@ -902,7 +936,7 @@ Launch attn_shape(const MzKv8& kv, const MzKv8Attn& a) {
     n.splits = (int)std::max(1L, std::min({cus / units, (long)kv.blocks / 10, 256L}));
     n.by_splits = inverse(n.splits);
     const long keep = ((long)kv.blocks + n.splits - 1) / n.splits * MZ_KV_BLK;
-    n.kept = a.align && keep * kept_queries(n, nq) <= KEPT_FLOATS ? (int)keep : 0;
+    n.kept = a.align && keep * kept_queries(n, nq) <= (units * n.splits <= cus ? KEPT_FLOATS_ALONE : KEPT_FLOATS) ? (int)keep : 0;
     return n;
 }
 static_assert(JOIN_COUNTERS >= 1024, "units that are shared have a counter each: fewer than the CUs");
