@@ -4,6 +4,7 @@
 #include "mz_kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -417,7 +418,9 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+// (the median of two numbers and infinity is the larger one. A maximum would make each operand quiet first, and so would a
+// median with an infinity that the compiler knows.)
+__device__ __forceinline__ float larger(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
 
 // what a row's queries see: token i positions first .. min(base + (causal ? i : 0), cap) - 1 of its slot
 struct Seen {
@@ -481,9 +484,11 @@ __device__ __forceinline__ int divided(int x, int d, unsigned r) {
 }
 constexpr int STATE = 66;  // floats of a query's partial state: 64 channels, maximum, sum
 
-// NW waves, which take the blocks in turn, or, with OWN, each 16 QT queries of its own and every block (no alignment rows).
+// NW waves, which take the blocks in turn, or, with OWN, each 16 QT queries of its own and every block (no alignment rows):
+// making fp16 of a block is then the four waves' common work, which meet once a block (8 prompts of 224 tokens over up to
+// 374 positions 13.4 us, 15.5 when each made its own, over 1500 positions 42 and 56).
 template <int FMT, int QT, bool ALIGN, int NW, bool OWN>
-__global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
+__global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
     static_assert(!(OWN && ALIGN));
     __shared__ float red[OWN ? 1 : NW][16][68], ms[NW][16], ls[NW][16];
     __shared__ float lse2s[16];
@@ -495,11 +500,13 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     const int tile = n.tiles - 1 - (int)blockIdx.y, split = blockIdx.z, grp = n.group;
     const int r = divided(pair, kv.heads, n.by_heads), kh = pair - r * kv.heads;
     const Seen s = seen_of(kv, a, r);
-    const int q0 = (OWN ? tile * NW + wave : tile) * 16 * QT, nq = a.tokens * grp, qn = min(q0 + 16 * QT, nq);  // these queries
-    if (OWN && q0 >= nq) return;
+    // the workgroup's queries, and this wave's
+    constexpr int SHARE = OWN ? NW : 1;
+    const int nq = a.tokens * grp, w0 = tile * 16 * QT * SHARE, wn = min(w0 + 16 * QT * SHARE, nq);
+    const int q0 = OWN ? w0 + 16 * QT * wave : w0, qn = min(q0 + 16 * QT, nq);
     auto token_of = [&](int x) { return divided(x, grp, n.by_group); };
-    if (token_of(q0) >= s.count) return;  // none of its tokens is there
-    const int hi = s.end(a, min(token_of(qn - 1), s.count - 1)), lo_end = s.end(a, token_of(q0));
+    if (token_of(w0) >= s.count) return;  // none of its tokens is there
+    const int lo_end = s.end(a, token_of(q0)), hi = s.end(a, min(token_of(wn - 1), s.count - 1));
     const int b_lo = s.first / MZ_KV_BLK, nb = max((hi + MZ_KV_BLK - 1) / MZ_KV_BLK - b_lo, 0);
     // (splits is at most 256, nb below 2^20)
     const int b0 = b_lo + (OWN || n.splits == 1 ? 0 : divided(nb * split, n.splits, n.by_splits));
@@ -518,7 +525,8 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     if constexpr (ALIGN)
         if (!n.kept) align_indices<64 * NW>(a, kh * grp, grp, mine, index);
     f16x8 qf[QT][2];
-    int end[QT];
+    int end[QT];  // what a lane's queries see ends here,
+    unsigned span[QT];  // and has these many positions
     float* al[QT];
     auto align_row = [&](int t) -> float* {
         const int x = q0 + 16 * t + c, i = token_of(x), k = x < nq && i < s.count ? index[x - i * grp] : -1;
@@ -532,6 +540,7 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
         qf[t][0] = on ? ld8(q) : f16x8{};
         qf[t][1] = on ? ld8(q + 8) : f16x8{};
         end[t] = on ? s.end(a, i) : 0;
+        span[t] = max(end[t] - s.first, 0);
         al[t] = ALIGN && !n.kept ? align_row(t) : nullptr;
     }
 
@@ -566,6 +575,8 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
         for (int u = 0; u < 4; u++) acc[t][u] = f32x4{};
     }
     const float scale2 = a.scale * LOG2E;
+    float inf = INFINITY;
+    asm("" : "+s"(inf));
     // P as one fp16 number, or as the sum of two where the products wait for memory anyway
     constexpr bool FINE = QT == 1 && !OWN;
     auto weighted = [&](f16x8 v, f16x8 p, f16x8 rest, f32x4 to) { return mfma16(v, p, FINE ? mfma16(v, rest, to) : to); };
@@ -573,11 +584,11 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
     struct Scales {
         float cs, vs, lg, rc;
     };
-    auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], const Scales& sc) {
+    auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], const Scales& sc, auto open_block) {
+        // the open block's fp16 numbers as they were given: any numbers, vs is 1 and says nothing about their size
+        constexpr bool given = decltype(open_block)::value;
         const int p0 = b * MZ_KV_BLK + 8 * g;  // this lane's positions
-        const float cs = sc.cs;
         const bool whole = b * MZ_KV_BLK >= s.first && (b + 1) * MZ_KV_BLK <= lo_end;  // seen by every query
-        const bool given = b == open;  // fp16 as it was given, any number: vs is 1 and says nothing about the numbers' size
         if (given ? unit == 0.f : sc.vs > unit) {
             const float to = given ? 9.5367431640625e-07f
                                    : __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, sc.vs) & 0x7f800000u) + 0x00800000u);
@@ -601,7 +612,11 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             if (!whole)
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    if (p0 + e < s.first || p0 + e >= end[t]) d[e >> 2][e & 3] = -INFINITY;
+                    if ((unsigned)(p0 - s.first + e) >= span[t]) d[e >> 2][e & 3] = -INFINITY;
+            // A block that a query does not see leaves it alone: codes are numbers, but the scales may be none, and so may be
+            // what was given.
+            const bool any = whole || b * MZ_KV_BLK < end[t];
+            const float cs = any ? sc.cs : 1.f;
             if (ALIGN && (n.kept ? 16 * t + c < qn - q0 : al[t] != nullptr)) {
                 const f32x4 x[2] = {d[0] * cs, d[1] * cs};
                 if (n.kept) {
@@ -616,9 +631,8 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
                         }
                 }
             }
-            // (the median of two numbers and infinity is the larger one; a maximum would make its operands quiet first)
-            const float top = cs * fmaxf(fmaxf(larger(d[0][0], d[0][1]), larger(d[0][2], d[0][3])),
-                                         fmaxf(larger(d[1][0], d[1][1]), larger(d[1][2], d[1][3])));
+            const float top = cs * fmaxf(fmaxf(larger(d[0][0], d[0][1], inf), larger(d[0][2], d[0][3], inf)),
+                                         fmaxf(larger(d[1][0], d[1][1], inf), larger(d[1][2], d[1][3], inf)));
             if (__ballot(top > m[t] + 8.f)) {
                 const float mn = fmaxf(m[t], column_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
@@ -630,10 +644,8 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             f16x8 p;
 #pragma unroll
             for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], cs, up - m[t]));
-            // (0 times a scale or a value that is no number is none: a query that does not see the block keeps its sums)
-            const bool any = whole || b * MZ_KV_BLK < end[t];
             const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            l[t] += any ? sum * down : 0.f;
+            l[t] += given && !any ? 0.f : sum * down;
             f16x8 rest = {};
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -641,18 +653,19 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
                 p[e] = (f16)hi;
                 if (FINE) rest[e] = (f16)(x[e] - hi);
             }
-            if (whole && direct) {
-#pragma unroll
-                for (int u = 0; u < 4; u++) acc[t][u] = weighted(vf[u], p, rest, acc[t][u]);
-            } else {
-                const float f = direct ? 1.f : sc.vs * per_unit;
+            if (!direct) {  // by itself, and nothing after it (no branch for the other case: the sums stay where they are)
+                const float f = any ? sc.vs * per_unit : 0.f;
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const f32x4 y = weighted(vf[u], p, rest, f32x4{});
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[t][u][e] = any ? fmaf(y[e], f, acc[t][u][e]) : acc[t][u][e];
+                    for (int e = 0; e < 4; e++) acc[t][u][e] = given && !any ? acc[t][u][e] : fmaf(y[e], f, acc[t][u][e]);
                 }
+                p = rest = f16x8{};
             }
+            if (!given)
+#pragma unroll
+                for (int u = 0; u < 4; u++) acc[t][u] = weighted(vf[u], p, rest, acc[t][u]);
         }
     };
     auto coded = [&](int b, const Raw& w, const Scales& sc) {
@@ -664,13 +677,13 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             vf[2 * j] = widen<FMT>(w.v[j][0], w.v[j][1]);
             vf[2 * j + 1] = widen<FMT>(w.v[j][2], w.v[j][3]);
         }
-        products(b, kf, vf, sc);
+        products(b, kf, vf, sc, std::false_type{});
     };
-    // Blocks b0 + wave, + 4, ...: DEPTH of them on their way. The open block, where it is this wave's, comes first; its codes
-    // are stale.
+    // Blocks b0 + wave, + NW, ..., or every block: DEPTH or AHEAD of them on their way. The open block, where it is this
+    // wave's, comes first; its codes are stale.
     // The scales of 60 of them lie in the lanes of two registers: scalar loads, which come back in any order, would have
     // every block wait for the newest of them.
-    constexpr int DEPTH = 2, WINDOW = 60, STEP = OWN ? 1 : NW;
+    constexpr int DEPTH = 2, WINDOW = 60, STEP = OWN ? 1 : NW, AHEAD = 2;
     Raw w[DEPTH];
     const int head = b0 + (OWN ? 0 : wave);
     if (head < b1) {
@@ -687,8 +700,16 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
         auto scales_of = [&](int i) {
             return Scales{lane_value(lanes.cs, i), lane_value(lanes.vs, i), lane_value(lanes.lg, i), lane_value(lanes.rc, i)};
         };
+        u32x4 raw[AHEAD];
+        const auto part = wave < 2 ? rk : rv;
+        const unsigned at0 = wave < 2 ? kat + 256 * wave : vat + 1024 * (wave - 2);
+        auto take = [&](int i) { return __builtin_amdgcn_raw_buffer_load_b128(part, at0, min(i, tail - b0) * MZ_KV_TILE, 0); };
+        if constexpr (OWN)
 #pragma unroll
-        for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
+            for (int i = 0; i < AHEAD; i++) raw[i] = take(i);
+        else
+#pragma unroll
+            for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
         scales(head);
         if (open >= b0 && open < b1 && (open - head) % STEP == 0) {
             f16x8 kf[2][2], vf[4];
@@ -706,20 +727,54 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
                     const int p = open * MZ_KV_BLK + 8 * g + e;
                     if (p < s.first || p >= hi) vf[j][e] = (f16)0.f;
                 }
-            products(open, kf, vf, Scales{scale2, 1.f, 0.f, 1.f});
+            products(open, kf, vf, Scales{scale2, 1.f, 0.f, 1.f}, std::true_type{});
         }
-        for (int b = head, at = 0; b <= tail; b += STEP * DEPTH, at += DEPTH) {
-            if (at == WINDOW) {
-                scales(b);
-                at = 0;
-            }
+        if constexpr (OWN) {
+            // Each wave makes fp16 of a quarter of a block (waves 0 and 1 of the keys) and puts it where all find it, a block
+            // ahead; what is behind the last block is that one again.
+            __shared__ f16x8 pieces[2][8][64];
+            auto put = [&](int b, const u32x4& x) {
+                pieces[b & 1][2 * wave][lane] = widen<FMT>(x[0], x[1]);
+                pieces[b & 1][2 * wave + 1][lane] = widen<FMT>(x[2], x[3]);
+            };
+            const int own_end = q0 < nq && token_of(q0) < s.count ? s.end(a, min(token_of(qn - 1), s.count - 1)) : 0;
+            put(0, raw[0]);
+            __syncthreads();
+            for (int w0 = 0; w0 <= tail - b0; w0 += WINDOW) {
+                if (w0) scales(b0 + w0);
+                const int w1 = min(w0 + WINDOW, tail - b0 + 1);
+                for (int i0 = w0; i0 < w1; i0 += AHEAD)
 #pragma unroll
-            for (int i = 0; i < DEPTH; i++) {
-                const int bi = b + STEP * i;
-                if (bi <= tail && bi != open) coded(bi, w[i], scales_of(at + i));
-                fetch(bi + STEP * DEPTH, w[i]);
+                    for (int j = 0; j < AHEAD; j++) {
+                        const int i = i0 + j, b = b0 + i;
+                        if (i >= w1) break;
+                        raw[j] = take(i + AHEAD);
+                        put(i + 1, raw[(j + 1) % AHEAD]);
+                        if (b * MZ_KV_BLK < own_end && b != open) {
+                            f16x8 kf[2][2], vf[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                kf[k >> 1][k & 1] = pieces[i & 1][k][lane];
+                                vf[k] = pieces[i & 1][4 + k][lane];
+                            }
+                            products(b, kf, vf, scales_of(i - w0), std::false_type{});
+                        }
+                        __syncthreads();
+                    }
             }
-        }
+        } else
+            for (int b = head, at = 0; b <= tail; b += STEP * DEPTH, at += DEPTH) {
+                if (at == WINDOW) {
+                    scales(b);
+                    at = 0;
+                }
+#pragma unroll
+                for (int i = 0; i < DEPTH; i++) {
+                    const int bi = b + STEP * i;
+                    if (bi <= tail && bi != open) coded(bi, w[i], scales_of(at + i));
+                    fetch(bi + STEP * DEPTH, w[i]);
+                }
+            }
     }
 
     // accumulator u of lane (c, g) holds channels 32 (u / 2) + 8 g + 2 e + u % 2 of query c
@@ -865,7 +920,8 @@ __global__ void __launch_bounds__(64 * NW, QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv
             for (unsigned has = rows(t); has; has &= has - 1) {
                 const int k = __ffs(has) - 1;
                 float* const row = row_of_query(t, k);
-                for (int p = b0 * MZ_KV_BLK + tid; p < min(b1 * MZ_KV_BLK, a.align_cols); p += STRIDE) shared_store(row + p, in_lds(16 * t + k, row, p));
+                for (int p = b0 * MZ_KV_BLK + tid; p < min(b1 * MZ_KV_BLK, a.align_cols); p += STRIDE)
+                    shared_store(row + p, in_lds(16 * t + k, row, p));
             }
         if (t + 1 < QT) __syncthreads();
     }
