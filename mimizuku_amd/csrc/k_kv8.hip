@@ -439,6 +439,11 @@ __device__ __forceinline__ Seen seen_of(const MzKv8& kv, const MzKv8Attn& a, int
         first = *(a.first ? a.first + r : kv.open);
         len = *(a.len ? a.len + (long)r * a.len_stride : kv.open);
         count = *(a.count ? a.count + r : kv.open);
+        slot = __builtin_amdgcn_readfirstlane(slot);
+        first = __builtin_amdgcn_readfirstlane(first);
+        len = __builtin_amdgcn_readfirstlane(len);
+        count = __builtin_amdgcn_readfirstlane(count);
+        asm("" : "+s"(slot), "+s"(first), "+s"(len), "+s"(count));  // (none is used before all are here)
     }
     Seen s;
     s.slot = a.slot ? slot : r;
@@ -495,8 +500,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     // x: (row, cache head), padded to a multiple of the XCDs, so that what shares keys and values shares an XCD; y: the tiles,
     // those that see most first; z: the shares of the blocks
-    const int pair = blockIdx.x;
-    if (pair >= a.rows * (long)kv.heads) return;
+    const int pairs = a.rows * kv.heads, pair = min((int)blockIdx.x, pairs - 1);
     const int tile = n.tiles - 1 - (int)blockIdx.y, split = blockIdx.z, grp = n.group;
     const int r = divided(pair, kv.heads, n.by_heads), kh = pair - r * kv.heads;
     const Seen s = seen_of(kv, a, r);
@@ -505,7 +509,8 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     const int nq = a.tokens * grp, w0 = tile * 16 * QT * SHARE, wn = min(w0 + 16 * QT * SHARE, nq);
     const int q0 = OWN ? w0 + 16 * QT * wave : w0, qn = min(q0 + 16 * QT, nq);
     auto token_of = [&](int x) { return divided(x, grp, n.by_group); };
-    if (token_of(w0) >= s.count) return;  // none of its tokens is there
+    // (one way out, behind the first loads)
+    if ((int)blockIdx.x >= pairs || token_of(w0) >= s.count) return;  // none of its tokens is there
     const int lo_end = s.end(a, token_of(q0)), hi = s.end(a, min(token_of(wn - 1), s.count - 1));
     const int b_lo = s.first / MZ_KV_BLK, nb = max((hi + MZ_KV_BLK - 1) / MZ_KV_BLK - b_lo, 0);
     // (splits is at most 256, nb below 2^20)
@@ -513,7 +518,9 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     const int b1 = b_lo + (OWN || n.splits == 1 ? nb : divided(nb * (split + 1), n.splits, n.by_splits));
 
     const long sh = s.slot * kv.heads + kh;
-    const int open_word = kv.open[sh], open = s.cap ? open_word - 1 : -1;
+    int zero = 0;
+    asm("" : "+v"(zero));
+    const int open_word = kv.open[sh + zero];  // (a vector load: the scalar ones would all be waited for together)
     const unsigned char* kc = kv.k + sh * kv.blocks * MZ_KV_TILE;
     const unsigned char* vc = kv.v + sh * kv.blocks * MZ_KV_TILE;
     const float* ksc = kv.k_scale + sh * kv.blocks;
@@ -711,6 +718,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
 #pragma unroll
             for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
         scales(head);
+        const int open = s.cap ? __builtin_amdgcn_readfirstlane(open_word) - 1 : -1;
         if (open >= b0 && open < b1 && (open - head) % STEP == 0) {
             f16x8 kf[2][2], vf[4];
             const f16* ko = kv.k_open + sh * MZ_KV_TILE;
