@@ -271,6 +271,9 @@ struct Writer {
     }
 };
 
+// 8 x 1500 positions of 20 heads (92 MB in and out) 20.0 us, 4.6 TB/s: the stream and ~345 vector instructions a side of a
+// block, nearly half of that time on every SIMD, hide each other in part. One position of 32 rows 5.1 us, a chain of four loads.
+//
 // Workgroup 0 of a (row, head) takes its first and its last block, which may want the open block and may leave one: a wave
 // for the keys and one for the values of each. The others take the blocks between, 2 * per each, whose positions are all new:
 // every wave `per` of keys or of values, the next one's on their way while one is coded.
@@ -314,7 +317,8 @@ __global__ void __launch_bounds__(256) write_kernel(MzKv8 kv, MzKv8Io a, int per
     if (threadIdx.x == 0) kv.open[sh] = (w.p + w.n) % MZ_KV_BLK ? last + 1 : 0;
 }
 
-// a workgroup: keys and values of two blocks of a (row, head), a wave each
+// a workgroup: keys and values of two blocks of a (row, head), a wave each (8 x 1500 positions of 20 heads, 92 MB in and out,
+// 16.6 us, 5.6 TB/s; a copy reaches 6.6)
 template <int FMT>
 __global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), side = wave & 1;
@@ -383,8 +387,13 @@ long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std:
 // ---------------------------------------------------------------- attention
 //
 // One pass over the cache with the running maximum and sum of the softmax. A workgroup takes 16 QT queries of one (row,
-// cache head) (its tokens times the query heads that share the cache head) and a share of the blocks; its four waves
-// take the blocks in turn, each with a state of its own, and join them at the end.
+// cache head) (its tokens times the query heads that share the cache head) and a share of the blocks; its waves take the
+// blocks in turn, each with a state of its own, and join them at the end.
+//
+// Bound by memory for single tokens: 4,104 bytes a block, of which 32 rows x 20 heads x 1500 positions (126 MB) take 23.6 us,
+// 6.7 TB/s behind the ~5 us of the launch and of the round trips to the first key and from the last (25.9 with six alignment
+// heads). One row: those round trips, 7.6 us. Prompts: vector instructions, about 95 a block of 16 queries (8 prompts of 224
+// tokens over up to 374 positions 13.2 us).
 //
 // Per block of 32 positions, with 16x16x32 products: S^T = K Q^T, the rows of tile j being positions 8 (i / 4) + 4 j + i % 4,
 // so that lane (query c, group g) of the two results holds the eight positions 8 g .. 8 g + 7 of its query. These
@@ -395,9 +404,9 @@ long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std:
 // Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' (as a
 // multiple of the state's unit, a power of two above every scale so far) into P before its rounding, or, where it is
 // below 2^-7 of the unit, into the block's product after it. With up to 16 queries, where the kernel waits for memory, P goes
-// into its product as the sum of two fp16 numbers (22 bits: the error is the output's own rounding; 32 rows of 1500 27.4 us
-// with one, 27.9 with two). With more it is rounded to one, half a step 2^-11 relative, as the output is (prompts of 224
-// tokens 16.0 us, 19.5 with two). P is at most 2^8: the maximum of a state is moved only when a score passes it by more than
+// into its product as the sum of two fp16 numbers (22 bits: the error is the output's own rounding; 32 rows of 1500 25.6 us
+// with one, 26.0 with two). With more it is rounded to one, half a step 2^-11 relative, as the output is (8 prompts of 224
+// tokens 13.1 us, 14.3 with two). P is at most 2^8: the maximum of a state is moved only when a score passes it by more than
 // 8 (in powers of two), so that most blocks need no exchange between lanes and no rescaling.
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
@@ -970,15 +979,15 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
 constexpr long KEPT_FLOATS = 8192, KEPT_FLOATS_ALONE = 24576;
 long kept_queries(const Launch& n, long nq) { return std::min(nq, 16L * n.qt); }
 
-// Measured, us, 20 heads unless stated; a unit is a tile of a (row, cache head).
+// Measured, us, 20 heads unless stated, no alignment rows; a unit is a tile of a (row, cache head).
 // Up to 16 queries: a tile of 16, and no more units than CUs: eight waves each instead of four (1500 positions, 160 units
-// 11.2 / 13.1, five beams of 256 units 12.1 / 13.7, but 260 units 16.8 / 15.9, 640 units 26.1 / 24.8), and with fewer
-// than half as many, the blocks shared by more workgroups until there is one a CU or a wave has about a block left (1500
-// positions of one row 10.6 with one workgroup, 8.8 with 2, 7.9 with 4, 8.2 with 6; 80 units 10.1, 9.4 with 2, 10.3 with 4;
-// 16,000 positions of 48 units 53 with one, 18.9 with 5, 20.6 with 8).
-// More queries: each wave 16 of its own, where that gives every CU a workgroup (40-token prompts of 8 rows 7.8, the waves taking
-// blocks in turn 8.9; 224 tokens 15.6 / 16.7), else tiles of 32 whose waves take the blocks in turn (224 tokens of one row
-// 8.3 / 10.7, of 3 rows 9.9 / 11.2).
+// 10.8 / 11.1, five beams of 256 units 10.8 / 11.4, but 260 units 15.7 / 14.4, 640 units 24.6 / 23.6), and with fewer than
+// half as many, the blocks shared by more workgroups until there is one a CU or a wave has about a block left (1500 positions
+// of one row 10.2 with one workgroup, 8.9 with 2, 7.5 with 4, 7.7 with 6; 80 units 10.2, 9.0 with 3, 10.2 with 4; 16,000
+// positions of 48 units 46 with one, 17.8 with 5, 19.7 with 8).
+// More queries: each wave 16 of its own, where that gives every CU a workgroup (224-token prompts of 8 rows 13.2, the waves
+// taking blocks in turn 14.7; 40 tokens of 16 rows 9.1 / 9.9), else tiles of 32 whose waves take the blocks in turn (224 tokens
+// of one row 7.6 / 10.0, of 3 rows 8.9 / 10.5).
 Launch attn_shape(const MzKv8& kv, const MzKv8Attn& a) {
     const long nq = (long)a.tokens * (a.heads / kv.heads), cus = mz_cu_count(), pairs = (long)a.rows * kv.heads;
     auto inverse = [](int d) { return (unsigned)std::min((1ULL << 32) / d, 0xffffffffULL); };

@@ -4,6 +4,11 @@
 // With m a row's maximum, at element i0, S the sum of exp(x - m) over the others and U that of exp(x - m)(x - m):
 // ln sum exp x = m + log1p(S), log p = (x - m) - log1p(S), entropy = log1p(S) - U / (1 + S). The last two terms are both
 // positive and S does not hold the 1 of the maximum, so that sure rows (S far below 1) keep their digits.
+//
+// Many rows are bound by memory: 7,040 rows of 51,866 fp32 logits (1.46 GB) 220 us, 6.65 TB/s, which is why a wave works on
+// 1024 elements while the next are on their way and looks for alternatives only where a chunk's best passes the list. One row
+// is a chain of dependent steps, 8.6 us: launch and logits 3.5, joining its 13 workgroups 1.9, five alternatives 3.6 (the lists
+// of the waves, and of the parts); 32 rows 10.8.
 #include <algorithm>
 
 #include "mz_common.h"
