@@ -128,7 +128,8 @@ int mz_mel_transpose(mz_ctx* c, uint64_t mel, uint64_t melT, int clips, int n_me
  *   MZ_KV8_E4M3: c an OCP e4m3 number,    scale = f32(top / 448), c = 448 x / top to the nearest, halves to even
  * where top is the block's largest magnitude (0: scale 0 and codes 0). A block is coded when its last position is
  * written; until then it is the open block of its (slot, head) (at most one) and holds its positions in fp16 as they
- * were given. A block with a NaN or an infinity in it gets the scale NaN: all of its positions stand for NaN. */
+ * were given. A block with a NaN or an infinity in it gets the scale NaN: all of its positions stand for NaN (codes are
+ * numbers: e4m3's own NaN is no code). */
 #define MZ_KV8_I8 0
 #define MZ_KV8_E4M3 1
 #define MZ_KV8_BLOCK 32

@@ -549,7 +549,7 @@ def test_alignment_rows(ctx, dev, fmt, tokens, heads, kvh, cols):
 
 @pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("rows,heads,tokens", [(10, 16, 5), (3, 7, 1), (20, 16, 1), (17, 16, 3), (10, 16, 6), (1, 2, 30),
-                                               (9, 15, 33)])
+                                               (9, 15, 33), (11, 12, 16), (9, 15, 16)])
 def test_alignment_rows_of_long_caches(ctx, dev, fmt, rows, heads, tokens):
     """The encoder's 1500 positions: scores kept by a workgroup (the most that are) or in their rows, by one workgroup or
     several that share the blocks, of four and of eight waves."""
@@ -577,6 +577,20 @@ def test_attention_of_many_rows(ctx, dev, fmt, rows, heads, kvh, tokens):
     length, first = [p + 1 for p in past], [r % 3 for r in range(rows)]
     for causal in (True, False):
         check_attention(b, q, run_attention(ctx, dev, b, q, causal, length, first=first, count=cnt), causal, length, first=first, count=cnt)
+    b.free()
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("rows,heads,tokens,length", [(16, 16, 1, 15700), (17, 16, 1, 8000), (17, 8, 20, 8000), (16, 16, 20, 2600)])
+def test_attention_over_more_blocks_than_a_wave_has_scales_of(ctx, dev, fmt, rows, heads, tokens, length):
+    """More than 60 blocks a wave, of eight and four waves and of waves with queries of their own; rows that share a slot."""
+    rng = np.random.default_rng(length)
+    b = filled(ctx, dev, rng, 1, heads, [length], fmt)
+    q = f16(rng, (rows, tokens, heads, 64), 1.5)
+    lens, slot = [length - 37 * r - tokens + 1 for r in range(rows)], [0] * rows
+    for first in (None, [61 * r for r in range(rows)]):
+        got = run_attention(ctx, dev, b, q, True, lens, slot=slot, first=first)
+        check_attention(b, q, got, True, lens, slot=slot, first=first)
     b.free()
 
 
