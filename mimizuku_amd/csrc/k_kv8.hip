@@ -538,8 +538,6 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     extern __shared__ float kept[];  // [query][n.kept]
     __shared__ int index[ALIGN ? 64 : 1];
     const int mine = ALIGN && tid < a.heads ? a.head_slot[tid] : -1;
-    if constexpr (ALIGN)
-        if (!n.kept) align_indices<64 * NW>(a, kh * grp, grp, mine, index);
     f16x8 qf[QT][2];
     int end[QT];  // what a lane's queries see ends here,
     unsigned span[QT];  // and has these many positions
@@ -557,7 +555,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
         qf[t][1] = on ? ld8(q + 8) : f16x8{};
         end[t] = on ? s.end(a, i) : 0;
         span[t] = max(end[t] - s.first, 0);
-        al[t] = ALIGN && !n.kept ? align_row(t) : nullptr;
+        al[t] = nullptr;
     }
 
     // A coded block as it lies. Blocks past this workgroup's share read as zeros, without a memory access: the loads need no
@@ -633,7 +631,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
             // what was given.
             const bool any = whole || b * MZ_KV_BLK < end[t];
             const float cs = any ? sc.cs : 1.f;
-            if (ALIGN && (n.kept ? 16 * t + c < qn - q0 : al[t] != nullptr)) {
+            if (ALIGN && al[t] != nullptr) {
                 const f32x4 x[2] = {d[0] * cs, d[1] * cs};
                 if (n.kept) {
                     f32x4* o = (f32x4*)(kept + (16 * t + c) * n.kept + p0 - b0 * MZ_KV_BLK);
@@ -702,6 +700,14 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     constexpr int DEPTH = 2, WINDOW = 60, STEP = OWN ? 1 : NW, AHEAD = 2;
     Raw w[DEPTH];
     const int head = b0 + (OWN ? 0 : wave);
+    if constexpr (!OWN)
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
+    if constexpr (ALIGN) {  // (while they are on their way)
+        align_indices<64 * NW>(a, kh * grp, grp, mine, index);
+#pragma unroll
+        for (int t = 0; t < QT; t++) al[t] = align_row(t);
+    }
     if (head < b1) {
         const int tail = head + (b1 - 1 - head) / STEP * STEP;
         Scales lanes;
@@ -723,9 +729,6 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
         if constexpr (OWN)
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) raw[i] = take(i);
-        else
-#pragma unroll
-            for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
         scales(head);
         const int open = s.cap ? __builtin_amdgcn_readfirstlane(open_word) - 1 : -1;
         if (open >= b0 && open < b1 && (open - head) % STEP == 0) {
@@ -812,12 +815,6 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
         }
         return;
     }
-    if constexpr (ALIGN)
-        if (n.kept) {
-            align_indices<64 * NW>(a, kh * grp, grp, mine, index);
-#pragma unroll
-            for (int t = 0; t < QT; t++) al[t] = align_row(t);
-        }
     // the waves' states joined, 16 queries at a time, by the first 256 threads
     const int col = tid >> 4 & 15, d4 = (tid & 15) * 4;
     const bool mine256 = NW == 4 || tid < 256;
