@@ -95,6 +95,11 @@ __device__ __forceinline__ Key other_half(Key k, int lane) {
     const auto l = __builtin_amdgcn_permlane32_swap((unsigned)k, (unsigned)k, false, false);
     return lane & 32 ? (Key)(unsigned)h[0] << 32 | (unsigned)l[0] : (Key)(unsigned)h[1] << 32 | (unsigned)l[1];
 }
+// the best 16 of the four rows' sorted ones, best first, in every row
+__device__ __forceinline__ Key best_of_rows(Key k, int lane) {
+    k = joined(k, other_row(k, lane), lane);
+    return joined(k, other_half(k, lane), lane);
+}
 // the best 16 of the wave's 64 keys, best first, in every row
 __device__ __forceinline__ Key best16(Key k, int lane) {
     k = step(k, moved<0xB1>(k), !(lane & 1));
@@ -107,13 +112,20 @@ __device__ __forceinline__ Key best16(Key k, int lane) {
     k = step(k, (Key)(unsigned)xor4((int)(k >> 32)) << 32 | (unsigned)xor4((int)k), !(lane & 4));
     k = step(k, moved<0x4E>(k), !(lane & 2));
     k = step(k, moved<0xB1>(k), !(lane & 1));
-    k = joined(k, other_row(k, lane), lane);
-    return joined(k, other_half(k, lane), lane);
+    return best_of_rows(k, lane);
 }
-// LDS written by other lanes of the wave is read behind this (a wave's LDS operations run in order; the compiler is told so)
-__device__ __forceinline__ void wave_lds() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+// the best 16 of n <= 16 parts' lists, a row of lanes each
+__device__ __forceinline__ Key best_of_parts(const float* part, int n, int alts, int lane) {
+    const int words = HEAD + 2 * alts, k = lane & 15;
+    Key r[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int i = 4 * j + (lane >> 4);
+        r[j] = i < n && k < alts ? *(const Key*)(part + i * words + HEAD + 2 * k) : 0;
+    }
+    if (n > 4) r[0] = joined(r[0], r[1], lane);
+    if (n > 8) r[0] = joined(r[0], joined(r[2], r[3], lane), lane);
+    return best_of_rows(r[0], lane);
 }
 // the lane with the largest of the wave's keys (v: their values), at least one of them not 0
 __device__ __forceinline__ int best_lane(float v, Key k) {
@@ -126,12 +138,11 @@ __device__ __forceinline__ int best_lane(float v, Key k) {
     return lane;
 }
 
-// The row's results from its parts (words as above, one lane each). The alternatives are taken one after the other from the
-// parts' lists. tok, xt: the given token and its logit.
-__device__ __forceinline__ void finish(const MzScores& p, long o, const float* part, int parts, int lane, int tok, float xt, Key (&pick)[64]) {
+// The row's results from its parts (words as above, one lane each) and its alternatives (lane k of a row of lanes: k). tok, xt:
+// the given token and its logit.
+__device__ __forceinline__ void finish(const MzScores& p, long o, const float* part, int parts, int lane, int tok, float xt, Key list) {
     const bool on = lane < parts;
-    const int words = HEAD + 2 * p.alts;
-    const float* mine = part + (on ? lane * words : 0);
+    const float* mine = part + (on ? lane * (HEAD + 2 * p.alts) : 0);
     const float mi = on ? mine[0] : -INFINITY, si = on ? mine[1] : 0.f, ui = on ? mine[2] : 0.f;
     const float m = wave_max(mi);
     // one of the parts with the row's maximum holds the element that S leaves out; the others' maxima count in it
@@ -145,28 +156,6 @@ __device__ __forceinline__ void finish(const MzScores& p, long o, const float* p
     if (lane == 0 && p.logp)
         p.logp[o] = tok < 0 ? 0.f : bad || tok >= p.vocab ? NAN : m == -INFINITY || xt == -INFINITY ? -INFINITY : (xt - m) - z;
     if (lane == 0 && p.entropy) p.entropy[o] = bad ? NAN : m == -INFINITY ? 0.f : z - U / (1.f + S);
-    if (!p.alts) return;
-    auto entry = [&](int k) -> Key {  // of the lane's list
-        return on && k < p.alts ? *(const Key*)(mine + HEAD + 2 * k) : 0;
-    };
-    Key x = entry(0), list = 0;
-    if (p.alts <= 10) {
-        // the part whose best is q-th has no more than alts - q of the row's: 55 at most
-        const Key firsts = best16(x, lane);
-        int q = x ? 0 : 64;
-        for (int k = 0; k < p.alts; k++) q += lane_key(firsts, k) > x;
-        pick[lane] = 0;
-        wave_lds();
-        if (q < p.alts)
-            for (int k = 0; k + q < p.alts; k++) pick[q * p.alts - q * (q - 1) / 2 + k] = entry(k);
-        wave_lds();
-        list = best16(pick[lane], lane);
-    } else
-        for (int k = 0, at = 0; k < p.alts; k++) {
-            const int l = best_lane(value_of(x), x);
-            if (lane == k) list = lane_key(x, l);
-            if (lane == l) x = entry(++at);
-        }
     if (lane >= p.alts) return;
     if (p.alt_ids) p.alt_ids[o * p.alts + lane] = bad || !list ? -1 : id_of(list);
     if (p.alt_logp) p.alt_logp[o * p.alts + lane] = bad ? NAN : list ? (value_of(list) - m) - z : -INFINITY;
@@ -179,7 +168,7 @@ __global__ void __launch_bounds__(256) score_kernel(MzScores p, int splits) {
     constexpr int V = 16 / sizeof(T), G = PER_LANE / V;  // elements of a 16-byte load, loads of a chunk
     typedef T TV __attribute__((ext_vector_type(V)));
     __shared__ __attribute__((aligned(8))) float lds[PARTS * MOST];
-    __shared__ Key pick[64];
+    __shared__ Key lists[64];  // of the waves' shares of the parts
     __shared__ Key bound;  // no element with a smaller key is an alternative of the row
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = blockIdx.x / splits, split = blockIdx.x - r * splits;
@@ -199,6 +188,7 @@ __global__ void __launch_bounds__(256) score_kernel(MzScores p, int splits) {
     auto from = [&](int e) { return max(min(e, p.vocab - V), 0); };
 
     float m = -INFINITY, S = 0.f, U = 0.f;  // m of the wave, the sums of the lane
+    bool first = true;        // nothing is in the list
     Key list = 0, least = 0;  // lane k of each row: alternative k; the last one, or a larger bound that another wave found
     // the given token and its logit, which each wait for a load
     const int tok = p.logp && n < p.token_stride ? p.tokens[r * p.token_stride + n] : -1;
@@ -292,7 +282,8 @@ __global__ void __launch_bounds__(256) score_kernel(MzScores p, int splits) {
             if (!can) break;
             bool next;  // the lane's best is in the list, or not as good as what is
             if (p.alts > 1 && (can & (can - 1))) {
-                list = joined(list, best16(mine, lane), lane);
+                list = first ? best16(mine, lane) : joined(list, best16(mine, lane), lane);
+                first = false;
                 const Key last = lane_key(list, p.alts - 1);
                 next = mine && mine >= last;
                 least = max(least, last);
@@ -303,6 +294,7 @@ __global__ void __launch_bounds__(256) score_kernel(MzScores p, int splits) {
                 list = row16 < place ? list : row16 == place ? in : before;
                 least = max(least, lane_key(list, p.alts - 1));
                 next = lane == l;
+                first = false;
             }
             float second = -INFINITY;
 #pragma unroll
@@ -345,7 +337,16 @@ __global__ void __launch_bounds__(256) score_kernel(MzScores p, int splits) {
         }
         __syncthreads();
     }
-    if (wave == 0) finish(p, r * p.out_stride + n, lds, 4 * splits, lane, tok, left_out ? -INFINITY : xt, pick);
+    Key best = 0;
+    if (p.alts && splits == 1) {
+        if (wave == 0) best = best_of_parts(lds, 4, p.alts, lane);
+    } else if (p.alts) {
+        best = best_of_parts(lds + wave * splits * words, splits, p.alts, lane);
+        if (lane < 16) lists[wave * 16 + lane] = best;
+        __syncthreads();
+        best = best_of_rows(lists[lane], lane);
+    }
+    if (wave == 0) finish(p, r * p.out_stride + n, lds, 4 * splits, lane, tok, left_out ? -INFINITY : xt, best);
 }
 
 int score_splits(const MzScores& p) {
