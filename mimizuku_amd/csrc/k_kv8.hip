@@ -271,8 +271,8 @@ struct Writer {
     }
 };
 
-// 8 x 1500 positions of 20 heads (92 MB in and out) 20.0 us, 4.6 TB/s: the stream and ~345 vector instructions a side of a
-// block, nearly half of that time on every SIMD, hide each other in part. One position of 32 rows 5.1 us, a chain of four loads.
+// 8 x 1500 positions of 20 heads (92 MB in and out) 19.8 us, 4.7 TB/s: a copy would take 14 behind the launch and the first round
+// trips; the quotients' correction is 0.8. One position of 32 rows 5.0 us, a chain of four loads.
 //
 // Workgroup 0 of a (row, head) takes its first and its last block, which may want the open block and may leave one: a wave
 // for the keys and one for the values of each. The others take the blocks between, 2 * per each, whose positions are all new:
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(256) write_kernel(MzKv8 kv, MzKv8Io a, int per
 }
 
 // a workgroup: keys and values of two blocks of a (row, head), a wave each (8 x 1500 positions of 20 heads, 92 MB in and out,
-// 16.6 us, 5.6 TB/s; a copy reaches 6.6)
+// 16.4 us, 5.6 TB/s; a copy reaches 6.6)
 template <int FMT>
 __global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), side = wave & 1;
@@ -391,9 +391,9 @@ long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std:
 // blocks in turn, each with a state of its own, and join them at the end.
 //
 // Bound by memory for single tokens: 4,104 bytes a block, of which 32 rows x 20 heads x 1500 positions (126 MB) take 23.6 us,
-// 6.7 TB/s behind the ~5 us of the launch and of the round trips to the first key and from the last (25.9 with six alignment
-// heads). One row: those round trips, 7.6 us. Prompts: vector instructions, about 95 a block of 16 queries (8 prompts of 224
-// tokens over up to 374 positions 13.2 us).
+// 6.7 TB/s behind the ~5 us of the launch and of the round trips to the first key and from the last (25.2 with six alignment
+// heads). One row: those round trips, 7.5 us (8.7). Prompts: vector instructions, about 95 a block of 16 queries (8 prompts of 224
+// tokens over up to 374 positions 13.0 us).
 //
 // Per block of 32 positions, with 16x16x32 products: S^T = K Q^T, the rows of tile j being positions 8 (i / 4) + 4 j + i % 4,
 // so that lane (query c, group g) of the two results holds the eight positions 8 g .. 8 g + 7 of its query. These
