@@ -403,10 +403,9 @@ long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std:
 //
 // Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' (as a
 // multiple of the state's unit, a power of two above every scale so far) into P before its rounding, or, where it is
-// below 2^-7 of the unit, into the block's product after it. With up to 16 queries, where the kernel waits for memory, P goes
-// into its product as the sum of two fp16 numbers (22 bits: the error is the output's own rounding; 32 rows of 1500 25.6 us
-// with one, 26.0 with two). With more it is rounded to one, half a step 2^-11 relative, as the output is (8 prompts of 224
-// tokens 13.1 us, 14.3 with two). P is at most 2^8: the maximum of a state is moved only when a score passes it by more than
+// below 2^-7 of the unit, into the block's product after it. P goes into its product as the sum of two fp16 numbers (22
+// bits), so that the error is the output's own rounding whatever the number of queries (one would add half a step 2^-11
+// relative). P is at most 2^8: the maximum of a state is moved only when a score passes it by more than
 // 8 (in powers of two), so that most blocks need no exchange between lanes and no rescaling.
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
@@ -591,9 +590,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     const float scale2 = a.scale * LOG2E;
     float inf = INFINITY;
     asm("" : "+s"(inf));
-    // P as one fp16 number, or as the sum of two where the products wait for memory anyway
-    constexpr bool FINE = QT == 1 && !OWN;
-    auto weighted = [&](f16x8 v, f16x8 p, f16x8 rest, f32x4 to) { return mfma16(v, p, FINE ? mfma16(v, rest, to) : to); };
+    auto weighted = [&](f16x8 v, f16x8 p, f16x8 rest, f32x4 to) { return mfma16(v, p, mfma16(v, rest, to)); };
     // A block's scales: cs the keys' in the exponent (of two), vs the values', with its logarithm and reciprocal.
     struct Scales {
         float cs, vs, lg, rc;
@@ -660,12 +657,12 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
             for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], cs, up - m[t]));
             const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             l[t] += given && !any ? 0.f : sum * down;
-            f16x8 rest = {};
+            f16x8 rest;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float hi = FINE ? __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x[e]) & 0xffffe000u) : x[e];
+                const float hi = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x[e]) & 0xffffe000u);
                 p[e] = (f16)hi;
-                if (FINE) rest[e] = (f16)(x[e] - hi);
+                rest[e] = (f16)(x[e] - hi);
             }
             if (!direct) {  // by itself, and nothing after it (no branch for the other case: the sums stay where they are)
                 const float f = any ? sc.vs * per_unit : 0.f;
