@@ -35,6 +35,33 @@ __device__ __forceinline__ f16x8 widen(unsigned lo, unsigned hi) {
     return f16x8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
 
+// eight codes as bf16, whose 8 bits hold every code of either format
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+template <int FMT>
+__device__ __forceinline__ bf16x8 widen_bf16(unsigned lo, unsigned hi) {
+    u32x4 r;
+    if (FMT == I8) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {  // (the high halves of two 32-bit numbers)
+            const unsigned w = (i & 2 ? hi : lo) >> (i & 1) * 16;
+            const float a = (float)(signed char)w, b = (float)(signed char)(w >> 8);
+            r[i] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+        }
+    } else {
+        r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+        r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+        r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+        r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+    }
+    return __builtin_bit_cast(bf16x8, r);
+}
+
+// a pair of fp16 numbers of eight bits as bf16
+__device__ __forceinline__ unsigned as_bf16(f16x2 v) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, (float)v[1]), __builtin_bit_cast(unsigned, (float)v[0]), 0x07060302u);
+}
+
 // f16(f32(code * scale)). The product is kept from the compiler: it would fold it and the conversion into one mixed-width
 // multiply-add of a positive zero, which rounds once and makes -0 to +0.
 __device__ __forceinline__ f16 stands_for(f16 code, float scale) {
@@ -401,12 +428,11 @@ long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std:
 // other in registers, with no exchange between lanes. The values are kept so that one 16-byte load gives a lane
 // both channels 2 p and 2 p + 1 of its eight positions, the keys so that one gives 16 channels of a position.
 //
-// Codes become fp16 exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values' (as a
-// multiple of the state's unit, a power of two above every scale so far) into P before its rounding, or, where it is
-// below 2^-7 of the unit, into the block's product after it. P goes into its product as the sum of two fp16 numbers (22
-// bits), so that the error is the output's own rounding whatever the number of queries (one would add half a step 2^-11
-// relative). P is at most 2^8: the maximum of a state is moved only when a score passes it by more than
-// 8 (in powers of two), so that most blocks need no exchange between lanes and no rescaling.
+// Codes become numbers of 16 bits exactly, the products sum in 32 bits, the keys' scale goes into the exponent, the values'
+// into P. P goes into its product as the sum of two bf16 numbers: 16 bits (each rounding is at most 2^-8 of what it rounds),
+// so that the error is the output's own rounding, and of the range of 32 bits, so that many positions far below a row's
+// largest keep their share (two fp16 numbers end at 2^-24). The maximum of a state is moved only when a score passes it by more
+// than 8 (in powers of two), so that most blocks need no exchange between lanes and no rescaling.
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
 
@@ -420,6 +446,11 @@ __device__ __forceinline__ float column_sum(float v) {
     const unsigned u = __builtin_bit_cast(unsigned, v);
     const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     return pair32_sum(__builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]));
+}
+
+// v p for p = high + low
+__device__ __forceinline__ f32x4 weighted(bf16x8 v, bf16x8 high, bf16x8 low, f32x4 to) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, high, __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, low, to, 0, 0, 0), 0, 0, 0);
 }
 
 __device__ __forceinline__ float lane_value(float v, int lane) {
@@ -498,7 +529,7 @@ __device__ __forceinline__ int divided(int x, int d, unsigned r) {
 constexpr int STATE = 66;  // floats of a query's partial state: 64 channels, maximum, sum
 
 // NW waves, which take the blocks in turn, or, with OWN, each 16 QT queries of its own and every block (no alignment rows):
-// making fp16 of a block is then the four waves' common work, which meet once a block (8 prompts of 224 tokens over up to
+// widening a block is then the four waves' common work, which meet once a block (8 prompts of 224 tokens over up to
 // 374 positions 13.4 us, 15.5 when each made its own, over 1500 positions 42 and 56).
 template <int FMT, int QT, bool ALIGN, int NW, bool OWN>
 __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
@@ -577,8 +608,6 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     };
 
     float m[QT], l[QT];
-    // the accumulators are in `unit`s, a power of two that no block's values' scale passes (lg_unit: its logarithm)
-    float unit = 0.f, per_unit = 0.f, lg_unit = -INFINITY;
     f32x4 acc[QT][4];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -590,31 +619,17 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     const float scale2 = a.scale * LOG2E;
     float inf = INFINITY;
     asm("" : "+s"(inf));
-    auto weighted = [&](f16x8 v, f16x8 p, f16x8 rest, f32x4 to) { return mfma16(v, p, mfma16(v, rest, to)); };
-    // A block's scales: cs the keys' in the exponent (of two), vs the values', with its logarithm and reciprocal.
+    // A block's scales: cs the keys' in the exponent (of two); of the values' the logarithm lg, which goes into P, and the
+    // reciprocal rc, which takes it out of the sum again; where it is 0 or no number lg is 0, rc 1, and P's factor is by.
     struct Scales {
-        float cs, vs, lg, rc;
+        float cs, lg, rc, by;
     };
-    auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], const Scales& sc, auto open_block) {
-        // the open block's fp16 numbers as they were given: any numbers, vs is 1 and says nothing about their size
+    // (low: what vf lacks of the open block's fp16 numbers)
+    auto products = [&](int b, const f16x8 (&kf)[2][2], const bf16x8 (&vf)[4], const bf16x8 (&low)[4], const Scales& sc, auto open_block) {
+        // the open block's fp16 numbers as they were given: any numbers
         constexpr bool given = decltype(open_block)::value;
         const int p0 = b * MZ_KV_BLK + 8 * g;  // this lane's positions
         const bool whole = b * MZ_KV_BLK >= s.first && (b + 1) * MZ_KV_BLK <= lo_end;  // seen by every query
-        if (given ? unit == 0.f : sc.vs > unit) {
-            const float to = given ? 9.5367431640625e-07f
-                                   : __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, sc.vs) & 0x7f800000u) + 0x00800000u);
-            per_unit = __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(unsigned, to));  // 1 / to
-            lg_unit = (float)((int)(__builtin_bit_cast(unsigned, to) >> 23) - 127);
-            const float f = unit * per_unit;
-#pragma unroll
-            for (int t = 0; t < QT; t++)
-#pragma unroll
-                for (int u = 0; u < 4; u++) acc[t][u] *= f;
-            unit = to;
-        }
-        // P is multiplied by vs / unit, in the exponent, if that is not small
-        const bool direct = !given && sc.lg - lg_unit >= -7.f;
-        const float up = direct ? sc.lg - lg_unit : 0.f, down = direct ? sc.rc * unit : 1.f;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             f32x4 d[2];
@@ -652,43 +667,46 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
                 for (int u = 0; u < 4; u++) acc[t][u] *= f;
             }
             float x[8];
-            f16x8 p;
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], cs, up - m[t]));
-            const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            l[t] += given && !any ? 0.f : sum * down;
-            f16x8 rest;
+            for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], cs, sc.lg - m[t]));
+            l[t] += (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) * sc.rc;
+            asm volatile("" : "+v"(l[t]));  // (the sum is taken here: later it would need copies of x)
+            if (!given && sc.by != 1.f) {
+                const float by = any ? sc.by : 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float hi = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x[e]) & 0xffffe000u);
-                p[e] = (f16)hi;
-                rest[e] = (f16)(x[e] - hi);
+                for (int e = 0; e < 8; e++) x[e] *= by;
             }
-            if (!direct) {  // by itself, and nothing after it (no branch for the other case: the sums stay where they are)
-                const float f = any ? sc.vs * per_unit : 0.f;
+            u32x4 high, rest;
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const f32x4 y = weighted(vf[u], p, rest, f32x4{});
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[t][u][e] = given && !any ? acc[t][u][e] : fmaf(y[e], f, acc[t][u][e]);
-                }
-                p = rest = f16x8{};
+            for (int e = 0; e < 4; e++) {
+                unsigned h = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x[2 * e], (__bf16)x[2 * e + 1]});
+                asm("" : "+v"(h));  // (rounded once)
+                const float r0 = x[2 * e] - __builtin_bit_cast(float, h << 16), r1 = x[2 * e + 1] - __builtin_bit_cast(float, h & 0xffff0000u);
+                high[e] = h;
+                rest[e] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)r0, (__bf16)r1});
             }
-            if (!given)
+            const bf16x8 p = __builtin_bit_cast(bf16x8, high), q = __builtin_bit_cast(bf16x8, rest);
 #pragma unroll
-                for (int u = 0; u < 4; u++) acc[t][u] = weighted(vf[u], p, rest, acc[t][u]);
+            for (int u = 0; u < 4; u++)
+                if constexpr (given) {  // by itself: nothing of it where nothing is seen
+                    const f32x4 y = weighted(vf[u], p, q, weighted(low[u], p, q, f32x4{}));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[t][u][e] = any ? acc[t][u][e] + y[e] : acc[t][u][e];
+                } else
+                    acc[t][u] = weighted(vf[u], p, q, acc[t][u]);
         }
     };
     auto coded = [&](int b, const Raw& w, const Scales& sc) {
-        f16x8 kf[2][2], vf[4];
+        f16x8 kf[2][2];
+        bf16x8 vf[4];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             kf[j][0] = widen<FMT>(w.k[j][0], w.k[j][1]);
             kf[j][1] = widen<FMT>(w.k[j][2], w.k[j][3]);
-            vf[2 * j] = widen<FMT>(w.v[j][0], w.v[j][1]);
-            vf[2 * j + 1] = widen<FMT>(w.v[j][2], w.v[j][3]);
+            vf[2 * j] = widen_bf16<FMT>(w.v[j][0], w.v[j][1]);
+            vf[2 * j + 1] = widen_bf16<FMT>(w.v[j][2], w.v[j][3]);
         }
-        products(b, kf, vf, sc, std::false_type{});
+        products(b, kf, vf, vf, sc, std::false_type{});
     };
     // Blocks b0 + wave, + NW, ..., or every block: DEPTH or AHEAD of them on their way. The open block, where it is this
     // wave's, comes first; its codes are stale.
@@ -712,12 +730,14 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
             const int at = min(b + STEP * lane, tail);
             const float ks = ksc[at], vs = vsc[at], cs = scale2 * ks;
             lanes.cs = cs == 0.f ? 1e-37f : cs;  // (all keys 0; what is not seen is -inf times it)
-            lanes.vs = vs;
-            lanes.lg = __builtin_amdgcn_logf(vs);
-            lanes.rc = __builtin_amdgcn_rcpf(vs);
+            const float lg = __builtin_amdgcn_logf(vs);
+            const bool into = fabsf(lg) < 100.f;
+            lanes.lg = into ? lg : 0.f;
+            lanes.rc = into ? __builtin_amdgcn_rcpf(vs) : 1.f;
+            lanes.by = into ? 1.f : vs;
         };
         auto scales_of = [&](int i) {
-            return Scales{lane_value(lanes.cs, i), lane_value(lanes.vs, i), lane_value(lanes.lg, i), lane_value(lanes.rc, i)};
+            return Scales{lane_value(lanes.cs, i), lane_value(lanes.lg, i), lane_value(lanes.rc, i), lane_value(lanes.by, i)};
         };
         u32x4 raw[AHEAD];
         const auto part = wave < 2 ? rk : rv;
@@ -728,33 +748,50 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
             for (int i = 0; i < AHEAD; i++) raw[i] = take(i);
         scales(head);
         const int open = s.cap ? __builtin_amdgcn_readfirstlane(open_word) - 1 : -1;
-        if (open >= b0 && open < b1 && (open - head) % STEP == 0) {
-            f16x8 kf[2][2], vf[4];
+        // what this wave's queries see ends here
+        const int own_end = !OWN ? hi : q0 < nq && token_of(q0) < s.count ? s.end(a, min(token_of(qn - 1), s.count - 1)) : 0;
+        if (open >= b0 && open < b1 && (open - head) % STEP == 0 && open * MZ_KV_BLK < own_end) {
+            f16x8 kf[2][2];
+            bf16x8 vf[4], low[4];
             const f16* ko = kv.k_open + sh * MZ_KV_TILE;
             const f16* vo = kv.v_open + sh * MZ_KV_TILE;
+            u32x4 there;  // what no query of the tile sees may be no number
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int p = open * MZ_KV_BLK + 8 * g + 2 * e;
+                there[e] = (p < s.first || p >= hi ? 0u : 0xffffu) | (p + 1 < s.first || p + 1 >= hi ? 0u : 0xffff0000u);
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 kf[j >> 1][j & 1] = ld8(ko + (ktok + 4 * (j >> 1)) * 64 + 16 * g + 8 * (j & 1));
-                vf[j] = ld8(vo + ((16 * (j >> 1) + c) * 4 + g) * 16 + 8 * (j & 1));
-            }
+                // eleven bits as eight and the other three, both exact
+                const u32x4 v = __builtin_bit_cast(u32x4, ld8(vo + ((16 * (j >> 1) + c) * 4 + g) * 16 + 8 * (j & 1)));
+                u32x4 v8, v3;
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {  // what no query of the tile sees may be no number
-                    const int p = open * MZ_KV_BLK + 8 * g + e;
-                    if (p < s.first || p >= hi) vf[j][e] = (f16)0.f;
+                for (int e = 0; e < 4; e++) {
+                    const unsigned y = v[e] & there[e], y8 = y & 0xfff8fff8u;
+                    v8[e] = as_bf16(__builtin_bit_cast(f16x2, y8));
+                    v3[e] = as_bf16(__builtin_bit_cast(f16x2, y) - __builtin_bit_cast(f16x2, y8));
                 }
-            products(open, kf, vf, Scales{scale2, 1.f, 0.f, 1.f}, std::true_type{});
+                vf[j] = __builtin_bit_cast(bf16x8, v8);
+                low[j] = __builtin_bit_cast(bf16x8, v3);
+            }
+            products(open, kf, vf, low, Scales{scale2, 0.f, 1.f, 1.f}, std::true_type{});
         }
         if constexpr (OWN) {
-            // Each wave makes fp16 of a quarter of a block (waves 0 and 1 of the keys) and puts it where all find it, a block
+            // Each wave widens a quarter of a block (waves 0 and 1 of the keys) and puts it where all find it, a block
             // ahead; what is behind the last block is that one again.
-            __shared__ f16x8 pieces[2][8][64];
+            __shared__ u32x4 pieces[2][8][64];
             auto put = [&](int b, const u32x4& x) {
-                pieces[b & 1][2 * wave][lane] = widen<FMT>(x[0], x[1]);
-                pieces[b & 1][2 * wave + 1][lane] = widen<FMT>(x[2], x[3]);
+                u32x4* o = &pieces[b & 1][2 * wave][lane];
+                if (wave < 2) {
+                    o[0] = __builtin_bit_cast(u32x4, widen<FMT>(x[0], x[1]));
+                    o[64] = __builtin_bit_cast(u32x4, widen<FMT>(x[2], x[3]));
+                } else {
+                    o[0] = __builtin_bit_cast(u32x4, widen_bf16<FMT>(x[0], x[1]));
+                    o[64] = __builtin_bit_cast(u32x4, widen_bf16<FMT>(x[2], x[3]));
+                }
             };
-            const int own_end = q0 < nq && token_of(q0) < s.count ? s.end(a, min(token_of(qn - 1), s.count - 1)) : 0;
             put(0, raw[0]);
             __syncthreads();
             for (int w0 = 0; w0 <= tail - b0; w0 += WINDOW) {
@@ -768,13 +805,14 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
                         raw[j] = take(i + AHEAD);
                         put(i + 1, raw[(j + 1) % AHEAD]);
                         if (b * MZ_KV_BLK < own_end && b != open) {
-                            f16x8 kf[2][2], vf[4];
+                            f16x8 kf[2][2];
+                            bf16x8 vf[4];
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
-                                kf[k >> 1][k & 1] = pieces[i & 1][k][lane];
-                                vf[k] = pieces[i & 1][4 + k][lane];
+                                kf[k >> 1][k & 1] = __builtin_bit_cast(f16x8, pieces[i & 1][k][lane]);
+                                vf[k] = __builtin_bit_cast(bf16x8, pieces[i & 1][4 + k][lane]);
                             }
-                            products(b, kf, vf, scales_of(i - w0), std::false_type{});
+                            products(b, kf, vf, vf, scales_of(i - w0), std::false_type{});
                         }
                         __syncthreads();
                     }
@@ -799,7 +837,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             const int x = q0 + 16 * t + c, i = token_of(x), h = kh * grp + x - i * grp;
-            const float ll = column_sum(l[t]), f = ll == 0.f ? 0.f : unit / ll;
+            const float ll = column_sum(l[t]), f = ll == 0.f ? 0.f : 1.f / ll;
             if (x >= nq || i >= s.count) continue;
             f16* o = a.out + r * a.out_row + i * a.out_token + h * a.out_head + 8 * g;
 #pragma unroll
@@ -891,8 +929,8 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
         for (int u = 0; u < 2; u++) {
             float* o = &red[wave][c][32 * u + 8 * g];
             const f32x4 x = acc[t][2 * u], y = acc[t][2 * u + 1];
-            *(f32x4*)o = f32x4{x[0] * unit, y[0] * unit, x[1] * unit, y[1] * unit};
-            *(f32x4*)(o + 4) = f32x4{x[2] * unit, y[2] * unit, x[3] * unit, y[3] * unit};
+            *(f32x4*)o = f32x4{x[0], y[0], x[1], y[1]};
+            *(f32x4*)(o + 4) = f32x4{x[2], y[2], x[3], y[3]};
         }
         if (g == 0) {
             ms[wave][c] = m[t];

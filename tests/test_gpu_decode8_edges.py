@@ -9,6 +9,13 @@ from oracle import decode8_ref as R
 pytestmark = pytest.mark.gpu
 
 
+def filled_with(ctx, dev, fmt, k, v):
+    """A cache whose one slot holds the sequence k, v [positions][heads][64]."""
+    b = Both(ctx, 1, k.shape[1], k.shape[0], fmt)
+    b.write(dev, k.astype(np.float16)[None], v.astype(np.float16)[None])
+    return b
+
+
 def expected(b, q, causal, length, **kw):
     """Outputs and lse in 64 bits, and how far an output may be from them. Probabilities are carried with 16 bits or more (2^-16
     relative, of two roundings to 8 bits each) whatever their size, sums are of 32-bit numbers in any order (a score's error
@@ -16,6 +23,36 @@ def expected(b, q, causal, length, **kw):
     w, lse, prob, (av, aq) = R.attention(b.r, q, causal, length, **kw)
     rel = 2 * 80 * U * aq + ((prob > 0).sum(-1) + 16) * U + 2.0 ** -16
     return w, lse, rel[..., None] * av + H * np.abs(w) + 2.0 ** -25
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("rows,heads,tokens", [(1, 1, 1), (32, 10, 1), (1, 2, 20), (40, 8, 20)])
+@pytest.mark.parametrize("n", [20, 1500, 15990])
+def test_a_long_tail_far_below_the_peak(ctx, dev, fmt, rows, heads, tokens, n):
+    """A sequence whose first block has large values and next to no weight, a peak whose own value is 0 in some channels, and
+    all other positions `down` powers of two below it, with values 1/120 of the first block's: what these channels get comes
+    from the tail alone. 20 positions: all of them in the open block, with values of thousands."""
+    rng = np.random.default_rng(n)
+    at = 40 if n > 40 else 3  # the peak
+    k = np.zeros((n, heads, 64))
+    k[..., 1:] = rng.standard_normal((n, heads, 63)) * 0.3
+    v = (0.3 + 0.2 * rng.random((n, heads, 64))) * (1 if n > 32 else 20000)
+    if n > 32:
+        v[:32] = 60.0 * rng.standard_normal((32, heads, 64))
+        k[:32, :, 0] = -1.0
+    k[at, :, 0] = 1.0
+    v[at, :, :32] = 0.0
+    b = filled_with(ctx, dev, fmt, k, v)
+    for down in (6, 12, 18, 40):
+        q = np.zeros((rows, tokens, heads, 64), np.float16)  # (a score is the first channel's product alone)
+        q[..., 0] = down * np.log(2) / 0.125
+        for first in (0, 32) if n > 32 else (0,):  # (without the first block no large values are met)
+            out, lse, _ = run_attention(ctx, dev, b, q, False, [n] * rows, slot=[0] * rows, first=[first] * rows)
+            w, wl, tol = expected(b, q[:1, :1], False, [n], slot=[0], first=[first])
+            err = np.abs(out.astype(np.float64) - w)
+            assert (err <= tol).all(), f"{down}: {(err / tol).max():.3g} x the bound, {(err / np.abs(w))[..., :32].max():.2g} of the output"
+            assert (np.abs(lse - wl) <= 160 * U * down + (n + 8) * U + 4 * U * np.abs(wl)).all()
+    b.free()
 
 
 @pytest.mark.parametrize("fmt", FMT)
