@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
     __shared__ int index[ALIGN ? 64 : 1];
     const int mine = ALIGN && tid < a.heads ? a.head_slot[tid] : -1;
     f16x8 qf[QT][2];
-    int end[QT];  // what a lane's queries see ends here,
+    int end[QT];  // what a lane's queries see ends here (0: they see nothing),
     unsigned span[QT];  // and has these many positions
     float* al[QT];
     auto align_row = [&](int t) -> float* {
@@ -585,6 +585,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
         qf[t][1] = on ? ld8(q + 8) : f16x8{};
         end[t] = on ? s.end(a, i) : 0;
         span[t] = max(end[t] - s.first, 0);
+        if (span[t] == 0) end[t] = 0;  // (also where the first position is in the block that the end is in)
         al[t] = nullptr;
     }
 

@@ -16,6 +16,31 @@ def filled_with(ctx, dev, fmt, k, v):
     return b
 
 
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("rows,heads,tokens", [(1, 2, 1), (1, 2, 9), (1, 2, 24), (17, 16, 1), (40, 20, 24)])
+@pytest.mark.parametrize("what", ["key", "value", "open value", "open key"])
+def test_a_query_that_sees_nothing_of_a_block_with_nan(ctx, dev, fmt, rows, heads, tokens, what):
+    """Padding in front: a row's first position lies inside a block and its first tokens end before it, in the same block, which
+    holds a NaN: out 0 and lse -inf. A later token that sees the block gets what it holds."""
+    rng = np.random.default_rng(tokens)
+    n = 60 if what.startswith("open") else 64
+    k, v = f16(rng, (n, heads, 64)), f16(rng, (n, heads, 64))
+    (k if what.endswith("key") else v)[45, :, 5] = np.nan  # block 1
+    b = Both(ctx, 1, heads, 64, fmt)
+    b.write(dev, k[None], v[None])
+    q = f16(rng, (rows, tokens, heads, 64), 1.5)
+    first, length = 44, 34  # token i sees positions 44 .. 33 + i
+    for causal in (False, True):
+        end = length + (np.arange(tokens) if causal else np.zeros(tokens, int))
+        out, lse, _ = run_attention(ctx, dev, b, q, causal, [length] * rows, slot=[0] * rows, first=[first] * rows)
+        none = end <= first
+        assert none.any()
+        assert (out[:, none] == 0).all() and (lse[:, none] == -np.inf).all()
+        if what in ("key", "value"):
+            assert np.isnan(out[:, ~none, :, 5]).all()  # the block is none as a whole
+    b.free()
+
+
 def expected(b, q, causal, length, **kw):
     """Outputs and lse in 64 bits, and how far an output may be from them. Probabilities are carried with 16 bits or more (2^-16
     relative, of two roundings to 8 bits each) whatever their size, sums are of 32-bit numbers in any order (a score's error
