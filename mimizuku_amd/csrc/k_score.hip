@@ -33,12 +33,13 @@ __device__ __forceinline__ void add(float x, float m, float& s, float& u) {
     u = fmaf(e, fmaxf(d, -200.f), u);
 }
 
-// A value and an id as one number: the larger the better, of equal values the lowest id; 0: none (below -inf with any id).
+// A value and an id as one number: the larger the better, of equal values (-0 is +0) the lowest id; 0: none (below -inf with
+// any id).
 // 62 bits, so that as a number of 64 bits it is positive, finite and in the same order, and v_max_f64 takes the larger one.
 typedef unsigned long long Key;
 constexpr unsigned IDS = 1u << 30;
 __device__ __forceinline__ Key key_of(float v, int id) {
-    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const unsigned u = __builtin_bit_cast(unsigned, v + 0.f);  // (a sum of zeros is +0 unless both are -0)
     return (Key)(u ^ ((unsigned)((int)u >> 31) | 0x80000000u)) << 30 | (IDS - 1 - (unsigned)id);
 }
 __device__ __forceinline__ float value_of(Key k) {

@@ -1,8 +1,8 @@
-"""Attention over 8-bit caches where its definition is easily missed. Against oracle/decode8_ref.py (numpy, 64 bits); helpers and
-the counting of roundings as in test_gpu_decode8.py."""
+"""Attention over 8-bit caches and token scores where their definitions are easily missed. Against oracle/decode8_ref.py (numpy,
+64 bits); helpers and the counting of roundings as in test_gpu_decode8.py."""
 import numpy as np
 import pytest
-from test_gpu_decode8 import FMT, Both, H, U, ctx, dev, f16, run_attention  # noqa: F401
+from test_gpu_decode8 import FMT, Both, H, U, check_scores, ctx, dev, f16, run_attention, run_scores  # noqa: F401
 
 from oracle import decode8_ref as R
 
@@ -95,3 +95,40 @@ def test_outputs_are_as_exact_for_prompts_as_for_single_tokens(ctx, dev, fmt, ro
     err = np.abs(out.astype(np.float64) - w)
     assert (err <= tol).all(), f"{(err / tol).max():.3g} x the bound at {np.argwhere(err > tol)[:3].tolist()}, {(err > tol).mean():.2g} of them"
     b.free()
+
+
+# ---------------------------------------------------------------- token scores
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("rows", [1, 40, 1100])
+@pytest.mark.parametrize("alts", [1, 5, 16])
+def test_zeros_of_either_sign_are_one_value(ctx, dev, dtype, rows, alts):
+    """The best logits are zeros, -0 at some ids and +0 at others, in one lane, in lanes, waves and workgroups of their own, a
+    few of them and (through the network) many: the lowest ids come first."""
+    rng = np.random.default_rng(rows + alts)
+    v = 20011
+    x = -1.0 - np.abs(rng.standard_normal((rows, v)))
+    for r in range(rows):
+        # (neighbours share a lane; 16 on another lane, 1024 on another wave, 8192 on another workgroup of a split row)
+        step = [1, 3, 16, 64, 1024, 5000, 8192, 700][r % 8] if rows > 1 else 5000
+        ids = (np.arange(3, v, step) if r % 3 else np.arange(v - 1, -1, -step))[:[2, 3, 9, 40][r // 8 % 4]]
+        x[r, ids] = np.where(rng.random(len(ids)) < 0.5, 0.0, -0.0)
+        x[r, ids.min()] = -0.0
+        x[r, ids.max()] = 0.0
+    x = x.astype(dtype)
+    tokens = rng.integers(0, v, rows)
+    mask = (rng.random(v) < 0.01).astype(np.uint8)
+    for m in (None, mask):
+        check_scores(x, tokens, run_scores(ctx, dev, x, tokens, m, alts), m, alts)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("vocab", [2, 70, 5000])
+def test_rows_of_zeros_of_either_sign(ctx, dev, dtype, vocab):
+    rng = np.random.default_rng(vocab)
+    x = np.where(rng.random((6, vocab)) < 0.5, 0.0, -0.0).astype(dtype)
+    x[:, 0], x[:, -1] = -0.0, 0.0
+    tokens = np.full(6, vocab - 1)
+    for alts in (1, 2, 16):
+        check_scores(x, tokens, run_scores(ctx, dev, x, tokens, None, alts), None, alts)
