@@ -119,10 +119,11 @@ __device__ __forceinline__ float block_scale(u16x2 m, float& top, float& rc) {
     return top / (FMT == I8 ? 127.f : 448.f);
 }
 
-// row r's slot and positions; false if there is nothing to do for it
+// row r's slot and tokens i0 .. i0 + n - 1, the first of them at position p, without those before the cache; false if there is
+// nothing to do for it
 struct Row {
     long slot;
-    int p, n;
+    int p, n, i0;
 };
 __device__ __forceinline__ bool row_of(const MzKv8& kv, const MzKv8Io& a, int r, Row& o) {
     // (if any array is there all are read, an absent one's place being some other word: the loads go out together)
@@ -135,13 +136,15 @@ __device__ __forceinline__ bool row_of(const MzKv8& kv, const MzKv8Io& a, int r,
     o.slot = a.slot ? slot : r;
     const long p = (long)a.pos_add + (a.pos ? pos : 0);
     o.n = a.count ? min(max(count, 0), a.tokens) : a.tokens;
-    o.p = (int)p;
-    return o.n > 0 && o.slot >= 0 && o.slot < kv.slots && p >= 0 && p < (long)kv.blocks * MZ_KV_BLK;
+    o.i0 = (int)min(max(-p, 0L), (long)o.n);
+    o.n -= o.i0;
+    o.p = (int)max(p, 0L);
+    return o.n > 0 && o.slot >= 0 && o.slot < kv.slots && p < (long)kv.blocks * MZ_KV_BLK;
 }
 
 // the same for a write, whose positions are all in the cache or not written
 __device__ __forceinline__ bool write_row(const MzKv8& kv, const MzKv8Io& a, int r, Row& o) {
-    return row_of(kv, a, r, o) && o.p + (long)o.n <= (long)kv.blocks * MZ_KV_BLK;
+    return row_of(kv, a, r, o) && o.i0 == 0 && o.p + (long)o.n <= (long)kv.blocks * MZ_KV_BLK;
 }
 
 // Lanes over a block, keys: 8 channels of positions lane / 8 + 8 i; values: 4 channels of 8 positions, so that whole
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(256) read_kernel(MzKv8 kv, MzKv8Io a) {
     if (hi <= lo) return;
     const long sh = w.slot * kv.heads + h, blk = sh * kv.blocks + b;
     const bool open = kv.open[sh] == b + 1;
-    f16* o = base + r * a.row_stride + h * a.head_stride + (long)(b * MZ_KV_BLK - w.p) * a.token_stride;
+    f16* o = base + r * a.row_stride + h * a.head_stride + (b * MZ_KV_BLK - w.p + (long)w.i0) * a.token_stride;
     if (side == 0) {
         const int d = (lane & 7) * 8;
         f16x8 x[4];

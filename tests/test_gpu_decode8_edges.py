@@ -1,8 +1,8 @@
-"""Attention over 8-bit caches and token scores where their definitions are easily missed. Against oracle/decode8_ref.py (numpy,
-64 bits); helpers and the counting of roundings as in test_gpu_decode8.py."""
+"""Attention over 8-bit caches, their reading and token scores where their definitions are easily missed. Against
+oracle/decode8_ref.py (numpy, 64 bits); helpers and the counting of roundings as in test_gpu_decode8.py."""
 import numpy as np
 import pytest
-from test_gpu_decode8 import FMT, Both, H, U, check_scores, ctx, dev, f16, run_attention, run_scores  # noqa: F401
+from test_gpu_decode8 import FMT, Both, H, U, check_scores, ctx, dev, f16, i32, run_attention, run_scores  # noqa: F401
 
 from oracle import decode8_ref as R
 
@@ -132,3 +132,36 @@ def test_rows_of_zeros_of_either_sign(ctx, dev, dtype, vocab):
     tokens = np.full(6, vocab - 1)
     for alts in (1, 2, 16):
         check_scores(x, tokens, run_scores(ctx, dev, x, tokens, None, alts), None, alts)
+
+
+# ---------------------------------------------------------------- reading
+
+
+@pytest.mark.parametrize("fmt", FMT)
+def test_read_from_before_the_cache(ctx, dev, fmt):
+    """Tokens at negative positions are left as they were, the others of their row are read."""
+    rng = np.random.default_rng(8)
+    b = Both(ctx, 2, 3, 128, fmt)
+    b.write(dev, f16(rng, (2, 128, 3, 64)), f16(rng, (2, 128, 3, 64)), count=[128, 77])
+    pos, count = [-5, -1, -40, -32, -70, -71, -(2 ** 31), -64, -3, 100, 127, 128], [10, 1, 70, 33, 70, 70, 70, 70, 0, 70, 70, 70]
+    n, t = len(pos), 70
+    slot = [r % 2 for r in range(n)]
+    init = f16(rng, (n, 3, t, 64))
+    for add in (0, 7, -(2 ** 31)):
+        ok, ov = dev(init), dev(init)
+        b.d.read(ok, ov, n, t, strides=(3 * t * 64, 64, t * 64), slot=dev(i32(slot)), pos=dev(i32(pos)), pos_add=add, count=dev(i32(count)))
+        for at, side in ((ok, 0), (ov, 1)):
+            want, src = init.copy(), b.r.stands_for(side)
+            for r in range(n):
+                for i in range(count[r]):
+                    p = pos[r] + add + i
+                    if 0 <= p < 128:
+                        want[r, :, i] = src[slot[r], :, p]
+            np.testing.assert_array_equal(ctx.download(at, init.shape, np.float16).view(np.uint16), want.view(np.uint16))
+    # without an array: pos_add alone, all tokens
+    o = dev(init[:2])
+    b.d.read(o, 0, 2, t, strides=(3 * t * 64, 64, t * 64), pos_add=-33)
+    want = init[:2].copy()
+    want[:, :, 33:] = b.r.stands_for(0)[:, :, :t - 33]
+    np.testing.assert_array_equal(ctx.download(o, want.shape, np.float16).view(np.uint16), want.view(np.uint16))
+    b.free()
