@@ -1017,13 +1017,16 @@ long kept_queries(const Launch& n, long nq) { return std::min(nq, 16L * n.qt); }
 
 // Measured, us, 20 heads unless stated, no alignment rows; a unit is a tile of a (row, cache head).
 // Up to 16 queries: a tile of 16, and no more units than CUs: eight waves each instead of four (1500 positions, 160 units
-// 10.8 / 11.1, five beams of 256 units 10.8 / 11.4, but 260 units 15.7 / 14.4, 640 units 24.6 / 23.6), and with fewer than
+// 10.1 / 11.0, five beams of 256 units 10.9 / 11.3, but 260 units 15.8 / 14.5, 640 units 24.8 / 23.5), and with fewer than
 // half as many, the blocks shared by more workgroups until there is one a CU or a wave has about a block left (1500 positions
-// of one row 10.2 with one workgroup, 8.9 with 2, 7.5 with 4, 7.7 with 6; 80 units 10.2, 9.0 with 3, 10.2 with 4; 16,000
-// positions of 48 units 46 with one, 17.8 with 5, 19.7 with 8).
-// More queries: each wave 16 of its own, where that gives every CU a workgroup (224-token prompts of 8 rows 13.2, the waves
-// taking blocks in turn 14.7; 40 tokens of 16 rows 9.1 / 9.9), else tiles of 32 whose waves take the blocks in turn (224 tokens
-// of one row 7.6 / 10.0, of 3 rows 8.9 / 10.5).
+// of one row 9.5 with one workgroup, 8.8 with 2, 7.6 with 4; 80 units 9.7, 8.8 with 3, 10.0 with 4; 16,000 positions of 48
+// units 47 with one, 20.0 with 5, 22.6 with 8).
+// More queries: each wave 16 of its own, or tiles of 32 whose waves take the blocks in turn. Under a causal mask the first where
+// that gives every CU a workgroup (224-token prompts of 8 rows 13.3 / 14.6, 40 tokens of 16 rows 8.7 / 10.2; but of one row
+// 10.2 / 7.6, of 3 rows 10.4 / 8.9). Without one all workgroups take the same time, and the first needs three and a half a CU,
+// or a last round of them leaves most CUs idle (224 tokens over 1500 positions: 7 rows, 2.2 workgroups a CU, 45.8 / 34.4, 8 rows
+// 46.0 / 39.6, 10 rows, 3.1, 56 / 47, 16 rows, 5.0, 68 / 74, 32 rows 136 / 150; over 374 positions 10 rows 21.2 / 20.9, 24 rows of
+// 128 tokens, 3.8, 22.1 / 26.4; the other way 32 rows of 40 tokens, 2.5, 17.2 / 19.4).
 Launch attn_shape(const MzKv8& kv, const MzKv8Attn& a) {
     const long nq = (long)a.tokens * (a.heads / kv.heads), cus = mz_cu_count(), pairs = (long)a.rows * kv.heads;
     auto inverse = [](int d) { return (unsigned)std::min((1ULL << 32) / d, 0xffffffffULL); };
@@ -1033,7 +1036,7 @@ Launch attn_shape(const MzKv8& kv, const MzKv8Attn& a) {
     n.by_group = inverse(n.group);
     n.waves = 4;
     n.splits = 1;
-    n.own = !a.align && nq > 16 && pairs * ((nq + 63) / 64) >= cus;
+    n.own = !a.align && nq > 16 && 2 * pairs * ((nq + 63) / 64) >= (a.causal ? 2 : 7) * cus;
     if (n.own) {
         n.tiles = (int)((nq + 63) / 64);
         return n;

@@ -51,7 +51,7 @@ def expected(b, q, causal, length, **kw):
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("rows,heads,tokens", [(1, 1, 1), (32, 10, 1), (1, 2, 20), (40, 8, 20)])
+@pytest.mark.parametrize("rows,heads,tokens", [(1, 1, 1), (32, 10, 1), (1, 2, 20), (40, 8, 20), (90, 10, 20)])
 @pytest.mark.parametrize("n", [20, 1500, 15990])
 def test_a_long_tail_far_below_the_peak(ctx, dev, fmt, rows, heads, tokens, n):
     """A sequence whose first block has large values and next to no weight, a peak whose own value is 0 in some channels, and
