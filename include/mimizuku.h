@@ -175,7 +175,10 @@ int mz_kv8_read(mz_ctx* c, const mz_kv8* kv, const mz_kv8_io* a);
 /* out = softmax(scale q . k) v over the positions that each query sees; row r's query token i, head h at
  * q + r * q_row + i * q_token + h * q_head (f16, strides in elements, multiples of 8, addresses multiples of 16 bytes;
  * the same for out, whose 64-channel rows must not overlap). Query head h reads the cache's head h / (heads /
- * kv->heads). Rows may share slots (beams over one encoder output). */
+ * kv->heads). Rows may share slots (beams over one encoder output). Probabilities are carried with 16 bits or more whatever
+ * their size and the number of queries, sums with 32, the output is rounded once. The same call gives the same bits;
+ * the last bits of a row may differ with the other rows of the call, its tokens, the cache's size and the device's CUs, by
+ * which the positions are shared out and so the order of their sums. */
 typedef struct {
     uint64_t q, out;
     int64_t q_row, q_token, q_head, out_row, out_token, out_head;
@@ -189,7 +192,7 @@ typedef struct {
      * cache, gets out 0 and lse -inf. Blocks of which a query sees nothing do not touch it, NaN or not; neither do
      * positions of the open block that no token of the call sees. (A NaN or infinity at a position of the open block
      * that later tokens of the call see can reach the earlier tokens that see the block: it is none as a whole, as it
-     * will be when it is coded.) */
+     * will be when it is coded. An infinite value of the open block may come out as NaN.) */
     uint64_t len; /* i32 */
     int len_stride, len_add;
     uint64_t first; /* i32 [rows] */
@@ -211,9 +214,11 @@ int mz_kv8_attention_bytes(mz_ctx* c, const mz_kv8* kv, const mz_kv8_attention_a
 
 /* What a model's answers are worth: for each of `rows` rows of `vocab` logits the log probability of a given token, the
  * distribution's entropy (both natural logarithms) and the `alts` (0 .. 16) most probable tokens with theirs, ties to
- * the lowest id. Ids with a nonzero mask byte have probability 0, as have logits of -inf; tokens of probability 0 are
- * no alternatives: where fewer are left, ids are -1 and log probabilities -inf. A row with a NaN or a logit of +inf
- * (unmasked) gets NaN throughout and ids -1; one with nothing left -inf, entropy 0 and ids -1. */
+ * the lowest id (-0 and +0 tie). Ids with a nonzero mask byte have probability 0, as have logits of -inf; tokens of
+ * probability 0 are no alternatives: where fewer are left, ids are -1 and log probabilities -inf. A row with a NaN or a
+ * logit of +inf (unmasked) gets NaN throughout and ids -1; one with nothing left -inf, entropy 0 and ids -1. The same call
+ * gives the same bits; the last bits of log probabilities and entropies may differ with the number of rows and the
+ * device's CUs, by which a row is split. */
 typedef struct {
     int dtype; /* MZ_DT_F16 or MZ_DT_F32 */
     int rows, vocab, alts;

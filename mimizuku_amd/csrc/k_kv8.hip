@@ -421,9 +421,11 @@ long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std:
 // blocks in turn, each with a state of its own, and join them at the end.
 //
 // Bound by memory for single tokens: 4,104 bytes a block, of which 32 rows x 20 heads x 1500 positions (126 MB) take 23.6 us,
-// 6.7 TB/s behind the ~5 us of the launch and of the round trips to the first key and from the last (25.2 with six alignment
-// heads). One row: those round trips, 7.5 us (8.7). Prompts: vector instructions, about 95 a block of 16 queries (8 prompts of 224
-// tokens over up to 374 positions 13.0 us).
+// 6.7 TB/s behind the ~5 us of the launch and of the round trips to the first key and from the last (25.5 with six alignment
+// heads). One row: those round trips, 7.6 us (8.7). Prompts: 8 of 224 tokens over up to 374 positions 13.2 us, the chain of the
+// longest, 12 blocks one after the other, each with a barrier, a round trip through LDS and two products that wait for each
+// other (waves wait half of their time, the vector units are busy for 39% of a CU's); over 1500 positions 39.4, vector
+// instructions: about 150 a block of 16 queries, products included.
 //
 // Per block of 32 positions, with 16x16x32 products: S^T = K Q^T, the rows of tile j being positions 8 (i / 4) + 4 j + i % 4,
 // so that lane (query c, group g) of the two results holds the eight positions 8 g .. 8 g + 7 of its query. These
@@ -532,8 +534,8 @@ __device__ __forceinline__ int divided(int x, int d, unsigned r) {
 constexpr int STATE = 66;  // floats of a query's partial state: 64 channels, maximum, sum
 
 // NW waves, which take the blocks in turn, or, with OWN, each 16 QT queries of its own and every block (no alignment rows):
-// widening a block is then the four waves' common work, which meet once a block (8 prompts of 224 tokens over up to
-// 374 positions 13.4 us, 15.5 when each made its own, over 1500 positions 42 and 56).
+// widening a block is then the four waves' common work, which meet once a block (an earlier build, 8 prompts of 224
+// tokens over up to 374 positions: 13.4 us, 15.5 when each made its own, over 1500 positions 42 and 56).
 template <int FMT, int QT, bool ALIGN, int NW, bool OWN>
 __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
     static_assert(!(OWN && ALIGN));
