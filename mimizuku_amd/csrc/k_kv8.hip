@@ -534,8 +534,8 @@ __device__ __forceinline__ int divided(int x, int d, unsigned r) {
 constexpr int STATE = 66;  // floats of a query's partial state: 64 channels, maximum, sum
 
 // NW waves, which take the blocks in turn, or, with OWN, each 16 QT queries of its own and every block (no alignment rows):
-// widening a block is then the four waves' common work, which meet once a block (an earlier build, 8 prompts of 224
-// tokens over up to 374 positions: 13.4 us, 15.5 when each made its own, over 1500 positions 42 and 56).
+// widening a block is then the four waves' common work, which meet once a block (measured with P as one fp16
+// number, 8 prompts of 224 tokens over up to 374 positions: 13.4 us, 15.5 when each made its own, over 1500 positions 42 and 56).
 template <int FMT, int QT, bool ALIGN, int NW, bool OWN>
 __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kernel(MzKv8 kv, MzKv8Attn a, Launch n) {
     static_assert(!(OWN && ALIGN));
