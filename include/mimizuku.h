@@ -243,6 +243,112 @@ typedef struct {
 int mz_token_scores(mz_ctx* c, const mz_score_args* a);
 int mz_token_scores_bytes(mz_ctx* c, const mz_score_args* a, size_t* bytes);
 
+/* ------------------------------------------------------------------ a decoder step of a caller's own: products with
+ * 4-bit weights, attention over an encoder's output, the next token
+ *
+ * No counterpart in the reference, whose weights are fp16, whose cross-attention takes 1500 positions and whose choice is
+ * greedy. As the kernels above: device addresses, work enqueued on the context's stream and capturable (no allocation, no
+ * host synchronisation); what the device arrays hold is read on the device. The same call gives the same bits. */
+
+/* Weights [n][k] in 4 bits: each group of 32, 64 or 128 columns of a row has one scale, code c (-8 .. 7) stands for
+ * c * scale. From weights w with hi and lo a group's largest and smallest, e = hi if hi > -lo else lo: scale = f16(e / -8),
+ * c = w / scale to the nearest, halves to even, 7 at most and -8 at least (scale 0: codes 0; a group with a NaN or an
+ * infinity in it: scale NaN). */
+typedef struct {
+    int n, k, group;  /* k a multiple of 128 */
+    uint64_t codes;   /* [ceil(n / 16)][k / 128][64][16 bytes]: row 16 t + i, columns 128 c + 32 s + 8 j .. + 7 are the
+                       * 32-bit word s of entry 16 j + i, column 8 j + e in its bits 4 (e / 2) + 16 (e % 2) .. + 3 as c + 8 */
+    uint64_t scales;  /* f16 [ceil(n / 16)][k / 128][4][128 / group][4]: row 16 t + 4 j + r, group g of the 128 columns
+                       * at [t][c][j][g][r] */
+} mz_w4;
+/* Lays n x k weights out in one buffer at `base` (256-byte aligned; 0 to ask for the size only): fills in *w and the
+ * buffer's size (either may be null). */
+int mz_w4_place(int n, int k, int group, uint64_t base, mz_w4* w, size_t* bytes);
+/* f16 weights [n][ld] (ld >= k, a multiple of 8; 16-byte aligned) into codes and scales; rows that pad the last tile
+ * become zeros. */
+int mz_w4_pack(mz_ctx* c, const mz_w4* w, uint64_t src, int64_t ld);
+/* What they stand for: f16(f32(c * scale)) into [n][ld], aligned likewise. */
+int mz_w4_unpack(mz_ctx* c, const mz_w4* w, uint64_t dst, int64_t ld);
+
+#define MZ_EPI_F32 5 /* mz_w4_linear: out f32 [m][ldo] = acc + bias */
+/* out [m][n] = epilogue(sum over groups of scale * (x . codes) + bias): products of codes and x in 32 bits, exact before
+ * they are summed, the scale applied to a group's sum, one rounding at the end (GELU's error included: 0.505 of an fp16
+ * step). Any m: 1 to 64 rows read the weights once. The last bits may differ with m and the device's CUs, by which the
+ * sums over k are shared out. x, bias and out are read and written by their elements' alignment, x by 16 bytes. */
+typedef struct {
+    int epilogue; /* MZ_EPI_F16, MZ_EPI_GELU_F16, MZ_EPI_RESID_F32 or MZ_EPI_F32 */
+    int m;
+    uint64_t x;   /* f16 [m][ldx], ldx >= k, a multiple of 8 */
+    int64_t ldx;
+    uint64_t bias; /* f16 [n], 0: none */
+    uint64_t out;  /* [m][ldo], ldo >= n; does not overlap x */
+    int64_t ldo;
+} mz_w4_linear_args;
+int mz_w4_linear(mz_ctx* c, const mz_w4* w, const mz_w4_linear_args* a);
+
+/* out = softmax(scale q . k) v of queries over fp16 keys and values of `slots` sequences (an encoder's outputs) of any
+ * length: position t, head h of slot s at k + s * k_slot + t * k_pos + h * k_head, its 64 channels together (v likewise;
+ * strides in elements, multiples of 8, addresses multiples of 16 bytes). MZ_BUF_XKV's tiles are such keys and values
+ * (k_pos 64, k_head 1536 * 64), and so are the rows of a product (k_pos its width, k_head 64). Queries, outputs, slots,
+ * counts, lse, alignment rows and the workspace are those of mz_kv8_attention_args: rows may share slots, query head h
+ * reads head h / (heads / kv_heads). There is no causal mask: row r's tokens all see the positions first[r] (first 0: 0)
+ * to below min(len[r], positions) (len 0: positions). A row that sees nothing, or whose slot lies outside, gets out 0 and
+ * lse -inf; keys and values that it does not see do not touch it, NaN or not. An infinite value that is seen comes out as
+ * NaN. Probabilities are carried with 21 bits or more of a row's largest, sums with 32, the output is rounded once. The
+ * last bits of a row may differ with the other rows of the call, its tokens, `positions` and the device's CUs. */
+typedef struct {
+    uint64_t q, out;
+    int64_t q_row, q_token, q_head, out_row, out_token, out_head;
+    uint64_t k, v;
+    int64_t k_slot, k_pos, k_head, v_slot, v_pos, v_head;
+    int rows, tokens, heads, kv_heads, slots, positions;
+    float scale;                      /* > 0, at most 2^20 */
+    uint64_t slot, count, first, len; /* i32 [rows], any may be 0 */
+    uint64_t lse;
+    uint64_t head_slot, align;
+    int align_heads, align_cols;
+    uint64_t work; /* mz_cross_attention_bytes bytes */
+    size_t work_bytes;
+} mz_cross_attention_args;
+int mz_cross_attention(mz_ctx* c, const mz_cross_attention_args* a);
+int mz_cross_attention_bytes(mz_ctx* c, const mz_cross_attention_args* a, size_t* bytes);
+
+/* The next token of each of `rows` rows of logits, drawn by a given random number. With m the row's largest unmasked logit
+ * and T its temperature, the weight of a token is exp((x - m) / T). In the order of falling logits, of equal ones (-0 and
+ * +0 are equal) the lower id first, those tokens are kept that are
+ *   among the first top_k (0 or less: no limit),
+ *   not behind the first place up to which the weights sum to top_p times the sum of the first top_k's (1 or more: no limit),
+ *   of weight min_p or more (0 or less: no limit; of the largest weight, 1);
+ * the first always is. The token drawn is the lowest kept id up to which the kept weights sum to more than u times their
+ * sum, at temperature 0 the first. Weights are computed in 64 bits and summed exactly as multiples of 2^-s, s = min(51, 62 -
+ * ceil(log2 vocab)): the order of sums does not matter, and tokens of weight below 2^-(s + 1) are not drawn.
+ * Ids with a nonzero mask byte and logits of -inf are no tokens. A row without any, one with a NaN or a logit of +inf
+ * (unmasked), and one whose temperature is negative or no finite number or whose top_p or min_p is NaN has the token -1,
+ * kept 0 and logp NaN (-inf where there is just nothing left). u below 0 or NaN counts as 0, of 1 or more as the largest
+ * below 1. */
+typedef struct {
+    int dtype; /* MZ_DT_F16 or MZ_DT_F32 */
+    int rows, vocab;
+    uint64_t logits; /* row r at element r * ld (ld >= vocab); any alignment of the element */
+    int64_t ld;
+    uint64_t mask; /* u8 [vocab], 0: none */
+    float temperature, top_p, min_p;                 /* for all rows, or */
+    int top_k;
+    uint64_t temperatures, top_ps, min_ps, top_ks;   /* f32 / i32 [rows]: a row's own, 0: the above */
+    /* row r's random number is u[r * stride + n] (f32), and its token, the logarithm of the token's share of the kept
+     * weights and the number of tokens kept go to that index of tokens (i32), logp (f32) and kept (i32) (logp and kept may
+     * be 0: not wanted), with n = *at + at_add (at 0: n = 0) as in mz_score_args. A row whose n is outside 0 .. stride - 1
+     * writes nothing. */
+    uint64_t u, tokens, logp, kept;
+    int64_t stride;
+    uint64_t at; /* i32 */
+    int at_add;
+    uint64_t work; /* mz_sample_bytes bytes, as mz_kv8_attention_args.work */
+    size_t work_bytes;
+} mz_sample_args;
+int mz_sample(mz_ctx* c, const mz_sample_args* a);
+int mz_sample_bytes(mz_ctx* c, const mz_sample_args* a, size_t* bytes);
+
 /* ------------------------------------------------------------------ engine (src/model.rs, src/transcribe.rs) */
 
 /* Model geometry (Dims, src/model.rs:14-25). */

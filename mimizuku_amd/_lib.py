@@ -68,7 +68,34 @@ class ScoreArgs(C.Structure):
                  ("alt_ids", u64), ("alt_logp", u64), ("work", u64), ("work_bytes", C.c_size_t)])
 
 
-EPI_F16, EPI_GELU_F16, EPI_RESID_F32, EPI_GELU_POS, EPI_HEADS = range(5)
+class W4(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n", "k", "group")] + [("codes", u64), ("scales", u64)]
+
+
+class W4LinearArgs(C.Structure):
+    _fields_ = [("epilogue", C.c_int), ("m", C.c_int), ("x", u64), ("ldx", C.c_int64), ("bias", u64), ("out", u64),
+                ("ldo", C.c_int64)]
+
+
+class CrossArgs(C.Structure):
+    _fields_ = ([("q", u64), ("out", u64)] +
+                [(n, C.c_int64) for n in ("q_row", "q_token", "q_head", "out_row", "out_token", "out_head")] +
+                [("k", u64), ("v", u64)] +
+                [(n, C.c_int64) for n in ("k_slot", "k_pos", "k_head", "v_slot", "v_pos", "v_head")] +
+                [(n, C.c_int) for n in ("rows", "tokens", "heads", "kv_heads", "slots", "positions")] +
+                [("scale", C.c_float)] + [(n, u64) for n in ("slot", "count", "first", "len", "lse", "head_slot", "align")] +
+                [("align_heads", C.c_int), ("align_cols", C.c_int), ("work", u64), ("work_bytes", C.c_size_t)])
+
+
+class SampleArgs(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("dtype", "rows", "vocab")] +
+                [("logits", u64), ("ld", C.c_int64), ("mask", u64)] +
+                [(n, C.c_float) for n in ("temperature", "top_p", "min_p")] + [("top_k", C.c_int)] +
+                [(n, u64) for n in ("temperatures", "top_ps", "min_ps", "top_ks", "u", "tokens", "logp", "kept")] +
+                [("stride", C.c_int64), ("at", u64), ("at_add", C.c_int), ("work", u64), ("work_bytes", C.c_size_t)])
+
+
+EPI_F16, EPI_GELU_F16, EPI_RESID_F32, EPI_GELU_POS, EPI_HEADS, EPI_F32 = range(6)
 (BUF_TOK, BUF_DONE, BUF_CTR, BUF_ALIGN, BUF_ENC_OUT, BUF_LOGITS, BUF_TRACE, BUF_XKV, BUF_DEC_X, BUF_ENC_X,
  BUF_DEC_TRACE, BUF_SELF_K, BUF_SELF_V, BUF_ALIGN_H) = range(14)
 DT_F16, DT_F32 = 0, 1
@@ -112,6 +139,14 @@ SIGNATURES = {
     "mz_kv8_attention_bytes": (i32, [P, C.POINTER(Kv8), C.POINTER(Kv8Attention), C.POINTER(sz)]),
     "mz_token_scores": (i32, [P, C.POINTER(ScoreArgs)]),
     "mz_token_scores_bytes": (i32, [P, C.POINTER(ScoreArgs), C.POINTER(sz)]),
+    "mz_w4_place": (i32, [i32, i32, i32, u64, C.POINTER(W4), C.POINTER(sz)]),
+    "mz_w4_pack": (i32, [P, C.POINTER(W4), u64, C.c_int64]),
+    "mz_w4_unpack": (i32, [P, C.POINTER(W4), u64, C.c_int64]),
+    "mz_w4_linear": (i32, [P, C.POINTER(W4), C.POINTER(W4LinearArgs)]),
+    "mz_cross_attention": (i32, [P, C.POINTER(CrossArgs)]),
+    "mz_cross_attention_bytes": (i32, [P, C.POINTER(CrossArgs), C.POINTER(sz)]),
+    "mz_sample": (i32, [P, C.POINTER(SampleArgs)]),
+    "mz_sample_bytes": (i32, [P, C.POINTER(SampleArgs), C.POINTER(sz)]),
     "mz_scratch_bytes": (sz, [C.POINTER(Dims), i32, i32, i32]),
     "mz_engine_new": (i32, [P, C.POINTER(Dims), C.POINTER(GenCfgC), i32, i32, C.POINTER(P)]),
     "mz_engine_put": (i32, [P, C.c_char_p, i32, P, C.POINTER(C.c_int64), i32]),

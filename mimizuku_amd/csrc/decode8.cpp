@@ -6,36 +6,12 @@
 #include <cmath>
 
 #include "../../include/mimizuku.h"
+#include "mz_args.h"
 #include "mz_internal.h"
 #include "mz_kernels.h"
 
-#define DP(T, x) ((T*)(uintptr_t)(x))
-
 namespace {
 
-// The context's device is current while a call runs, whatever was before and will be after.
-class OnDevice {
-public:
-    explicit OnDevice(int device) {
-        if ((status_ = mz_hip(hipGetDevice(&before_), "hipGetDevice"))) return;
-        if (before_ == device) before_ = -1;
-        else status_ = mz_hip(hipSetDevice(device), "hipSetDevice");
-    }
-    ~OnDevice() {
-        if (before_ >= 0) hipSetDevice(before_);
-    }
-    OnDevice(const OnDevice&) = delete;
-    OnDevice& operator=(const OnDevice&) = delete;
-    int status() const { return status_; }
-
-private:
-    int before_ = -1, status_ = MZ_OK;
-};
-
-bool aligned(uint64_t p, uint64_t n) { return p % n == 0; }
-
-// Elements of each tensor stay below this, so that no 64-bit byte offset of a kernel can wrap.
-constexpr int64_t MOST = (int64_t)1 << 46;
 constexpr int MAX_BLOCKS = (1 << 20) - 1;  // of a slot: its codes lie within 2^31 bytes, as far as a buffer descriptor reaches
 constexpr int MAX_SCORE_ROWS = (1 << 24) - 1;  // a workgroup of 256 threads each: a launch has fewer than 2^32 along x
 
@@ -51,26 +27,6 @@ int check_cache(const char* who, const mz_kv8* kv, MzKv8* out) {
     *out = {kv->format, kv->slots, kv->heads, kv->blocks, DP(unsigned char, kv->k), DP(unsigned char, kv->v),
             DP(float, kv->k_scale), DP(float, kv->v_scale), DP(f16, kv->k_open), DP(f16, kv->v_open), DP(int, kv->open)};
     return MZ_OK;
-}
-
-// Offsets of rows x tokens x heads 64-channel rows: in range, and multiples of 8 elements.
-bool strides_ok(const int64_t (&stride)[3], const int64_t (&n)[3]) {
-    for (int i = 0; i < 3; i++)
-        if (stride[i] < 0 || stride[i] % 8 || stride[i] > MOST || (n[i] > 1 && stride[i] > MOST / (n[i] - 1))) return false;
-    return true;
-}
-
-// Whether those rows lie apart from each other, each dimension's steps outside what the smaller ones span.
-bool apart(const int64_t (&stride)[3], const int64_t (&n)[3]) {
-    int order[3] = {0, 1, 2};
-    std::sort(order, order + 3, [&](int a, int b) { return stride[a] < stride[b]; });
-    int64_t span = 64;
-    for (int i : order) {
-        if (n[i] <= 1) continue;
-        if (stride[i] < span) return false;
-        span += stride[i] * (n[i] - 1);
-    }
-    return true;
 }
 
 int check_io(const char* who, const mz_kv8* kv, const mz_kv8_io* a, const MzKv8* cache, MzKv8Io* out) {
@@ -136,12 +92,6 @@ int check_scores(const char* who, const mz_score_args* a, MzScores* out) {
     *out = {a->dtype == MZ_DT_F16, a->rows, a->vocab, a->alts, DP(const void, a->logits), (long)a->ld,
             DP(const unsigned char, a->mask), DP(const int, a->tokens), (long)a->token_stride, DP(const int, a->at), a->at_add,
             DP(float, a->logp), DP(float, a->entropy), (long)a->out_stride, DP(int, a->alt_ids), DP(float, a->alt_logp), nullptr};
-    return MZ_OK;
-}
-
-int check_work(const char* who, uint64_t work, size_t have, size_t need) {
-    if (need && (!work || !aligned(work, 256) || have < need))
-        return mz_fail(MZ_ERR_ARG, "%s: needs a workspace of %zu bytes, aligned to 256 (given %zu)", who, need, work ? have : (size_t)0);
     return MZ_OK;
 }
 

@@ -318,3 +318,68 @@ struct MzScores {
 };
 size_t mz_scores_work(const MzScores& p);
 hipError_t mz_scores_launch(hipStream_t s, const MzScores& p);
+
+// ---------------------------------------------------------------- products with 4-bit weights (mz_w4 in mimizuku.h)
+struct MzW4 {
+    int n, k, group;
+    unsigned char* codes;
+    f16* scales;
+};
+struct MzW4Linear {
+    int epilogue, m;
+    const f16* x;
+    long ldx;
+    const f16* bias;
+    void* out;
+    long ldo;
+};
+// what a launch takes: rows of weights, rows of x
+#define MZ_W4_MOST_N (1 << 26)
+#define MZ_W4_MOST_M (1 << 20)
+hipError_t mz_w4_pack_launch(hipStream_t s, const MzW4& w, const f16* src, long ld);
+hipError_t mz_w4_unpack_launch(hipStream_t s, const MzW4& w, f16* dst, long ld);
+hipError_t mz_w4_linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a);
+
+// ---------------------------------------------------------------- attention over an encoder's output (mz_cross_attention_args)
+struct MzCross {
+    const f16* q;
+    f16* out;
+    long q_row, q_token, q_head, out_row, out_token, out_head;
+    const f16 *k, *v;
+    long k_slot, k_pos, k_head, v_slot, v_pos, v_head;
+    int rows, tokens, heads, kv_heads, slots, positions;
+    float scale;
+    const int *slot, *count, *first, *len;
+    float* lse;
+    const int* head_slot;  // null without alignment rows
+    float* align;
+    int align_heads, align_cols;
+    float* work;
+};
+// whether one launch takes it: rows x kv_heads below 2^23 - 8, tokens x query heads of each at most 16 x 65535
+bool mz_cross_fits(const MzCross& a);
+size_t mz_cross_work(const MzCross& a);
+hipError_t mz_cross_launch(hipStream_t s, const MzCross& a);
+
+// ---------------------------------------------------------------- the next token (mz_sample_args)
+struct MzSample {
+    int half;  // logits fp16
+    int rows, vocab;
+    const void* logits;
+    long ld;
+    const unsigned char* mask;
+    float temperature, top_p, min_p;
+    int top_k;
+    const float *temperatures, *top_ps, *min_ps;
+    const int* top_ks;
+    const float* u;
+    int* tokens;
+    float* logp;
+    int* kept;
+    long stride;
+    const int* at;
+    int at_add;
+    float* work;
+};
+size_t mz_sample_work(const MzSample& p);
+hipError_t mz_sample_launch(hipStream_t s, const MzSample& p);
