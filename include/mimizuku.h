@@ -258,8 +258,7 @@ typedef struct {
     int n, k, group;  /* k a multiple of 128 */
     uint64_t codes;   /* [ceil(n / 16)][k / 128][64][16 bytes]: row 16 t + i, columns 128 c + 32 s + 8 j .. + 7 are the
                        * 32-bit word s of entry 16 j + i, column 8 j + e in its bits 4 (e / 2) + 16 (e % 2) .. + 3 as c + 8 */
-    uint64_t scales;  /* f16 [ceil(n / 16)][k / 128][4][128 / group][4]: row 16 t + 4 j + r, group g of the 128 columns
-                       * at [t][c][j][g][r] */
+    uint64_t scales;  /* f16 [ceil(n / 16)][k / 128][16 rows][128 / group] */
 } mz_w4;
 /* Lays n x k weights out in one buffer at `base` (256-byte aligned; 0 to ask for the size only): fills in *w and the
  * buffer's size (either may be null). */

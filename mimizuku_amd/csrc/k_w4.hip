@@ -1,4 +1,6 @@
 // Products with 4-bit weights (mz_w4 in mimizuku.h).
+#include <algorithm>
+
 #include "mz_common.h"
 #include "mz_kernels.h"
 
@@ -67,12 +69,11 @@ __global__ void __launch_bounds__(256) pack_kernel(MzW4 w, const f16* src, long 
         q[s] = word;
     }
     *(u32x4*)(w.codes + (entry * 64 + lane) * 16) = q;
-    // row i is row 4 (i / 4) + i % 4: place [i / 4][group][i % 4]
     const int groups = 128 / w.group;
     if (j == 0)
 #pragma unroll
         for (int s = 0; s < 4; s++)
-            if (s % words == 0) w.scales[(entry * 4 + (i >> 2)) * groups * 4 + s / words * 4 + (i & 3)] = scale[s];
+            if (s % words == 0) w.scales[(entry * 16 + i) * groups + s / words] = scale[s];
 }
 
 __global__ void __launch_bounds__(256) unpack_kernel(MzW4 w, f16* dst, long ld) {
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(256) unpack_kernel(MzW4 w, f16* dst, long ld) 
     const int words = w.group / 32, groups = 128 / w.group;
 #pragma unroll
     for (int s = 0; s < 4; s++) {
-        const float d = (float)w.scales[(entry * 4 + (i >> 2)) * groups * 4 + s / words * 4 + (i & 3)];
+        const float d = (float)w.scales[(entry * 16 + i) * groups + s / words];
         f16x8 y;
 #pragma unroll
         for (int e = 0; e < 8; e++) y[e] = (f16)((float)((int)(q[s] >> bit_of(e) & 15) - 8) * d);
@@ -94,34 +95,257 @@ __global__ void __launch_bounds__(256) unpack_kernel(MzW4 w, f16* dst, long ld) 
     }
 }
 
-// A thread: one output of a tile of 16 rows of weights x 16 rows of x.
-__global__ void __launch_bounds__(256) linear_kernel(MzW4 w, MzW4Linear a) {
-    const int i = threadIdx.x & 15, mi = blockIdx.y * 16 + (threadIdx.x >> 4), chunks = w.k / 128, groups = 128 / w.group;
-    const long t = blockIdx.x, n = t * 16 + i;
-    if (mi >= a.m || n >= w.n) return;
-    const f16* x = a.x + mi * a.ldx;
-    float sum = 0.f;
-    for (int c = 0; c < chunks; c++) {
+// ---------------------------------------------------------------- products
+
+// the eight codes of a word, as they are: 1024 + (c + 8) and 1024 + 16 (c + 8) are fp16 numbers whose low bits are c + 8
+__device__ __forceinline__ f16x8 numbers(unsigned q) {
+    const unsigned one = 0x000F000Fu, sixteen = 0x00F000F0u, magic = 0x64006400u;
+    const unsigned q8 = q >> 8;
+    const f16x2 off1 = {(f16)-1032.f, (f16)-1032.f}, off16 = {(f16)-72.f, (f16)-72.f}, by = {(f16)0.0625f, (f16)0.0625f};
+    const f16x2 a = __builtin_bit_cast(f16x2, (q & one) | magic) + off1;
+    const f16x2 b = __builtin_bit_cast(f16x2, (q & sixteen) | magic) * by + off16;
+    const f16x2 c = __builtin_bit_cast(f16x2, (q8 & one) | magic) + off1;
+    const f16x2 d = __builtin_bit_cast(f16x2, (q8 & sixteen) | magic) * by + off16;
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <int G>  // groups of 128 columns
+struct Scales {
+    f16 v[G];
+};
+template <int G>
+__device__ __forceinline__ Scales<G> scales_at(const f16* p) {
+    if constexpr (G == 4) return __builtin_bit_cast(Scales<4>, *(const f16x4*)p);
+    else if constexpr (G == 2) return __builtin_bit_cast(Scales<2>, *(const f16x2*)p);
+    else return Scales<1>{*p};
+}
+
+__device__ __forceinline__ void finish(const MzW4Linear& a, int m, int n, float y) {
+    if (a.bias) y += (float)a.bias[n];
+    const long o = m * a.ldo + n;
+    switch (a.epilogue) {
+        case 0: ((f16*)a.out)[o] = (f16)y; break;
+        case 1: ((f16*)a.out)[o] = (f16)gelu_erf_h(y); break;
+        case 2: ((float*)a.out)[o] += y; break;
+        default: ((float*)a.out)[o] = y;
+    }
+}
+
+// One entry, 16 rows of weights x 128 columns, times 16 MT rows of x: operand lane 16 j + i holds row i, columns 32 s + 8 j .. of
+// either; the result's lane 16 j + i holds column i (a row of weights) and rows 4 j .. 4 j + 3 (of x).
+template <int MT, int G, typename X>
+__device__ __forceinline__ void entry_product(u32x4 q, Scales<G> scale, X x, f32x4 (&sum)[MT]) {
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        f32x4 part[MT];
+#pragma unroll
+        for (int z = 0; z < 4 / G; z++) {
+            const int s = g * (4 / G) + z;
+            const f16x8 w = numbers(q[s]);
+#pragma unroll
+            for (int t = 0; t < MT; t++) part[t] = mfma16(x(t, s), w, z ? part[t] : f32x4{});
+        }
+        const float d = (float)scale.v[g];
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[t][e] = fmaf(part[t][e], d, sum[t][e]);
+    }
+}
+
+// Few rows of weights: a workgroup takes 16 of them, its waves the entries in turn, x from memory; their sums meet in LDS.
+template <int MT, int G>
+__global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW4Linear a) {
+    constexpr int LD = 68;  // (of 64 results: four rows of x 4 banks apart, so that reading 16 columns of 4 rows meets no conflict)
+    extern __shared__ float red[];  // [wave][4 MT][LD]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / 64;
+    const int i = lane & 15, j = lane >> 4, chunks = w.k / 128, m0 = blockIdx.y * 16 * MT;
+    const long t = blockIdx.x;
+    const f16* x[MT];
+#pragma unroll
+    for (int u = 0; u < MT; u++) x[u] = a.x + min(m0 + 16 * u + i, a.m - 1) * a.ldx + 8 * j;
+    f32x4 sum[MT] = {};
+    for (int c = wave; c < chunks; c += waves) {
         const long entry = t * chunks + c;
-        for (int g = 0; g < groups; g++) {
-            float part = 0.f;
-            for (int k = g * w.group; k < (g + 1) * w.group; k += 8) {
-                const int s = k / 32, j = k / 8 % 4;
-                const unsigned q = *(const unsigned*)(w.codes + (entry * 64 + 16 * j + i) * 16 + 4 * s);
-                const f16x8 v = ld8(x + c * 128 + k);
-                for (int e = 0; e < 8; e++) part = fmaf((float)((int)(q >> bit_of(e) & 15) - 8), (float)v[e], part);
+        const u32x4 q = *(const u32x4*)(w.codes + (entry * 64 + lane) * 16);
+        const Scales<G> scale = scales_at<G>(w.scales + (entry * 16 + i) * G);
+        f16x8 v[MT][4];
+#pragma unroll
+        for (int u = 0; u < MT; u++)
+#pragma unroll
+            for (int s = 0; s < 4; s++) v[u][s] = ld8(x[u] + c * 128 + 32 * s);
+        entry_product<MT, G>(q, scale, [&](int u, int s) { return v[u][s]; }, sum);
+    }
+#pragma unroll
+    for (int u = 0; u < MT; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) red[(wave * 4 * MT + 4 * u + e) * LD + lane] = sum[u][e];
+    __syncthreads();
+    for (int o = threadIdx.x; o < 256 * MT; o += blockDim.x) {
+        const int n = o & 15, m = o >> 4;  // row m of a tile of x is result 16 (m / 4) + n of m % 4
+        const int at = (4 * (m >> 4) + (m & 3)) * LD + 16 * (m >> 2 & 3) + n;
+        float y = 0.f;
+        for (int k = 0; k < waves; k++) y += red[k * 4 * MT * LD + at];
+        if (m0 + m < a.m && t * 16 + n < w.n) finish(a, m0 + m, (int)(t * 16 + n), y);
+    }
+}
+
+// Many rows of weights: x lies in LDS, in the order of operands, and each wave takes 16 rows of weights and all of their columns,
+// the next entries on their way.
+template <int MT, int G>
+__global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
+    extern __shared__ u32x4 xs[];  // [chunk][s][MT][64]
+    constexpr int AHEAD = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / 64;
+    const int i = lane & 15, j = lane >> 4, chunks = w.k / 128, m0 = blockIdx.y * 16 * MT, tiles = (w.n + 15) / 16;
+    const int t = blockIdx.x * waves + wave, tt = min(t, tiles - 1);
+    // entries past the last read as zeros, without a memory access: loads need no branches
+    const auto rc = rsrc(w.codes + (long)tt * chunks * 1024, chunks * 1024);
+    const auto rs = rsrc(w.scales + (long)tt * chunks * 16 * G, chunks * 16 * G * 2);
+    u32x4 q[AHEAD];
+    Scales<G> scale[AHEAD];
+    auto fetch = [&](int c, int to) {
+        q[to] = __builtin_amdgcn_raw_buffer_load_b128(rc, c * 1024 + lane * 16, 0, 2);
+        const int at = (c * 16 + i) * G * 2;
+        if constexpr (G == 4) scale[to] = __builtin_bit_cast(Scales<4>, __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 2));
+        else if constexpr (G == 2) scale[to] = __builtin_bit_cast(Scales<2>, __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 2));
+        else scale[to] = __builtin_bit_cast(Scales<1>, __builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 2));
+    };
+#pragma unroll
+    for (int d = 0; d < AHEAD; d++) fetch(d, d);
+    for (int f = wave; f < chunks * 4 * MT; f += waves) {
+        const int u = f % MT, c4 = f / MT;  // 32 columns
+        xs[f * 64 + lane] = __builtin_bit_cast(u32x4, ld8(a.x + min(m0 + 16 * u + i, a.m - 1) * a.ldx + c4 * 32 + 8 * j));
+    }
+    __syncthreads();
+    f32x4 sum[MT] = {};
+    for (int c0 = 0; c0 < chunks; c0 += AHEAD)
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++) {
+            const int c = c0 + d;
+            if (c < chunks)
+                entry_product<MT, G>(q[d], scale[d], [&](int u, int s) { return __builtin_bit_cast(f16x8, xs[((c * 4 + s) * MT + u) * 64 + lane]); }, sum);
+            fetch(c + AHEAD, d);
+        }
+    const int n = t * 16 + i;
+    if (t >= tiles || n >= w.n) return;
+#pragma unroll
+    for (int u = 0; u < MT; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int m = m0 + 16 * u + 4 * j + e;
+            if (m < a.m) finish(a, m, n, sum[u][e]);
+        }
+}
+
+// Many rows of x: tiles of 32 MT rows of x x 32 NT of weights, four waves of 16 MT x 16 NT. 128 columns at a time: those of x go
+// straight into LDS, in two buffers, the weights' codes into registers.
+template <int MT, int NT, int G>
+__global__ void __launch_bounds__(256, 2) tile_kernel(MzW4 w, MzW4Linear a) {
+    extern __shared__ u32x4 xs[];  // [2][32 MT rows][16 pieces of 8 columns, piece p of row r at p ^ r % 16]
+    constexpr int ROWS = 32 * MT;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, j = lane >> 4, chunks = w.k / 128, tiles = (w.n + 15) / 16;
+    const int m0 = blockIdx.y * ROWS, wm = (wave & 1) * 16 * MT, t0 = blockIdx.x * 2 * NT + (wave >> 1) * NT;
+    // row r of the tile is loaded by lanes 16 (r % 4) .. + 15 of wave r / 4 % 4, piece by piece
+    auto load_x = [&](int c) {
+#pragma unroll
+        for (int z = 0; z < ROWS / 16; z++) {
+            const int r = 16 * z + 4 * wave + j, p = i ^ (r & 15);
+            const f16* from = a.x + min(m0 + r, a.m - 1) * a.ldx + c * 128 + 8 * p;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)(xs + (c & 1) * ROWS * 16 + (16 * z + 4 * wave) * 16), 16, 0, 0);
+        }
+    };
+    u32x4 q[NT];
+    Scales<G> scale[NT];
+    auto load_w = [&](int c) {
+#pragma unroll
+        for (int u = 0; u < NT; u++) {
+            const long entry = (long)min(t0 + u, tiles - 1) * chunks + c;
+            q[u] = *(const u32x4*)(w.codes + (entry * 64 + lane) * 16);
+            scale[u] = scales_at<G>(w.scales + (entry * 16 + i) * G);
+        }
+    };
+    f32x4 sum[MT][NT] = {};
+    load_x(0);
+    load_w(0);
+    for (int c = 0; c < chunks; c++) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of x have arrived,
+        __syncthreads();                     // everyone's have, and nobody reads the other buffer any more
+        u32x4 qc[NT];
+        Scales<G> sc[NT];
+#pragma unroll
+        for (int u = 0; u < NT; u++) qc[u] = q[u], sc[u] = scale[u];
+        if (c + 1 < chunks) {
+            load_x(c + 1);
+            load_w(c + 1);
+        }
+        const u32x4* buf = xs + (c & 1) * ROWS * 16;
+        f32x4 part[MT][NT];
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            f16x8 x[MT];
+#pragma unroll
+            for (int u = 0; u < MT; u++) x[u] = __builtin_bit_cast(f16x8, buf[(wm + 16 * u + i) * 16 + ((4 * s + j) ^ i)]);
+#pragma unroll
+            for (int v = 0; v < NT; v++) {
+                const f16x8 y = numbers(qc[v][s]);
+#pragma unroll
+                for (int u = 0; u < MT; u++) part[u][v] = mfma16(x[u], y, s % (4 / G) ? part[u][v] : f32x4{});
+                if (s % (4 / G) == 4 / G - 1) {
+                    const float d = (float)sc[v].v[s / (4 / G)];
+#pragma unroll
+                    for (int u = 0; u < MT; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sum[u][v][e] = fmaf(part[u][v][e], d, sum[u][v][e]);
+                }
             }
-            sum = fmaf((float)w.scales[(entry * 4 + (i >> 2)) * groups * 4 + g * 4 + (i & 3)], part, sum);
         }
     }
-    if (a.bias) sum += (float)a.bias[n];
-    const long o = mi * a.ldo + n;
-    switch (a.epilogue) {
-        case 0: ((f16*)a.out)[o] = (f16)sum; break;
-        case 1: ((f16*)a.out)[o] = (f16)gelu_erf_h(sum); break;
-        case 2: ((float*)a.out)[o] += sum; break;
-        default: ((float*)a.out)[o] = sum;
+#pragma unroll
+    for (int v = 0; v < NT; v++) {
+        const int n = (t0 + v) * 16 + i;
+        if (n >= w.n) continue;
+#pragma unroll
+        for (int u = 0; u < MT; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int m = m0 + wm + 16 * u + 4 * j + e;
+                if (m < a.m) finish(a, m, n, sum[u][v][e]);
+            }
     }
+}
+
+int blocks(long x, long per) { return (int)((x + per - 1) / per); }
+
+template <int G>
+void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
+    const int tiles = blocks(w.n, 16), chunks = w.k / 128, cus = mz_cu_count();
+    if (a.m > 64 && (long)blocks(a.m, 128) * blocks(w.n, 128) >= cus) {
+        hipLaunchKernelGGL((tile_kernel<4, 4, G>), dim3(blocks(w.n, 128), blocks(a.m, 128)), dim3(256), 2 * 128 * 256, s, w, a);
+        return;
+    }
+    if (a.m > 64 && (long)blocks(a.m, 64) * blocks(w.n, 64) >= cus / 2) {
+        hipLaunchKernelGGL((tile_kernel<2, 2, G>), dim3(blocks(w.n, 64), blocks(a.m, 64)), dim3(256), 2 * 64 * 256, s, w, a);
+        return;
+    }
+    const int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4, my = blocks(a.m, 16 * mt);
+    const size_t lds = (size_t)chunks * 4 * mt * 1024;
+    if (tiles >= 4 * cus && lds <= 160 * 1024) {
+        const int waves = std::min(16, blocks(tiles, (long)cus * blocks(tiles, 16L * cus)));
+        const dim3 grid(blocks(tiles, waves), my), block(64 * waves);
+        if (mt == 1) hipLaunchKernelGGL((row_kernel<1, G>), grid, block, lds, s, w, a);
+        else if (mt == 2) hipLaunchKernelGGL((row_kernel<2, G>), grid, block, lds, s, w, a);
+        else hipLaunchKernelGGL((row_kernel<4, G>), grid, block, lds, s, w, a);
+        return;
+    }
+    const int most = mt == 4 ? 8 : 16, waves = blocks(chunks, blocks(chunks, most));
+    const dim3 grid(tiles, my), block(64 * waves);
+    const size_t red = (size_t)waves * 4 * mt * 68 * 4;
+    if (mt == 1) hipLaunchKernelGGL((split_kernel<1, G>), grid, block, red, s, w, a);
+    else if (mt == 2) hipLaunchKernelGGL((split_kernel<2, G>), grid, block, red, s, w, a);
+    else hipLaunchKernelGGL((split_kernel<4, G>), grid, block, red, s, w, a);
 }
 
 unsigned entry_groups(const MzW4& w) { return (unsigned)(((long)(w.n + 15) / 16 * (w.k / 128) + 3) / 4); }
@@ -139,6 +363,8 @@ hipError_t mz_w4_unpack_launch(hipStream_t s, const MzW4& w, f16* dst, long ld) 
 }
 
 hipError_t mz_w4_linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
-    hipLaunchKernelGGL(linear_kernel, dim3((w.n + 15) / 16, (a.m + 15) / 16), dim3(256), 0, s, w, a);
+    if (w.group == 32) linear_launch<4>(s, w, a);
+    else if (w.group == 64) linear_launch<2>(s, w, a);
+    else linear_launch<1>(s, w, a);
     return hipGetLastError();
 }

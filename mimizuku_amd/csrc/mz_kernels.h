@@ -334,7 +334,7 @@ struct MzW4Linear {
     long ldo;
 };
 // what a launch takes: rows of weights, rows of x
-#define MZ_W4_MOST_N (1 << 26)
+#define MZ_W4_MOST_N (1 << 25)  // (tiles of 16 rows, a workgroup of up to 1024 threads each: fewer than 2^32 along x)
 #define MZ_W4_MOST_M (1 << 20)
 hipError_t mz_w4_pack_launch(hipStream_t s, const MzW4& w, const f16* src, long ld);
 hipError_t mz_w4_unpack_launch(hipStream_t s, const MzW4& w, f16* dst, long ld);

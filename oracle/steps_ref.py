@@ -28,7 +28,7 @@ def w4_codes(w, group):
 
 
 def w4_bytes_of(codes, scales, group):
-    """The two arrays as the header lays them out: u8 [tiles][k / 128][64][16], f16 [tiles][k / 128][4][128 / group][4]."""
+    """The two arrays as the header lays them out: u8 [tiles][k / 128][64][16], f16 [tiles][k / 128][16][128 / group]."""
     n, k = codes.shape
     tiles, chunks, groups = -(-n // 16), k // 128, 128 // group
     c = np.zeros((tiles * 16, k), np.int64)
@@ -39,7 +39,7 @@ def w4_bytes_of(codes, scales, group):
         words |= v[..., e].transpose(0, 2, 4, 1, 3) << np.uint32(4 * (e // 2) + 16 * (e % 2))
     s = np.zeros((tiles * 16, k // group), np.float16)
     s[:n] = scales
-    s = s.reshape(tiles, 4, 4, chunks, groups).transpose(0, 3, 1, 4, 2)  # [tile][j][r][chunk][g]
+    s = s.reshape(tiles, 16, chunks, groups).transpose(0, 2, 1, 3)
     return np.ascontiguousarray(words).view(np.uint8).reshape(tiles, chunks, 64, 16), np.ascontiguousarray(s)
 
 
