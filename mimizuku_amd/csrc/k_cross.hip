@@ -1,12 +1,31 @@
 // Attention over an encoder's fp16 keys and values of any length (mz_cross_attention_args in mimizuku.h).
+//
+// One pass over the positions with the running maximum and sum of the softmax. A workgroup takes 16 QT queries of one (row, kv
+// head) (its tokens times the query heads that share the kv head) and a share of the blocks of 32 positions; its waves take the
+// blocks in turn, each with a state of its own, and join them at the end.
+//
+// Per block, with 16x16x32 products: S^T = K Q^T, the rows of tile j being positions 8 (i / 4) + 4 j + i % 4, so that lane (query
+// c, group g) of the two results holds the eight positions 8 g .. 8 g + 7 of its query: in this order they are the k values of
+// that lane in the product O^T = V^T P^T, so probabilities never leave their registers. Values lie by positions: lane (i, g) loads
+// channels 4 i .. 4 i + 3 of those eight positions, eight bytes each, and 16 byte permutations make of them its operands of four
+// products, whose row i is channel 4 i + u.
+//
+// P goes into its product as the sum of two fp16 numbers, 20 bits or more down to 2^-31 of a row's largest: one alone would add an error of
+// the size of the output's rounding. The maximum of a state is moved only when a score passes it by more than 8 (in powers of
+// two), so that most blocks need no exchange between lanes and no rescaling; P is carried times 2^7, at most 2^15.
 #include <algorithm>
 
+#include "mz_attn.h"
 #include "mz_common.h"
 #include "mz_kernels.h"
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int BLK = 32;
+constexpr float UP = 7.f;  // log2 of what P is carried times
 
 // what a row's queries see: positions first .. end - 1 of its slot
 struct Seen {
@@ -14,70 +33,502 @@ struct Seen {
     int first, end, count;
 };
 __device__ __forceinline__ Seen seen_of(const MzCross& a, int r) {
+    // (all that there are go out together, an absent one's place being some other word: a branch around each would wait for one
+    // after the other)
+    int slot = 0, first = 0, len = 0, count = 0;
+    const int* any = a.slot ? a.slot : a.first ? a.first : a.len ? a.len : a.count;
+    if (any) {
+        slot = *(a.slot ? a.slot + r : any);
+        first = *(a.first ? a.first + r : any);
+        len = *(a.len ? a.len + r : any);
+        count = *(a.count ? a.count + r : any);
+        slot = __builtin_amdgcn_readfirstlane(slot);
+        first = __builtin_amdgcn_readfirstlane(first);
+        len = __builtin_amdgcn_readfirstlane(len);
+        count = __builtin_amdgcn_readfirstlane(count);
+    }
     Seen s;
-    s.slot = a.slot ? a.slot[r] : r;
-    s.count = a.count ? min(max(a.count[r], 0), a.tokens) : a.tokens;
-    s.first = a.first ? max(a.first[r], 0) : 0;
-    s.end = a.len ? min(max(a.len[r], 0), a.positions) : a.positions;
+    s.slot = a.slot ? slot : r;
+    s.count = a.count ? min(max(count, 0), a.tokens) : a.tokens;
+    s.first = a.first ? max(first, 0) : 0;
+    s.end = a.len ? min(max(len, 0), a.positions) : a.positions;
     if (s.slot < 0 || s.slot >= a.slots) s.slot = s.end = 0;
     s.end = max(s.end, s.first);  // (nothing: first .. first)
     return s;
 }
 
-// A wave: one query. 64 positions at a time, a lane a position for the scores and a channel for the sums.
-__global__ void __launch_bounds__(64) simple_kernel(MzCross a) {
-    __shared__ float qs[64];
-    const int lane = threadIdx.x, pair = blockIdx.x, i = blockIdx.y / (a.heads / a.kv_heads);
-    const int r = pair / a.kv_heads, kh = pair - r * a.kv_heads, grp = a.heads / a.kv_heads, h = kh * grp + blockIdx.y % grp;
-    const Seen s = seen_of(a, r);
-    if (i >= s.count) return;
-    qs[lane] = (float)a.q[r * a.q_row + i * a.q_token + h * a.q_head + lane];
-    __syncthreads();
-    const f16* k = a.k + s.slot * a.k_slot + kh * a.k_head;
-    const f16* v = a.v + s.slot * a.v_slot + kh * a.v_head;
-    const float scale2 = a.scale * LOG2E;
-    auto score = [&](int p) {
-        float d = 0.f;
-        for (int c = 0; c < 64; c += 8) {
-            const f16x8 x = ld8(k + p * a.k_pos + c);
-            for (int e = 0; e < 8; e++) d = fmaf((float)x[e], qs[c + e], d);
-        }
-        return d * scale2;
-    };
-    float m = NOTHING, l = 0.f, o = 0.f;
-    for (int p0 = s.first; p0 < s.end; p0 += 64) {
-        const int p = p0 + lane;
-        const float d = p < s.end ? score(p) : -INFINITY;
-        const float mn = fmaxf(m, wave_max(d)), f = __builtin_amdgcn_exp2f(m - mn), x = __builtin_amdgcn_exp2f(d - mn);
-        m = mn;
-        l = l * f + wave_sum(x);
-        o *= f;
-        for (int j = 0; j < min(64, s.end - p0); j++)
-            o = fmaf(__shfl(x, j), (float)v[(p0 + j) * a.v_pos + lane], o);
+struct Launch {
+    int qt, tiles, splits;  // queries of a workgroup / 16, such tiles of a (row, kv head), workgroups that share the blocks
+    int waves, own;         // waves of a workgroup; whether each has 32 queries of its own (qt is not used then)
+    int kept;               // alignment rows: scores that a workgroup keeps in LDS for each query, 0: in their rows
+    int group;              // query heads of a kv head
+    unsigned by_heads, by_group, by_splits;  // for dividing by kv_heads, group and splits (see divided)
+};
+
+// The bytes of `n` positions `step` bytes apart, as far as a buffer descriptor reaches: what lies behind reads as zeros. (A block's
+// are below 2^30 + 2^7.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t positions_at(const f16* p, long step, int n) {
+    const long bytes = n > 0 ? (n - 1) * step + 128 : 0;
+    return rsrc(p, (unsigned)min(bytes, 0x7fffffffL));
+}
+
+// A block as it lies: keys as operands of two tiles, values by positions.
+struct Raw {
+    u32x4 k[2][2];
+    u32x2 v[8];
+};
+
+// the four operands of values: row i of product u is channel 4 i + u
+__device__ __forceinline__ void by_channels(const u32x2 (&v)[8], f16x8 (&to)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const unsigned sel = u & 1 ? 0x07060302u : 0x05040100u;  // the high or low halves of both
+        u32x4 x;
+#pragma unroll
+        for (int p = 0; p < 4; p++) x[p] = __builtin_amdgcn_perm(v[2 * p + 1][u >> 1], v[2 * p][u >> 1], sel);
+        to[u] = __builtin_bit_cast(f16x8, x);
     }
-    a.out[r * a.out_row + i * a.out_token + h * a.out_head + lane] = (f16)(l == 0.f ? 0.f : o / l);
-    const float lse2 = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
-    if (a.lse && lane == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
-    if (!a.align) return;
-    const int at = a.head_slot[h];
-    bool mine = at >= 0 && at < a.align_heads;
-    for (int j = 0; j < h; j++) mine &= a.head_slot[j] != at;
-    if (!mine) return;
-    float* row = a.align + (((long)r * a.tokens + i) * a.align_heads + at) * a.align_cols;
-    for (int p = lane; p < a.align_cols; p += 64)
-        row[p] = p >= s.first && p < s.end ? __builtin_amdgcn_exp2f(score(p) - lse2) : 0.f;
+}
+
+template <int QT>
+struct State {
+    float m[QT], l[QT];
+    f32x4 acc[QT][4];  // result u of lane (c, g) holds channels 16 g + 4 e + u of query c
+};
+
+template <int QT, bool ALIGN, int NW, bool OWN>
+__global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kernel(MzCross a, Launch n) {
+    static_assert(!(OWN && ALIGN));
+    __shared__ float red[OWN ? 1 : NW][16][68], ms[NW][16], ls[NW][16];
+    __shared__ float lse2s[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    // x: (row, kv head), padded to a multiple of the XCDs, so that what shares keys and values shares an XCD; y: the tiles; z: the
+    // shares of the blocks
+    const int pairs = a.rows * a.kv_heads, pair = min((int)blockIdx.x, pairs - 1);
+    const int tile = blockIdx.y, split = blockIdx.z, grp = n.group;
+    const int r = divided(pair, a.kv_heads, n.by_heads), kh = pair - r * a.kv_heads;
+    const Seen s = seen_of(a, r);
+    constexpr int SHARE = OWN ? NW : 1;
+    const int nq = a.tokens * grp, w0 = tile * 16 * QT * SHARE;
+    const int q0 = OWN ? w0 + 16 * QT * wave : w0;  // this wave's first query
+    auto token_of = [&](int x) { return divided(x, grp, n.by_group); };
+    if ((int)blockIdx.x >= pairs || token_of(w0) >= s.count) return;  // none of its tokens is there
+    const int nb = (s.end - s.first + BLK - 1) / BLK;
+    // (splits is at most 256, nb below 2^26: products below 2^31 where splits is above 1 only if nb is below 2^23)
+    const int b0 = OWN || n.splits == 1 ? 0 : (int)((long)nb * split / n.splits);
+    const int b1 = OWN || n.splits == 1 ? nb : (int)((long)nb * (split + 1) / n.splits);
+
+    const f16* kbase = a.k + s.slot * a.k_slot + kh * a.k_head + s.first * a.k_pos;
+    const f16* vbase = a.v + s.slot * a.v_slot + kh * a.v_head + s.first * a.v_pos;
+    const int there = s.end - s.first;  // positions
+
+    extern __shared__ float kept[];  // [query][n.kept]
+    __shared__ int index[ALIGN ? 64 : 1];
+    const int mine = ALIGN && tid < a.heads ? a.head_slot[tid] : -1;
+    f16x8 qf[QT][2];
+    float* al[QT];
+    auto align_row = [&](int t) -> float* {
+        const int x = q0 + 16 * t + c, i = token_of(x), k = x < nq && i < s.count ? index[x - i * grp] : -1;
+        return k >= 0 ? a.align + (((long)r * a.tokens + i) * a.align_heads + k) * a.align_cols : nullptr;
+    };
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const int x = q0 + 16 * t + c, i = token_of(x), h = kh * grp + x - i * grp;
+        const bool on = x < nq && i < s.count;
+        const f16* q = a.q + r * a.q_row + (on ? i * a.q_token + h * a.q_head : 0) + 8 * g;
+        qf[t][0] = on ? ld8(q) : f16x8{};
+        qf[t][1] = on ? ld8(q + 32) : f16x8{};
+        al[t] = nullptr;
+    }
+
+    // Blocks past the last read as zeros, without a memory access: the loads need no branches, around which the compiler would
+    // wait for all that is on its way.
+    const unsigned kstep = (unsigned)(a.k_pos * 2), vstep = (unsigned)(a.v_pos * 2);
+    const unsigned kat = (8 * (c >> 2) + (c & 3)) * kstep + 16 * g, vat = 8 * g * vstep + 8 * c;
+    constexpr int POLICY = QT == 1 && !OWN ? 2 : 0;  // nontemporal where no other workgroup reads the same
+    auto fetch = [&](int b, Raw& w) {
+        const int left = b < b1 ? there - b * BLK : 0;
+        const auto rk = positions_at(kbase + (long)b * BLK * a.k_pos, kstep, left);
+        const auto rv = positions_at(vbase + (long)b * BLK * a.v_pos, vstep, left);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int z = 0; z < 2; z++) w.k[j][z] = __builtin_amdgcn_raw_buffer_load_b128(rk, kat + 4 * j * kstep + 64 * z, 0, POLICY);
+#pragma unroll
+        for (int e = 0; e < 8; e++) w.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, vat + e * vstep, 0, POLICY);
+    };
+
+    State<QT> st;
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        st.m[t] = NOTHING;
+        st.l[t] = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; u++) st.acc[t][u] = f32x4{};
+    }
+    const float scale2 = a.scale * LOG2E;
+    float inf = INFINITY;
+    asm("" : "+s"(inf));
+    auto products = [&](int b, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4]) {
+        const int p0 = b * BLK + 8 * g;  // this lane's positions
+        const bool whole = (b + 1) * BLK <= there;
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            f32x4 d[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) d[j] = mfma16(kf[j][1], qf[t][1], mfma16(kf[j][0], qf[t][0], f32x4{}));
+            if (!whole)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (p0 + e >= there) d[e >> 2][e & 3] = -INFINITY;
+            if (ALIGN && al[t] != nullptr) {
+                const f32x4 x[2] = {d[0] * scale2, d[1] * scale2};
+                if (n.kept) {
+                    f32x4* o = (f32x4*)(kept + (16 * t + c) * n.kept + p0 - b0 * BLK);
+                    o[0] = x[0];
+                    o[1] = x[1];
+                } else {
+                    for (int e = 0; e < 8; e++)
+                        if (p0 + e < there && s.first + p0 + e < a.align_cols) {
+                            float* o = al[t] + s.first + p0 + e;
+                            if (n.splits > 1) shared_store(o, x[e >> 2][e & 3]);
+                            else *o = x[e >> 2][e & 3];
+                        }
+                }
+            }
+            const float top = scale2 * fmaxf(fmaxf(larger(d[0][0], d[0][1], inf), larger(d[0][2], d[0][3], inf)),
+                                             fmaxf(larger(d[1][0], d[1][1], inf), larger(d[1][2], d[1][3], inf)));
+            if (__ballot(top > st.m[t] + 8.f)) {
+                const float mn = fmaxf(st.m[t], column_max(top)), f = __builtin_amdgcn_exp2f(st.m[t] - mn);
+                st.m[t] = mn;
+                st.l[t] *= f;
+#pragma unroll
+                for (int u = 0; u < 4; u++) st.acc[t][u] *= f;
+            }
+            const float less = UP - st.m[t];
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(fmaf(d[e >> 2][e & 3], scale2, less));
+            st.l[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            u32x4 high, rest;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const auto h = __builtin_amdgcn_cvt_pkrtz(x[2 * e], x[2 * e + 1]);
+                high[e] = __builtin_bit_cast(unsigned, h);
+                rest[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(x[2 * e] - (float)h[0], x[2 * e + 1] - (float)h[1]));
+            }
+            const f16x8 p = __builtin_bit_cast(f16x8, high), q = __builtin_bit_cast(f16x8, rest);
+#pragma unroll
+            for (int u = 0; u < 4; u++) st.acc[t][u] = mfma16(vf[u], p, mfma16(vf[u], q, st.acc[t][u]));
+        }
+    };
+    if constexpr (OWN) {
+        // Each wave loads a quarter of a block, the keys' two tiles or half of the values' positions, and puts it as operands where
+        // all find it, a block ahead; what is behind the last block is that one again.
+        __shared__ u32x4 pieces[2][8][64];
+        u32x4 raw[2];
+        u32x2 rv[8];
+        const bool values = wave >= 2;
+        auto take = [&](int i) {
+            const int b = min(i, nb - 1), left = there - b * BLK;
+            if (!values) {
+                const auto rk = positions_at(kbase + (long)b * BLK * a.k_pos, kstep, left);
+#pragma unroll
+                for (int z = 0; z < 2; z++) raw[z] = __builtin_amdgcn_raw_buffer_load_b128(rk, kat + 4 * wave * kstep + 64 * z, 0, 0);
+            } else {
+                const auto r2 = positions_at(vbase + (long)b * BLK * a.v_pos, vstep, left);
+#pragma unroll
+                for (int e = 0; e < 8; e++) rv[e][0] = __builtin_amdgcn_raw_buffer_load_b32(r2, vat + 4 * (wave - 2) + e * vstep, 0, 0);
+            }
+        };
+        auto put = [&](int i) {
+            u32x4* o = &pieces[i & 1][2 * wave][lane];
+            if (!values) {
+                o[0] = raw[0];
+                o[64] = raw[1];
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const unsigned sel = u ? 0x07060302u : 0x05040100u;
+                    u32x4 x;
+#pragma unroll
+                    for (int p = 0; p < 4; p++) x[p] = __builtin_amdgcn_perm(rv[2 * p + 1][0], rv[2 * p][0], sel);
+                    o[64 * u] = x;
+                }
+            }
+        };
+        if (nb > 0) {
+            take(0);
+            put(0);
+            take(1);
+            __syncthreads();
+            for (int i = 0; i < nb; i++) {
+                put(i + 1);
+                take(i + 2);
+                f16x8 kf[2][2], vf[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    kf[k >> 1][k & 1] = __builtin_bit_cast(f16x8, pieces[i & 1][k][lane]);
+                    vf[k] = __builtin_bit_cast(f16x8, pieces[i & 1][4 + k][lane]);
+                }
+                products(i, kf, vf);
+                lds_barrier();
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const int x = q0 + 16 * t + c, i = token_of(x), h = kh * grp + x - i * grp;
+            const float ll = column_sum(st.l[t]), f = ll == 0.f ? 0.f : 1.f / ll;
+            if (x >= nq || i >= s.count) continue;
+            f16* o = a.out + r * a.out_row + i * a.out_token + h * a.out_head + 16 * g;
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                f16x8 y;
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = (f16)(st.acc[t][e & 3][2 * z + (e >> 2)] * f);
+                *(f16x8*)(o + 8 * z) = y;
+            }
+            if (a.lse && g == 0)
+                a.lse[((long)r * a.tokens + i) * a.heads + h] = ll == 0.f ? -INFINITY : (st.m[t] - UP + __builtin_amdgcn_logf(ll)) * LN2;
+        }
+        return;
+    } else {
+        constexpr int DEPTH = 2;
+        Raw w[DEPTH];
+        const int head = b0 + wave;
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) fetch(head + NW * i, w[i]);
+        if constexpr (ALIGN) {  // (while they are on their way)
+            align_indices<64 * NW>(a.head_slot, a.align_heads, kh * grp, grp, mine, index);
+#pragma unroll
+            for (int t = 0; t < QT; t++) al[t] = align_row(t);
+        }
+        for (int b = head; b < b1; b += NW * DEPTH)
+#pragma unroll
+            for (int i = 0; i < DEPTH; i++) {
+                const int bi = b + NW * i;
+                if (bi < b1) {
+                    f16x8 kf[2][2], vf[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) kf[j >> 1][j & 1] = __builtin_bit_cast(f16x8, w[i].k[j >> 1][j & 1]);
+                    by_channels(w[i].v, vf);
+                    products(bi, kf, vf);
+                }
+                fetch(bi + NW * DEPTH, w[i]);
+            }
+    }
+
+    // the waves' states joined, 16 queries at a time, by the first 256 threads
+    const int col = tid >> 4 & 15, d4 = (tid & 15) * 4;
+    const bool mine256 = NW == 4 || tid < 256;
+    // Alignment rows of 16 queries: their scores (in powers of two, get(query, row, position)) to probabilities, 0 where nothing
+    // is seen, by all threads, eight of a row's scores a thread at a time and the first ones of four rows.
+    constexpr int STRIDE = 64 * NW;
+    auto rows = [&](int t) { return (unsigned)__ballot(al[t] != nullptr) & 0xffff; };
+    auto row_of_query = [&](int t, int k) {
+        const unsigned long at = (unsigned long)al[t];
+        return (float*)((unsigned long)(unsigned)__builtin_amdgcn_readlane((int)(at >> 32), k) << 32 |
+                        (unsigned)__builtin_amdgcn_readlane((int)at, k));
+    };
+    const int to = min(s.end, a.align_cols);
+    auto scores = [&](int t, int k, int p0, float (&x)[8], auto get) {
+        const float* row = row_of_query(t, k);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int p = p0 + STRIDE * j;
+            x[j] = -INFINITY;
+            if (p >= s.first && p < to) x[j] = get(16 * t + k, row, p);
+        }
+    };
+    // of the first FEW of the rows `has`
+    constexpr int FEW = 4;
+    typedef float Few[FEW][8];
+    auto few_scores = [&](int t, unsigned has, Few& x, auto get) {
+#pragma unroll
+        for (int u = 0; u < FEW; u++) {
+            if (!has) break;
+            scores(t, __ffs(has) - 1, tid, x[u], get);
+            has &= has - 1;
+        }
+    };
+    // (x: those of the first rows are on their way)
+    auto probabilities = [&](int t, Few& x, auto get) {
+        for (unsigned has = rows(t); has;) {
+#pragma unroll
+            for (int u = 0; u < FEW; u++) {
+                if (!has) break;
+                const int k = __ffs(has) - 1;
+                has &= has - 1;
+                float* const row = row_of_query(t, k);
+                const float lse2 = lse2s[k];
+                for (int p0 = tid; p0 < a.align_cols; p0 += 8 * STRIDE) {
+                    if (p0 != tid) scores(t, k, p0, x[u], get);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (p0 + STRIDE * j < a.align_cols)
+                            row[p0 + STRIDE * j] = x[u][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[u][j] - lse2);
+                }
+            }
+            few_scores(t, has, x, get);
+        }
+    };
+    const int share0 = s.first + b0 * BLK;
+    auto in_lds = [&](int q, const float*, int p) { return kept[q * n.kept + p - share0]; };
+    auto in_place = [&](int, const float* row, int p) { return row[p]; };
+    auto in_memory = [&](int, const float* row, int p) { return shared_load(row + p); };
+    auto emit = [&](int t, float mm, float ll, f32x4 o, Few& x, auto get) {
+        const int q = q0 + 16 * t + col, i = token_of(q), h = kh * grp + q - i * grp;
+        const float inv = ll == 0.f ? 0.f : 1.f / ll, lse2 = ll == 0.f ? -INFINITY : mm - UP + __builtin_amdgcn_logf(ll);
+        if (mine256 && q < nq && i < s.count) {
+            st4(a.out + r * a.out_row + i * a.out_token + h * a.out_head + d4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            if (a.lse && d4 == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
+        }
+        if (ALIGN) {
+            if (mine256 && d4 == 0) lse2s[col] = lse2;
+            __syncthreads();
+            probabilities(t, x, get);
+            __syncthreads();
+        }
+    };
+    float* const states = a.work + JOIN_COUNTERS + ((long)pair * n.tiles + tile) * n.splits * (16 * QT) * STATE;
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const float lt = column_sum(st.l[t]);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            *(f32x4*)&red[wave][c][16 * g + 4 * e] = f32x4{st.acc[t][0][e], st.acc[t][1][e], st.acc[t][2][e], st.acc[t][3][e]};
+        if (g == 0) {
+            ms[wave][c] = st.m[t];
+            ls[wave][c] = lt;
+        }
+        __syncthreads();
+        float mm = ms[0][col], ll = 0.f;
+#pragma unroll
+        for (int k = 1; k < NW; k++) mm = fmaxf(mm, ms[k][col]);
+        f32x4 o = {};
+#pragma unroll
+        for (int k = 0; k < NW; k++) {
+            const float f = __builtin_amdgcn_exp2f(ms[k][col] - mm);
+            ll = fmaf(f, ls[k][col], ll);
+            const f32x4 y = *(const f32x4*)&red[k][col][d4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(f, y[e], o[e]);
+        }
+        if (n.splits == 1) {
+            Few x;
+            if (n.kept) {
+                few_scores(t, ALIGN ? rows(t) : 0, x, in_lds);
+                emit(t, mm, ll, o, x, in_lds);
+            } else {
+                few_scores(t, ALIGN ? rows(t) : 0, x, in_place);
+                emit(t, mm, ll, o, x, in_place);
+            }
+        } else if (mine256 && q0 + 16 * t + col < nq) {
+            float* w = states + (split * (16 * QT) + 16 * t + col) * STATE;
+            shared_store(w + d4, o[0], o[1]);
+            shared_store(w + d4 + 2, o[2], o[3]);
+            if (d4 == 0) shared_store(w + 64, mm, ll);
+        }
+        if (ALIGN && n.splits > 1 && n.kept)  // the share's scores to where the last workgroup finds them
+            for (unsigned has = rows(t); has; has &= has - 1) {
+                const int k = __ffs(has) - 1;
+                float* const row = row_of_query(t, k);
+                for (int p = share0 + tid; p < min(min(s.first + b1 * BLK, s.end), a.align_cols); p += STRIDE)
+                    shared_store(row + p, in_lds(16 * t + k, row, p));
+            }
+        if (t + 1 < QT) __syncthreads();
+    }
+    if (n.splits == 1 || !last_of((unsigned*)a.work + (long)pair * n.tiles + tile, n.splits)) return;
+    // the last of the workgroups that share these queries joins their states
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        float mm = NOTHING, ll = 0.f;
+        f32x4 o = {};
+        Few x;
+        few_scores(t, ALIGN ? rows(t) : 0, x, in_memory);  // (they come with the states)
+        if (mine256 && q0 + 16 * t + col < nq)
+            for (int k0 = 0; k0 < n.splits; k0 += 4) {
+                float2 y[4][3];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float* w = states + (min(k0 + k, n.splits - 1) * (16 * QT) + 16 * t + col) * STATE;
+                    y[k][0] = shared_load2(w + d4);
+                    y[k][1] = shared_load2(w + d4 + 2);
+                    y[k][2] = shared_load2(w + 64);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (k0 + k >= n.splits) continue;
+                    const float mn = fmaxf(mm, y[k][2].x), f0 = __builtin_amdgcn_exp2f(mm - mn), f1 = __builtin_amdgcn_exp2f(y[k][2].x - mn);
+                    mm = mn;
+                    ll = fmaf(ll, f0, y[k][2].y * f1);
+                    o = f32x4{fmaf(o[0], f0, y[k][0].x * f1), fmaf(o[1], f0, y[k][0].y * f1), fmaf(o[2], f0, y[k][1].x * f1),
+                              fmaf(o[3], f0, y[k][1].y * f1)};
+                }
+            }
+        emit(t, mm, ll, o, x, in_memory);
+    }
+}
+
+// LDS for the scores of alignment rows
+constexpr long KEPT_FLOATS = 8192, KEPT_FLOATS_ALONE = 24576;
+long kept_queries(const Launch& n, long nq) { return std::min(nq, 16L * n.qt); }
+
+Launch cross_shape(const MzCross& a) {
+    const long grp = a.heads / a.kv_heads, nq = (long)a.tokens * grp, cus = mz_cu_count(), pairs = (long)a.rows * a.kv_heads;
+    const long blocks = ((long)a.positions + BLK - 1) / BLK;
+    auto inverse = [](int d) { return (unsigned)std::min((1ULL << 32) / d, 0xffffffffULL); };
+    Launch n{};
+    n.group = (int)grp;
+    n.by_heads = inverse(a.kv_heads);
+    n.by_group = inverse(n.group);
+    n.waves = 4;
+    n.splits = 1;
+    n.own = !a.align && nq > 16 && pairs * ((nq + 127) / 128) >= cus;
+    if (n.own) {
+        n.tiles = (int)((nq + 127) / 128);
+        return n;
+    }
+    n.qt = nq <= 16 ? 1 : 2;
+    n.tiles = (int)((nq + 16 * n.qt - 1) / (16 * n.qt));
+    const long units = pairs * n.tiles;
+    if (units <= cus && n.qt == 1) n.waves = 8;
+    n.splits = (int)std::max(1L, std::min({cus / units, blocks / 10, 256L}));
+    const long keep = (blocks + n.splits - 1) / n.splits * BLK;
+    n.kept = a.align && keep * kept_queries(n, nq) <= (units * n.splits <= cus ? KEPT_FLOATS_ALONE : KEPT_FLOATS) ? (int)keep : 0;
+    return n;
+}
+static_assert(JOIN_COUNTERS >= 1024, "units that are shared have a counter each: fewer than the CUs");
+
+template <bool ALIGN>
+void launch(hipStream_t s, const MzCross& a, const Launch& n) {
+    const size_t lds = (size_t)n.kept * kept_queries(n, (long)a.tokens * n.group) * 4;
+    const dim3 grid(((long)a.rows * a.kv_heads + 7) / 8 * 8, n.tiles, n.splits);
+    if constexpr (!ALIGN)
+        if (n.own) {
+            hipLaunchKernelGGL((cross_kernel<2, false, 4, true>), grid, dim3(256), 0, s, a, n);
+            return;
+        }
+    if (n.qt == 2) hipLaunchKernelGGL((cross_kernel<2, ALIGN, 4, false>), grid, dim3(256), lds, s, a, n);
+    else if (n.waves == 4) hipLaunchKernelGGL((cross_kernel<1, ALIGN, 4, false>), grid, dim3(256), lds, s, a, n);
+    else hipLaunchKernelGGL((cross_kernel<1, ALIGN, 8, false>), grid, dim3(512), lds, s, a, n);
 }
 
 }  // namespace
 
+// (a launch has fewer than 2^32 threads along x, and 2^16 workgroups along y and z; a block's positions lie within 2^30 bytes)
 bool mz_cross_fits(const MzCross& a) {
     const long nq = (long)a.tokens * (a.heads / a.kv_heads);
-    return (long)a.rows * a.kv_heads < (1L << 23) - 8 && nq <= 16L * 65535;
+    return (long)a.rows * a.kv_heads < (1L << 23) - 8 && nq <= 16L * 65535 && a.k_pos <= 1 << 24 && a.v_pos <= 1 << 24;
 }
 
-size_t mz_cross_work(const MzCross& a) { return 0; }
+size_t mz_cross_work(const MzCross& a) {
+    const Launch n = cross_shape(a);
+    return n.splits > 1 ? ((size_t)a.rows * a.kv_heads * n.tiles * n.splits * 16 * n.qt * STATE + JOIN_COUNTERS) * 4 : 0;
+}
 
 hipError_t mz_cross_launch(hipStream_t s, const MzCross& a) {
-    hipLaunchKernelGGL(simple_kernel, dim3(a.rows * a.kv_heads, a.tokens * (a.heads / a.kv_heads)), dim3(64), 0, s, a);
+    const Launch n = cross_shape(a);
+    a.align ? launch<true>(s, a, n) : launch<false>(s, a, n);
     return hipGetLastError();
 }

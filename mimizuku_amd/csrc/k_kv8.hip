@@ -1,5 +1,6 @@
 // Key/value caches held in 8 bits: writing, reading back, and attention over them (layout and definitions: mz_kv8 in
 // mimizuku.h).
+#include "mz_attn.h"
 #include "mz_common.h"
 #include "mz_kernels.h"
 
@@ -439,20 +440,6 @@ long write_groups(const MzKv8& kv, const MzKv8Io& a, int per) { return 1 + (std:
 // largest keep their share (two fp16 numbers end at 2^-24). The maximum of a state is moved only when a score passes it by more
 // than 8 (in powers of two), so that most blocks need no exchange between lanes and no rescaling.
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, NOTHING = -1e30f;
-
-// maximum / sum over the four lanes of a column (lane ^ 16, ^ 32), in each of them
-__device__ __forceinline__ float column_max(float v) {
-    const unsigned u = __builtin_bit_cast(unsigned, v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return pair32_max(fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])));
-}
-__device__ __forceinline__ float column_sum(float v) {
-    const unsigned u = __builtin_bit_cast(unsigned, v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return pair32_sum(__builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]));
-}
-
 // v p for p = high + low
 __device__ __forceinline__ f32x4 weighted(bf16x8 v, bf16x8 high, bf16x8 low, f32x4 to) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, high, __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, low, to, 0, 0, 0), 0, 0, 0);
@@ -461,10 +448,6 @@ __device__ __forceinline__ f32x4 weighted(bf16x8 v, bf16x8 high, bf16x8 low, f32
 __device__ __forceinline__ float lane_value(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
-
-// (the median of two numbers and infinity is the larger one. A maximum would make each operand quiet first, and so would a
-// median with an infinity that the compiler knows.)
-__device__ __forceinline__ float larger(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
 
 // what a row's queries see: token i positions first .. min(base + (causal ? i : 0), cap) - 1 of its slot
 struct Seen {
@@ -499,25 +482,6 @@ __device__ __forceinline__ Seen seen_of(const MzKv8& kv, const MzKv8Attn& a, int
     return s;
 }
 
-// Alignment indices of the query heads h0 .. h0 + n - 1, by all threads of the workgroup: of heads with one index the
-// first has it. mine: head_slot[threadIdx.x], requested earlier.
-template <int THREADS>
-__device__ __forceinline__ void align_indices(const MzKv8Attn& a, int h0, int n, int mine, int (&index)[64]) {
-    __shared__ int slots[64];
-    const int tid = threadIdx.x;
-    for (int j = tid; j < h0 + n; j += THREADS) {
-        const int s = j == tid ? mine : a.head_slot[j];
-        if (j >= h0) slots[j - h0] = index[j - h0] = s < a.align_heads ? s : -1;
-    }
-    __syncthreads();
-    for (int j = tid; j < h0 + n; j += THREADS) {
-        const int s = j == tid ? mine : a.head_slot[j];
-        for (int k = max(0, j - h0 + 1); k < n; k++)
-            if (slots[k] == s) index[k] = -1;
-    }
-    __syncthreads();
-}
-
 struct Launch {
     int qt, tiles, splits;  // queries of a workgroup / 16, such tiles of a (row, cache head), workgroups that share the blocks
     int waves, own;         // waves of a workgroup; whether each has 16 queries of its own (qt is not used then)
@@ -525,13 +489,6 @@ struct Launch {
     int group;              // query heads of a cache head
     unsigned by_heads, by_group, by_splits;  // for dividing by the cache's heads, group and splits (see divided)
 };
-// x / d for x below 2^31 by r = min(2^32 / d, 2^32 - 1): no more than one too small before the correction (a division by a
-// number not known beforehand takes about twenty dependent instructions)
-__device__ __forceinline__ int divided(int x, int d, unsigned r) {
-    const int q = (int)__umulhi((unsigned)x, r);
-    return q + ((q + 1) * (long)d <= x);
-}
-constexpr int STATE = 66;  // floats of a query's partial state: 64 channels, maximum, sum
 
 // NW waves, which take the blocks in turn, or, with OWN, each 16 QT queries of its own and every block (no alignment rows):
 // widening a block is then the four waves' common work, which meet once a block (measured with P as one fp16
@@ -725,7 +682,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 5 : QT == 1 ? 4 : 2) attn_kerne
 #pragma unroll
         for (int i = 0; i < DEPTH; i++) fetch(head + STEP * i, w[i]);
     if constexpr (ALIGN) {  // (while they are on their way)
-        align_indices<64 * NW>(a, kh * grp, grp, mine, index);
+        align_indices<64 * NW>(a.head_slot, a.align_heads, kh * grp, grp, mine, index);
 #pragma unroll
         for (int t = 0; t < QT; t++) al[t] = align_row(t);
     }

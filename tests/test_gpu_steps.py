@@ -10,7 +10,7 @@ u = 2^-24 in 32 bits and h = 2^-11 in fp16 (half a step each):
   a score's exponent    (64 products and sums + 16 for the scale, the maximum and exp2) u sum |q k| scale = ds
   lse                   ds + (n + 8) u (a sum of n terms, in any order) + 4 u |lse|
   a probability         relative 2 ds + (n + 16) u, and 2^-120 for those at the bottom of the range
-  attention's output    the probabilities' error, 2^-22 and n 2^-31 of the largest for their two fp16 parts, times sum p |v|; h
+  attention's output    the probabilities' error, 2^-20 and n 2^-31 of the largest for their two fp16 parts, times sum p |v|; h
                         for the output's own; 2^-24 for numbers below fp16's normal range
   a drawn token's logp  u |logp| + 2^-40
 """
@@ -273,7 +273,7 @@ def check_cross(q, k, v, got, head_slot=None, **kw):
     err = ds + (n + 8) * U + 4 * U * np.abs(np.where(some, r["lse"], 0))
     bad = ~(np.abs(got["lse"] - np.where(some, r["lse"], 0)) <= err) & some
     assert not bad.any(), (np.argwhere(bad)[:4], got["lse"][bad][:4], r["lse"][bad][:4])
-    rel = (2 * ds + (n + 16) * U + 2.0 ** -22)[..., None]
+    rel = (2 * ds + (n + 16) * U + 2.0 ** -20)[..., None]
     far = np.abs(v.astype(np.float64)).max()
     tol = rel * r["size"] + (n * 2.0 ** -31)[..., None] * far + H * (1 + rel) * np.abs(r["out"]) + 2.0 ** -24
     bad = ~(np.abs(got["out"] - r["out"]) <= tol) & some[..., None]
@@ -435,7 +435,7 @@ def test_cross_layouts(ctx, dev):
 def test_cross_past_32_bits(ctx, dev):
     """Positions and slots whose offsets pass 2^32 bytes."""
     rng = np.random.default_rng(9)
-    pos, heads, far = 70, 2, 1 << 26  # positions 2^27 bytes apart: 8.7 GiB
+    pos, heads, far = 140, 2, 1 << 24  # positions 2^25 bytes apart: 4.4 GiB
     k, v, q = f16(rng, (1, pos, heads, 64)), f16(rng, (1, pos, heads, 64)), f16(rng, (1, 1, heads, 64), 1.5)
     base = ctx.alloc(pos * far * 2 + 4096)
     try:

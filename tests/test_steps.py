@@ -161,6 +161,7 @@ def test_cross_refuses(fn):
                 dict(k=SOME + 8), dict(v=SOME + 4), dict(slot=SOME + 1), dict(count=SOME + 2), dict(first=SOME + 3),
                 dict(len=SOME + 1), dict(lse=SOME + 2), dict(align=SOME + 1), dict(q_head=60), dict(q_row=-8),
                 dict(k_pos=60), dict(k_slot=-64), dict(v_head=4), dict(v_slot=1 << 47), dict(k_pos=1 << 44, positions=100),
+                dict(k_pos=(1 << 24) + 8), dict(v_pos=(1 << 24) + 8),
                 dict(out_row=0), dict(out_head=32), dict(out_token=64, tokens=2, out_row=4096), dict(align=SOME),
                 dict(align=SOME, head_slot=SOME, align_heads=0, align_cols=4),
                 dict(align=SOME, head_slot=SOME, align_heads=2, align_cols=0), dict(out_row=1 << 47),
