@@ -17,9 +17,11 @@
 namespace {
 
 typedef unsigned long long u64;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int BINS = THREADS, BIN_BITS = 10, LIST = THREADS;
+constexpr int MOST_ROUNDS = 30;  // pieces of a thread that have a word of LDS
 
 // a logit as a number in the opposite order, -0 and +0 alike
 __device__ __forceinline__ unsigned order_of(float v) {
@@ -28,27 +30,88 @@ __device__ __forceinline__ unsigned order_of(float v) {
 }
 __device__ __forceinline__ float value_at(unsigned o) { return __builtin_bit_cast(float, o ^ (~(unsigned)((int)o >> 31) & 0x7fffffffu)); }
 
-// exp((x - top) / t) in steps of 2^-shift, 0 for -inf. With s = (x - top) / (t ln 2), n the whole number next to it and f = s - n:
-// n is in the low bits of s + 1.5 * 2^52, 2^f is a polynomial of degree 8 through its values at nine Chebyshev nodes (relative
-// error below 1.1e-12), 2^n goes into its exponent, and the sum with 2^52 has the result, rounded, in its low 52 bits.
+constexpr float LOWEST = -3.40282347e38f;
+
+// exp((x - top) / t) in steps of 2^-shift of finite x. With s = (x - top) / (t ln 2), n the whole number next to it and f = s - n:
+// n + shift is in the low bits of s + (1.5 * 2^52 + shift), 2^f is a polynomial of degree 8 through its values at nine Chebyshev
+// nodes (relative error below 1.1e-12), n goes into its exponent, and the sum with 2^52 has the result, rounded, in its low 52 bits.
+// What is 200 powers of two below the top has weight 0, as has what is next to the top where t is too small for it to count.
 struct Weights {
-    double top, per;  // per: 1 / (t ln 2)
-    double lowest;    // -200 / per: what is further below the top has weight 0
-    int shift;
-    __device__ __forceinline__ u64 operator()(float x) const {
-        const double d = fmax((double)x - top, lowest), s = fma(d, per, 0x1.8p52), f = fma(d, per, 0x1.8p52 - s);
-        double p = 0x1.63d136366db24p-20;
-        p = fma(p, f, 0x1.00dc4a532fb8ep-16);
-        p = fma(p, f, 0x1.4308ac85aa947p-13);
-        p = fma(p, f, 0x1.5d8745a728441p-10);
-        p = fma(p, f, 0x1.3b2ab7181b755p-7);
-        p = fma(p, f, 0x1.c6b08dd6fd234p-5);
-        p = fma(p, f, 0x1.ebfbdff823cedp-3);
-        p = fma(p, f, 0x1.62e42fef84cf0p-1);
-        p = fma(p, f, 1.0);
-        const u64 bits = __builtin_bit_cast(u64, p) + ((u64)(__builtin_bit_cast(u64, s) + shift) << 52);
-        return __builtin_bit_cast(u64, __builtin_bit_cast(double, bits) + 0x1p52) & ((1ULL << 52) - 1);
+    double top, per, magic;
+    float lowest, inf;  // (inf: the median with a number that the compiler does not know is the larger one, in one instruction)
+    double c[8];  // (in registers: as immediate numbers each would take two more instructions)
+    __device__ __forceinline__ Weights(float top_, float t, int shift) {
+        const double gap = (double)top_ - (double)fmaxf(value_at(order_of(top_) + 1), LOWEST);  // to the next number below
+        top = top_;
+        per = 1.4426950408889634 / (double)t;
+        double far = (double)t * (200.0 / 1.4426950408889634);
+        if (far < gap) {
+            per = 200.0 / gap;
+            far = gap;
+        }
+        magic = 0x1.8p52 + shift;
+        lowest = fmaxf((float)(top - far), LOWEST);
+        c[0] = 0x1.63d136366db24p-20;
+        c[1] = 0x1.00dc4a532fb8ep-16;
+        c[2] = 0x1.4308ac85aa947p-13;
+        c[3] = 0x1.5d8745a728441p-10;
+        c[4] = 0x1.3b2ab7181b755p-7;
+        c[5] = 0x1.c6b08dd6fd234p-5;
+        c[6] = 0x1.ebfbdff823cedp-3;
+        c[7] = 0x1.62e42fef84cf0p-1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) asm("" : "+v"(c[i]));
+        inf = INFINITY;
+        asm("" : "+s"(inf));
     }
+    // of N logits side by side: each is a chain of dependent steps. RAW: with the bits above, ABOVE, for sums of whole pieces
+    template <int N, bool RAW>
+    __device__ __forceinline__ void of(const float* x, u64* to) const {
+        double d[N], s[N], f[N], p[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) d[k] = (double)__builtin_amdgcn_fmed3f(x[k], lowest, inf) - top;
+#pragma unroll
+        for (int k = 0; k < N; k++) s[k] = fma(d[k], per, magic);
+#pragma unroll
+        for (int k = 0; k < N; k++) f[k] = fma(d[k], per, magic - s[k]);
+#pragma unroll
+        for (int k = 0; k < N; k++) p[k] = fma(c[0], f[k], c[1]);
+#pragma unroll
+        for (int i = 2; i < 8; i++)
+#pragma unroll
+            for (int k = 0; k < N; k++) p[k] = fma(p[k], f[k], c[i]);
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            u32x2 b = __builtin_bit_cast(u32x2, fma(p[k], f[k], 1.0));
+            b[1] += __builtin_bit_cast(u32x2, s[k])[0] << 20;
+            b = __builtin_bit_cast(u32x2, __builtin_bit_cast(double, b) + 0x1p52);
+            if (!RAW) b[1] &= 0xfffffu;
+            to[k] = __builtin_bit_cast(u64, b);
+        }
+    }
+    __device__ __forceinline__ u64 operator()(float x) const {
+        u64 w;
+        of<1, false>(&x, &w);
+        return w;
+    }
+    template <int V>
+    __device__ __forceinline__ void of_piece(const float (&x)[V], u64 (&w)[V]) const {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) of<4, false>(x + k, w + k);
+    }
+    // the sum of a piece's weights, of -inf too (`plain`)
+    template <int V>
+    __device__ __forceinline__ u64 sum_of_piece(const float (&x)[V]) const {
+        u64 w[V], sum = 0;
+#pragma unroll
+        for (int k = 0; k < V; k += 4) of<4, true>(x + k, w + k);
+#pragma unroll
+        for (int k = 0; k < V; k++) sum += w[k];
+        return sum - V * ABOVE;
+    }
+    static constexpr u64 ABOVE = 0x433ULL << 52;
+    // whether -inf has weight 0: something finite is further below the top than `lowest`
+    __device__ __forceinline__ bool plain() const { return top > (double)LOWEST; }
 };
 
 // ---------------------------------------------------------------- sums over a workgroup
@@ -67,8 +130,13 @@ struct Max {
 };
 template <int CTRL, typename T>
 __device__ __forceinline__ T moved_of(T v) {
-    if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, moved<CTRL>(__builtin_bit_cast(u64, v)));
-    else return __builtin_bit_cast(T, dpp_i<CTRL>(__builtin_bit_cast(int, v)));
+    // (every lane reads another: there is no old value)
+    if constexpr (sizeof(T) == 8) {
+        const u32x2 b = __builtin_bit_cast(u32x2, v);
+        return __builtin_bit_cast(T, u32x2{(unsigned)__builtin_amdgcn_mov_dpp((int)b[0], CTRL, 0xF, 0xF, true),
+                                           (unsigned)__builtin_amdgcn_mov_dpp((int)b[1], CTRL, 0xF, 0xF, true)});
+    } else
+        return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 template <typename T>
 __device__ __forceinline__ T lane_of(T v, int lane) {
@@ -97,17 +165,24 @@ __device__ __forceinline__ T block_all(T v, F f) {
 }
 // the sum up to and with this lane's: within rows of 16 lanes by 1, 2, 4 and 8, then row 0's last into row 1 and row 2's into row
 // 3, then row 1's last into both
-__device__ __forceinline__ u64 wave_running(u64 v) {
-    auto step = [&](auto lo_hi) {
-        v += (u64)(unsigned)lo_hi((int)(v >> 32)) << 32 | (unsigned)lo_hi((int)v);
-    };
-    step([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true); });
-    step([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true); });
-    step([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true); });
-    step([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true); });
-    step([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); });
-    step([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); });
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved_in(u64 v) {
+    const u32x2 b = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(u64, u32x2{(unsigned)__builtin_amdgcn_update_dpp(0, (int)b[0], CTRL, ROWS, 0xF, true),
+                                         (unsigned)__builtin_amdgcn_update_dpp(0, (int)b[1], CTRL, ROWS, 0xF, true)});
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved_in(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, true));
+}
+template <typename T>
+__device__ __forceinline__ T wave_running(T v) {
+    v += moved_in<0x111, 0xF>(v);
+    v += moved_in<0x112, 0xF>(v);
+    v += moved_in<0x114, 0xF>(v);
+    v += moved_in<0x118, 0xF>(v);
+    v += moved_in<0x142, 0xA>(v);
+    return v + moved_in<0x143, 0xC>(v);
 }
 
 // the wave's keys in order, best first
@@ -134,21 +209,25 @@ struct Row {
     const unsigned char* mask;
     int vocab, off, pieces;  // 16-byte pieces of memory; the first begins `off` elements before the row
     int rounds;              // pieces of a thread
+    float* largest;          // of each piece, in LDS (null: too many)
 
-    __device__ __forceinline__ void open(const MzSample& a, long r) {
+    __device__ __forceinline__ void open(const MzSample& a, long r, float* lds) {
         row = (const T*)a.logits + r * a.ld;
         mask = a.mask;
         vocab = a.vocab;
         off = (int)((uintptr_t)row % 16 / sizeof(T));
         pieces = (vocab + off + V - 1) / V;
         rounds = (pieces + THREADS - 1) / THREADS;
+        largest = rounds <= MOST_ROUNDS ? lds + threadIdx.x : nullptr;
     }
-    // where piece p's elements begin, and where they are read: pieces at the row's ends are moved into it
-    __device__ __forceinline__ int begin(int p) const { return p * V - off; }
-    __device__ __forceinline__ int from(int p) const { return max(min(begin(p), vocab - V), 0); }
-    __device__ __forceinline__ int piece(int j) const { return min(j * THREADS + (int)threadIdx.x, pieces); }
+    // where this thread's piece j begins, and where it is read: pieces at the row's ends are moved into it
+    __device__ __forceinline__ int begin(int j) const { return (j * THREADS + (int)threadIdx.x) * V - off; }
+    __device__ __forceinline__ int from(int j) const {
+        const int e = begin(j);
+        return j == 0 || j >= rounds - 1 ? max(min(e, vocab - V), 0) : e;
+    }
     __device__ __forceinline__ Piece load(int j) const {
-        const int e = from(piece(j));
+        const int e = from(j);
         Piece p;
         if (vocab >= V) {
             p.raw = *(const Loaded*)(row + e);
@@ -168,7 +247,7 @@ struct Row {
 #pragma unroll
         for (int k = 0; k < V; k++) y[k] = (float)p.raw[k];
         if (j == 0 || j >= rounds - 1) {
-            const int b = begin(piece(j)), e = from(piece(j));
+            const int b = begin(j), e = from(j);
 #pragma unroll
             for (int k = 0; k < V; k++)
                 if (e + k < b || e + k >= min(b + V, vocab)) y[k] = -INFINITY;
@@ -182,7 +261,7 @@ struct Row {
                 for (int k = 0; k < V; k++) y[k] = p.bits[k / 4] & 0xffu << (k % 4 * 8) ? -INFINITY : y[k];
         }
     }
-    // f(piece, its logits), AHEAD pieces on their way
+    // f(j, its logits), AHEAD pieces on their way
     template <int AHEAD, typename F>
     __device__ __forceinline__ void each_piece(F f) const {
         Piece p[AHEAD];
@@ -198,7 +277,7 @@ struct Row {
                 const Piece now = p[d];
                 p[d] = load(j + AHEAD);
                 logits(j, now, y);
-                f(j * THREADS + (int)threadIdx.x, y);
+                f(j, y);
             }
     }
     // f(x, id) of the tokens, one at a time: little code, for what is hardly ever needed
@@ -210,27 +289,46 @@ struct Row {
             if (x > -INFINITY) f(x, id);
         }
     }
-    // f(x, id) of the tokens not below v
-    template <int AHEAD, typename F>
+    // f(x, id) of the tokens not below v; pieces whose largest is are not read
+    template <typename F>
     __device__ __forceinline__ void each_from(float v, F f) const {
-        each_piece<AHEAD>([&](int p, const float (&y)[V]) {
-            float most = y[0];
-#pragma unroll
-            for (int k = 1; k < V; k++) most = fmaxf(most, y[k]);
-            if (!(most >= v)) return;
-            const int e = from(min(p, pieces));
+        unsigned has = 0;  // this thread's pieces
+        if (largest)
+#pragma unroll 4
+            for (int j = 0; j < rounds; j++) has |= (unsigned)(largest[j * THREADS] >= v) << j;
+        int j = -1;
+        auto next = [&]() {
+            if (!largest) return j + 1;
+            const int i = has ? __ffs(has) - 1 : rounds;
+            has &= has - 1;
+            return i;
+        };
+        j = next();
+        if (j >= rounds) return;
+        Piece p = load(j);
+        do {
+            const Piece now = p;
+            const int at = j;
+            j = next();
+            if (j < rounds) p = load(j);  // on its way while this one is taken
+            float y[V];
+            logits(at, now, y);
+            const int e = from(at);
 #pragma unroll
             for (int k = 0; k < V; k++)
                 if (y[k] >= v && y[k] > -INFINITY) f(y[k], e + k);
-        });
+        } while (j < rounds);
     }
 };
 
 struct Shared {
     u64 sums[BINS];
+    float wave_about[WAVES], about;
+    float wave_best[WAVES];
+    unsigned wave_count[WAVES];
     u64 wave_sum[WAVES];
     u64 before, here;
-    unsigned at, lo, hi;
+    unsigned at, drawn_x;
     int n;
     float lx[LIST];
     int lid[LIST];
@@ -260,8 +358,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
     const long r = blockIdx.x, n = a.at ? (long)*a.at + a.at_add : 0;
     if (n < 0 || n >= a.stride) return;
     const long at = r * a.stride + n;
+    extern __shared__ float largest[];
     Row<T, MASK> row;
-    row.open(a, r);
+    row.open(a, r, largest);
     const float t = a.temperatures ? a.temperatures[r] : a.temperature, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
     const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, u0 = a.u[at];
     const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
@@ -271,19 +370,36 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
         if (a.kept) a.kept[at] = kept;
     };
 
+    float inf = INFINITY;  // (the median with a number that the compiler does not know is the larger one, in one instruction)
+    asm("" : "+s"(inf));
     float best = -INFINITY;  // this thread's largest
     unsigned count = 0;      // tokens
     bool nan = false;
-    row.template each_piece<4>([&](int, auto& y) {
+    row.template each_piece<4>([&](int j, auto& y) {
+        float most = y[0];
+#pragma unroll
+        for (int k = 1; k < row.V; k++) most = __builtin_amdgcn_fmed3f(most, y[k], inf);
 #pragma unroll
         for (int k = 0; k < row.V; k++) {
-            best = fmaxf(best, y[k]);
             count += y[k] > -INFINITY;
             nan |= y[k] != y[k];
         }
+        best = __builtin_amdgcn_fmed3f(best, most, inf);
+        if (row.largest) row.largest[j * THREADS] = most;
     });
-    const float top = block_all(best, Max());
-    count = block_all(count | (nan ? 1u << 31 : 0), [](unsigned x, unsigned y) { return ((x | y) & 1u << 31) | ((x + y) & 0x7fffffff); });
+    {
+        const float m = wave_max(best);
+        unsigned c = row_all(count, Add());
+        c = lane_of(c, 0) + lane_of(c, 16) + lane_of(c, 32) + lane_of(c, 48);
+        const bool any = __ballot(nan);
+        if (lane == 0) {
+            sh.wave_best[tid >> 6] = m;
+            sh.wave_count[tid >> 6] = any ? 1u << 31 : c;
+        }
+    }
+    __syncthreads();
+    const float top = row_all(sh.wave_best[lane & 15], Max());
+    count = row_all(sh.wave_count[lane & 15], [](unsigned x, unsigned y) { return (x | y) >> 31 ? 1u << 31 : x + y; });
     const bool bad = count >> 31 || top == INFINITY || !(t >= 0.f) || t == INFINITY || top_p != top_p || min_p != min_p;
     if (bad || !count) {
         if (tid == 0) answer(-1, bad ? NAN : -INFINITY, 0);
@@ -291,13 +407,12 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
     }
     if (t == 0.f || top_k == 1 || top_p <= 0.f) {  // the first
         unsigned id = ~0u;
-        row.template each_from<4>(top, [&](float, int i) { id = min(id, (unsigned)i); });
+        row.each_from(top, [&](float, int i) { id = min(id, (unsigned)i); });
         id = block_all(id, Min());
         if (tid == 0) answer((int)id, 0.f, 1);
         return;
     }
-    const double per = 1.4426950408889634 / (double)t;
-    const Weights weight = {(double)top, per, -200.0 / per, shift};
+    const Weights weight(top, t, shift);
     const float u = u0 >= 0.f ? fminf(u0, 0x1.fffffep-1f) : 0.f;
     const bool limit_k = top_k > 0 && (unsigned)top_k < count, limit_p = top_p < 1.f, limit_m = min_p > 0.f;
     float low = -INFINITY;  // the lowest logit of weight min_p or more
@@ -306,8 +421,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
         low = (float)l;
         if ((double)low < l) low = value_at(order_of(low) - 1);
     }
-    // intervals of values: 32 to a factor of two of weights, the last one without an end
-    const float per_bin = 32.f * (float)per;
+    // intervals of values, the last one without an end
+    float per_bin = 1.f;
     auto value_bin = [&](float x) { return (int)fminf((top - x) * per_bin, BINS - 1.f); };
 
     // Limits so far: tokens of an order below cut's, or cut's with an id up to last.
@@ -321,24 +436,23 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
     struct Edge {
         float least, tie;
         int last;
-        __device__ __forceinline__ bool has(float x, int id) const { return x >= least && !(x == tie && id > last); }
+        __device__ __forceinline__ bool has(float x, int id) const { return (x >= least) & ((x != tie) | (id <= last)); }
     };
     auto edge_of = [&](float low) {
-        return Edge{cut == ~0u ? low : fmaxf(low, value_at(cut)), cut == ~0u ? NAN : value_at(cut), last};
+        return Edge{fmaxf(cut == ~0u ? low : fmaxf(low, value_at(cut)), LOWEST), cut == ~0u ? NAN : value_at(cut), last};
     };
     u64 total = 0;        // what top_p is a share of
     bool listed = false;  // all tokens that the limits can leave are in the list: this thread's
     int m = 0;            // its length
     float lx = -INFINITY;
     int lid = 0;
-    // tokens not below `from` in intervals `first` to `final` into the list; whether it holds them all
-    auto gather = [&](float from, int first, int final) {
+    // tokens from `from` to `upto` into the list; whether it holds them all
+    auto gather = [&](float from, float upto) {
         __syncthreads();
         if (tid == 0) sh.n = 0;
         __syncthreads();
-        row.template each_from<4>(from, [&](float x, int id) {
-            const int b = value_bin(x);
-            if (b < first || b > final || !inside(x, id)) return;
+        row.each_from(from, [&](float x, int id) {
+            if (x > upto || !inside(x, id)) return;
             const int i = atomicAdd(&sh.n, 1);
             if (i < LIST) {
                 sh.lx[i] = x;
@@ -354,27 +468,29 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
     auto logp_of = [&](float x, u64 sum) { return (float)(((double)x - (double)top) / (double)t - log(ldexp((double)sum, -shift))); };
 
     // The lowest order, of values or of ids, for which the sum of weights (`unit`: of ones) over what `each` has of that order and
-    // below, with `before` in front, is at least need (`above`: more); the sums in front of it and of it. Each pass sums up
-    // intervals; of the one with the place the range is found and divided again.
+    // below, with `before` in front, is at least need (`above`: more); the sums in front of it and of it. The range of what is
+    // left is divided into intervals, until one with the place is a single order.
     u64 before = 0, here = 0;
-    int id_bits = 0;
-    while ((a.vocab - 1) >> id_bits >= BINS) id_bits++;
     auto search = [&](const auto& each, bool by_id, bool unit, double need, bool above) {
+        auto order = [&](float x, int id) { return by_id ? (unsigned)id : order_of(x); };
         unsigned lo = 0, hi = ~0u;
-        int bits = -1;  // (of the first pass: none)
         for (;;) {
-            __syncthreads();
-            sh.sums[tid] = 0;
-            if (tid == 0) {
-                sh.lo = ~0u;
-                sh.hi = 0;
-            }
-            __syncthreads();
-            auto order = [&](float x, int id) { return by_id ? (unsigned)id : order_of(x); };
-            auto bin = [&](float x, int id) { return bits >= 0 ? (int)((order(x, id) - lo) >> bits) : by_id ? id >> id_bits : value_bin(x); };
-            auto ranged = [&](float x, int id) { return order(x, id) >= lo && order(x, id) <= hi; };
+            unsigned l = ~0u, h = 0;
             each([&](float x, int id) {
-                if (ranged(x, id)) atomicAdd(&sh.sums[bin(x, id)], unit ? 1 : weight(x));
+                const unsigned o = order(x, id);
+                if (o >= lo && o <= hi) {
+                    l = min(l, o);
+                    h = max(h, o);
+                }
+            });
+            lo = block_all(l, Min());
+            hi = block_all(h, Max());
+            sh.sums[tid] = 0;
+            __syncthreads();
+            const int bits = max(0, 32 - __clz(hi - lo) - BIN_BITS);
+            each([&](float x, int id) {
+                const unsigned o = order(x, id);
+                if (o >= lo && o <= hi) atomicAdd(&sh.sums[(o - lo) >> bits], unit ? 1 : weight(x));
             });
             __syncthreads();
             u64 mine, all;
@@ -388,24 +504,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
             __syncthreads();
             before = sh.before;
             here = sh.here;
-            const int place = (int)sh.at;
-            if (bits == 0) return lo + place;
-            unsigned l = ~0u, h = 0;
-            each([&](float x, int id) {
-                if (ranged(x, id) && bin(x, id) == place) {
-                    l = min(l, order(x, id));
-                    h = max(h, order(x, id));
-                }
-            });
-            if (l <= h) {
-                atomicMin(&sh.lo, l);
-                atomicMax(&sh.hi, h);
-            }
-            __syncthreads();
-            lo = sh.lo;
-            hi = sh.hi;
-            if (lo == hi) return lo;
-            bits = max(0, 32 - __clz(hi - lo) - BIN_BITS);
+            lo += sh.at << bits;
+            if (bits == 0) return lo;
+            hi = min(hi, lo + (1u << bits) - 1);
         }
     };
 
@@ -417,9 +518,21 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
         bool ready = listed;  // the list has what is needed
         bool known = false;   // what can be needed is not below `from`
         float from = -INFINITY;
-        int place = BINS - 1;
         before = 0;
-        if (unit && top_k <= LIST / 2 && __syncthreads_count(best > -INFINITY) >= top_k) {
+        if (unit) {  // down to the least of the threads' best logits, or of all
+            const bool few = __syncthreads_count(best > -INFINITY) >= top_k;
+            float least = few && best > -INFINITY ? best : top;
+            if (!few)
+                row.template each_piece<2>([&](int j, auto& y) {
+#pragma unroll
+                    for (int k = 0; k < row.V; k++) least = y[k] > -INFINITY ? fminf(least, y[k]) : least;
+                });
+            least = block_all(least, Min());
+            per_bin = least < top ? BINS * 0.9999f / (top - least) : 1.f;
+            known = few && top_k <= LIST / 2;
+        } else  // 32 to a factor of two of weights
+            per_bin = 32.f * (float)weight.per;
+        if (known) {
             // Not below the k-th of the threads' best logits, or the least of those in the intervals up to it.
             const int b = best > -INFINITY ? value_bin(best) : BINS - 1;
             __syncthreads();
@@ -433,56 +546,114 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
             __syncthreads();
             const float edge = block_all(b <= (int)sh.at ? best : INFINITY, Min());
             from = limit_p ? edge : fmaxf(edge, low);
-            known = true;
         }
-        // The list: first, not below `from`; then, with the intervals' sums, the tokens up to the end of the one that has the limit;
-        // then that interval's.
-        u64 front = 0;
-        for (int attempt = known ? 0 : 1; !ready && attempt < 3; attempt++) {
-            if (attempt == 1) {
-                __syncthreads();
-                sh.sums[tid] = 0;
-                __syncthreads();
-                u64 rest = 0;  // of the last interval
-                const Edge edge = edge_of(-INFINITY);
-                row.template each_piece<1>([&](int p, auto& y) {
-                    const int e = row.from(min(p, row.pieces));
-                    u64 w[row.V];
-                    int b[row.V];
+        if (known) ready = listed = gather(from, INFINITY);
+        if (!ready) {
+            // About where: the tokens of each interval, counted, with its middle's weight.
+            __syncthreads();
+            sh.sums[tid] = 0;
+            __syncthreads();
+            unsigned* const counts = (unsigned*)sh.sums;
+            const Edge edge = edge_of(-INFINITY);
+            const bool uncut = cut == ~0u;
+            // (what is in none goes to a word of the thread's own: a branch around each atomic takes longer)
+            auto count_in = [&](auto in) {
+                row.template each_piece<2>([&](int j, auto& y) {
+                    const int e = row.from(j);
 #pragma unroll
                     for (int k = 0; k < row.V; k++) {
-                        w[k] = unit ? y[k] > -INFINITY : weight(y[k]);
-                        if (!edge.has(y[k], e + k)) w[k] = 0;
-                        b[k] = value_bin(y[k]);
-                        if (b[k] == BINS - 1) rest += w[k];
+                        const unsigned b = (unsigned)((top - y[k]) * per_bin);  // (infinity: the largest number)
+                        atomicAdd(&counts[(b < BINS - 1) & in(y[k], e + k) ? b : BINS + tid], 1);
                     }
-#pragma unroll
-                    for (int k = 0; k < row.V; k++)
-                        if (b[k] < BINS - 1) atomicAdd(&sh.sums[b[k]], w[k]);
                 });
-                rest = block_all(rest, Add());
-                if (tid == BINS - 1) sh.sums[tid] = rest;
+            };
+            if (uncut) count_in([](float, int) { return true; });
+            else count_in([&](float x, int id) { return edge.has(x, id); });
+            __syncthreads();
+            // (the last one has the others)
+            const unsigned rest = (uncut ? count : (unsigned)top_k) - block_all(tid < BINS - 1 ? counts[tid] : 0, Add());
+            const unsigned here_n = tid == BINS - 1 ? rest : counts[tid];
+            const float w = unit ? 1.f : __builtin_amdgcn_exp2f((tid + 0.5f) * (-1.f / 32.f));
+            __syncthreads();
+            sh.sums[tid] = here_n;
+            const float sum = wave_running(here_n * w);
+            if (lane == 63) sh.wave_about[tid >> 6] = sum;
+            __syncthreads();
+            float every = 0.f, ahead = 0.f;
+#pragma unroll
+            for (int k = 0; k < WAVES; k++) {
+                if (k == tid >> 6) ahead = every;
+                every += sh.wave_about[k];
+            }
+            const float about = ahead + sum;
+            u64 mine, all;
+            const u64 run = running(sh, mine, all);
+            float goal = unit ? (float)top_k : top_p * every, off = 0.f;
+            // (the next attempt knows what a sum really is)
+            for (int attempt = 0; attempt < 4; attempt++) {
+                const int first = block_all(about + off >= goal ? tid : BINS - 1, Min());
+                // With what is in front of it, and some behind, if that is few enough for one wave; otherwise some intervals around it.
+                if (tid == first) {
+                    sh.before = run - mine;
+                    sh.here = run;
+                }
                 __syncthreads();
-                u64 mine, all;
-                const u64 run = running(sh, mine, all);
+                const bool few = sh.here <= 56;
+                const u64 room = few ? 0 : 128;
+                const int b0 = few ? 0 : block_all(run - mine + room >= sh.before ? tid : BINS - 1, Min());
+                const int b1 = block_all(run <= (few ? 60 : sh.here + room) ? tid : 0, Max());
+                const int end = max(b1, first) + 1;
+                const float high = b0 ? top - b0 / per_bin : INFINITY;
+                from = end >= BINS ? LOWEST : fmaxf(top - end / per_bin, LOWEST);
+                if (tid == b0) sh.about = about - here_n * w;
+                // Exactly: what is in front of these, and all.
+                u64 in_front = 0, sums = 0;
+                if (unit)
+                    row.template each_piece<1>([&](int j, auto& y) {
+                        const int e = row.from(j);
+#pragma unroll
+                        for (int k = 0; k < row.V; k++) in_front += y[k] > high && edge.has(y[k], e + k);
+                    });
+                else if (!b0 && uncut && weight.plain())
+                    row.template each_piece<1>([&](int, auto& y) { sums += weight.sum_of_piece(y); });
+                else if (uncut && weight.plain())
+                    row.template each_piece<1>([&](int, auto& y) {
+                        u64 w[row.V];
+                        weight.of_piece(y, w);
+#pragma unroll
+                        for (int k = 0; k < row.V; k++) {
+                            sums += w[k];
+                            in_front += y[k] > high ? w[k] : 0;
+                        }
+                    });
+                else
+                    row.template each_piece<1>([&](int j, auto& y) {
+                        const int e = row.from(j);
+                        u64 w[row.V];
+                        weight.of_piece(y, w);
+#pragma unroll
+                        for (int k = 0; k < row.V; k++) {
+                            w[k] = edge.has(y[k], e + k) ? w[k] : 0;
+                            sums += w[k];
+                            in_front += y[k] > high ? w[k] : 0;
+                        }
+                    });
+                in_front = block_all(in_front, Add());
                 if (!unit) {
-                    total = all;
+                    total = block_all(sums, Add());
                     need = (double)top_p * (double)total;
                 }
-                if ((double)run >= need && !((double)(run - mine) >= need)) {
-                    sh.before = run - mine;
-                    sh.at = tid;
-                }
+                if (!gather(from, high)) break;
+                const u64 within = block_all(lx > -INFINITY ? unit ? 1 : weight(lx) : 0, Add());
+                ready = (!b0 || (double)in_front < need) && (double)(in_front + within) >= need;
+                listed = ready && !b0;
+                before = ready ? in_front : 0;
+                if (ready) break;
+                const double scale = unit ? 1.0 : ldexp(1.0, -shift);
+                goal = (float)(need * scale);
+                off = (float)((double)in_front * scale) - sh.about;
                 __syncthreads();
-                place = (int)sh.at;
-                front = sh.before;
-                // (not above any of the interval's: a product more than exact ends of it)
-                from = place == BINS - 1 ? -INFINITY : top - (place + 1.01f) * 1.00001f / per_bin;
-                from = from > -INFINITY ? from : -INFINITY;
             }
-            ready = gather(from, attempt == 2 ? place : 0, place);
-            listed = ready && attempt < 2;
-            if (ready && attempt == 2) before = front;
         }
         if (!unit && total == 0) {
             total = block_all(lx > -INFINITY && inside(lx, lid) ? weight(lx) : 0, Add());
@@ -521,14 +692,14 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
             before = 0;
         }
     }
-    if (!limit_k && !limit_p && limit_m) listed = gather(low, 0, BINS - 1);
+    if (!limit_k && !limit_p && limit_m) listed = gather(low, INFINITY);
 
     if (listed && m <= 64) {
         if (tid >= 64) return;
         const Key k = sorted_wave(lx > -INFINITY ? key_of(lx, lid) : 0, lane);
         const float x = value_of(k);
         const u64 w = k ? weight(x) : 0, run = wave_running(w);
-        if (limit_k) total = lane_key(run, min(top_k, 64) - 1);
+        if (limit_k && !total) total = lane_key(run, min(top_k, 64) - 1);
         const bool keep = k && !(limit_k && lane >= top_k) && !(limit_p && lane && (double)(run - w) >= (double)top_p * (double)total) && x >= low;
         const int c = __popcll(__ballot(keep));
         const u64 sum = lane_key(run, c - 1);
@@ -543,6 +714,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
     auto kept = [&](float x, int id) { return x >= low && inside(x, id); };
     u64 sum = 0;
     unsigned c = 0, drawn;
+    float drawn_x;
     if (listed) {
         auto each = [&](auto f) {
             if (lx > -INFINITY && kept(lx, lid)) f(lx, lid);
@@ -554,6 +726,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
         sum = block_all(sum, Add());
         before = 0;
         drawn = search(each, true, false, (double)u * (double)sum, true);
+        drawn_x = (float)row.row[drawn];
     } else {
         // Sums of 16 pieces or more each, then the token among those that the sum with it has, by ids.
         int piece_bits = 4;
@@ -562,19 +735,32 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
         sh.sums[tid] = 0;
         __syncthreads();
         const Edge edge = edge_of(low);
-        row.template each_piece<1>([&](int p, auto& y) {
-            const int e = row.from(min(p, row.pieces));
-            u64 w = 0;
+        const bool every = cut == ~0u && low == -INFINITY && weight.plain();
+        if (every) {
+            row.template each_piece<1>([&](int j, auto& y) {
+                const u64 w = row_all(weight.sum_of_piece(y), Add());
+                if ((tid & 15) == 0) atomicAdd(&sh.sums[(j * THREADS + tid) >> piece_bits], w);
+            });
+            c = tid == 0 ? count : 0;
+        } else {
+            auto sum_up = [&](auto in) {
+                row.template each_piece<1>([&](int j, auto& y) {
+                    const int e = row.from(j);
+                    u64 each[row.V], w = 0;
+                    weight.of_piece(y, each);
 #pragma unroll
-            for (int k = 0; k < row.V; k++) {
-                const u64 v = weight(y[k]);
-                const bool in = edge.has(y[k], e + k);
-                w += in ? v : 0;
-                c += in && y[k] > -INFINITY;
-            }
-            w = row_all(w, Add());
-            if ((tid & 15) == 0) atomicAdd(&sh.sums[p >> piece_bits], w);
-        });
+                    for (int k = 0; k < row.V; k++) {
+                        const bool has = in(y[k], e + k);
+                        w += has ? each[k] : 0;
+                        c += has;
+                    }
+                    w = row_all(w, Add());
+                    if ((tid & 15) == 0) atomicAdd(&sh.sums[(j * THREADS + tid) >> piece_bits], w);
+                });
+            };
+            if (edge.last >= a.vocab || cut == ~0u) sum_up([&](float x, int) { return x >= edge.least; });
+            else sum_up([&](float x, int id) { return edge.has(x, id); });
+        }
         __syncthreads();
         u64 mine;
         const u64 run = running(sh, mine, sum);
@@ -591,21 +777,25 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
         for (int p0 = 0; ; p0 += THREADS / row.V) {
             __syncthreads();
             sh.sums[tid] = 0;
-            const int p = first + p0 + tid / row.V, id = row.begin(p) + tid % row.V;
+            const int id = (first + p0 + tid / row.V) * row.V - row.off + tid % row.V;
             float x = -INFINITY;
             if (p0 + tid / row.V < pieces && id >= 0 && id < row.vocab && !(MASK && row.mask[id])) x = (float)row.row[id];
             sh.sums[tid] = edge.has(x, id) ? weight(x) : 0;
             __syncthreads();
             u64 mine, all;
             const u64 run = running(sh, mine, all) + before;
-            if ((double)run > need && !((double)(run - mine) > need)) sh.n = id;
+            if ((double)run > need && !((double)(run - mine) > need)) {
+                sh.n = id;
+                sh.drawn_x = __builtin_bit_cast(unsigned, x);
+            }
             before += all;
             if (__syncthreads_or((double)run > need) || p0 + THREADS / row.V >= pieces) break;
         }
         drawn = (unsigned)sh.n;
+        drawn_x = __builtin_bit_cast(float, sh.drawn_x);
     }
     c = block_all(c, Add());
-    if (tid == 0) answer((int)drawn, logp_of((float)row.row[drawn], sum), (int)c);
+    if (tid == 0) answer((int)drawn, logp_of(drawn_x, sum), (int)c);
 }
 
 // weights are multiples of 2^-shift: a row's sum stays below 2^62, and a weight has at most 52 bits
@@ -617,9 +807,12 @@ int shift_of(int vocab) {
 
 template <typename T>
 void launch(hipStream_t s, const MzSample& p) {
+    constexpr int V = 16 / sizeof(T);
     const dim3 grid(p.rows), block(THREADS);
-    if (p.mask) hipLaunchKernelGGL((sample_kernel<T, true>), grid, block, 0, s, p, shift_of(p.vocab));
-    else hipLaunchKernelGGL((sample_kernel<T, false>), grid, block, 0, s, p, shift_of(p.vocab));
+    const long rounds = (((long)p.vocab + 2 * V - 2) / V + THREADS - 1) / THREADS;
+    const size_t lds = rounds <= MOST_ROUNDS ? rounds * THREADS * 4 : 0;
+    if (p.mask) hipLaunchKernelGGL((sample_kernel<T, true>), grid, block, lds, s, p, shift_of(p.vocab));
+    else hipLaunchKernelGGL((sample_kernel<T, false>), grid, block, lds, s, p, shift_of(p.vocab));
 }
 
 }  // namespace
