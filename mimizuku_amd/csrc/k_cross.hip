@@ -59,10 +59,11 @@ __device__ __forceinline__ Seen seen_of(const MzCross& a, int r) {
 
 struct Launch {
     int qt, tiles, splits;  // queries of a workgroup / 16, such tiles of a (row, kv head), workgroups that share the blocks
-    int waves, own;         // waves of a workgroup; whether each has 32 queries of its own (qt is not used then)
+    int waves, own;         // waves of a workgroup; whether each has 16 qt queries of its own
+    int per;                // most blocks of a share
     int kept;               // alignment rows: scores that a workgroup keeps in LDS for each query, 0: in their rows
     int group;              // query heads of a kv head
-    unsigned by_heads, by_group, by_splits;  // for dividing by kv_heads, group and splits (see divided)
+    unsigned by_heads, by_group;  // for dividing by kv_heads and group (see divided)
 };
 
 // The bytes of `n` positions `step` bytes apart, as far as a buffer descriptor reaches: what lies behind reads as zeros. (A block's
@@ -90,14 +91,28 @@ __device__ __forceinline__ void by_channels(const u32x2 (&v)[8], f16x8 (&to)[4])
     }
 }
 
+// x less the fp16 number in the low or the high half of h, in one instruction (the compiler takes a conversion and a subtraction)
+__device__ __forceinline__ float less_low(float x, unsigned h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float less_high(float x, unsigned h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+
 template <int QT>
 struct State {
     float m[QT], l[QT];
     f32x4 acc[QT][4];  // result u of lane (c, g) holds channels 16 g + 4 e + u of query c
 };
 
+// NW waves, which take the blocks in turn, or, with OWN, four times 16 QT queries of their own and every block, or, eight of them,
+// two such fours that have half of the blocks each (no alignment rows).
 template <int QT, bool ALIGN, int NW, bool OWN>
-__global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kernel(MzCross a, Launch n) {
+__global__ void __launch_bounds__(64 * NW, OWN ? (NW == 8 && QT == 1 ? 4 : 2) : QT == 1 ? 4 : 2) cross_kernel(MzCross a, Launch n) {
     static_assert(!(OWN && ALIGN));
     __shared__ float red[OWN ? 1 : NW][16][68], ms[NW][16], ls[NW][16];
     __shared__ float lse2s[16];
@@ -108,15 +123,17 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
     const int tile = blockIdx.y, split = blockIdx.z, grp = n.group;
     const int r = divided(pair, a.kv_heads, n.by_heads), kh = pair - r * a.kv_heads;
     const Seen s = seen_of(a, r);
-    constexpr int SHARE = OWN ? NW : 1;
+    constexpr int SHARE = OWN ? 4 : 1;
     const int nq = a.tokens * grp, w0 = tile * 16 * QT * SHARE;
-    const int q0 = OWN ? w0 + 16 * QT * wave : w0;  // this wave's first query
+    const int q0 = OWN ? w0 + 16 * QT * (wave & 3) : w0;  // this wave's first query
     auto token_of = [&](int x) { return divided(x, grp, n.by_group); };
     if ((int)blockIdx.x >= pairs || token_of(w0) >= s.count) return;  // none of its tokens is there
     const int nb = (s.end - s.first + BLK - 1) / BLK;
-    // (splits is at most 256, nb below 2^26: products below 2^31 where splits is above 1 only if nb is below 2^23)
-    const int b0 = OWN || n.splits == 1 ? 0 : (int)((long)nb * split / n.splits);
-    const int b1 = OWN || n.splits == 1 ? nb : (int)((long)nb * (split + 1) / n.splits);
+    // (shorter rows are shared by fewer)
+    const int splits = OWN || n.splits == 1 ? 1 : min(n.splits, max(1, (nb + n.per - 1) / n.per));
+    if (!OWN && split >= splits) return;
+    const int b0 = splits == 1 ? 0 : (int)((long)nb * split / splits);
+    const int b1 = splits == 1 ? nb : (int)((long)nb * (split + 1) / splits);
 
     const f16* kbase = a.k + s.slot * a.k_slot + kh * a.k_head + s.first * a.k_pos;
     const f16* vbase = a.v + s.slot * a.v_slot + kh * a.v_head + s.first * a.v_pos;
@@ -135,17 +152,16 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
     for (int t = 0; t < QT; t++) {
         const int x = q0 + 16 * t + c, i = token_of(x), h = kh * grp + x - i * grp;
         const bool on = x < nq && i < s.count;
-        const f16* q = a.q + r * a.q_row + (on ? i * a.q_token + h * a.q_head : 0) + 8 * g;
+        const f16* q = a.q + r * a.q_row + (on ? i * a.q_token + h * a.q_head : 0) + 16 * g;
         qf[t][0] = on ? ld8(q) : f16x8{};
-        qf[t][1] = on ? ld8(q + 32) : f16x8{};
+        qf[t][1] = on ? ld8(q + 8) : f16x8{};
         al[t] = nullptr;
     }
 
     // Blocks past the last read as zeros, without a memory access: the loads need no branches, around which the compiler would
     // wait for all that is on its way.
     const unsigned kstep = (unsigned)(a.k_pos * 2), vstep = (unsigned)(a.v_pos * 2);
-    const unsigned kat = (8 * (c >> 2) + (c & 3)) * kstep + 16 * g, vat = 8 * g * vstep + 8 * c;
-    constexpr int POLICY = QT == 1 && !OWN ? 2 : 0;  // nontemporal where no other workgroup reads the same
+    const unsigned kat = (8 * (c >> 2) + (c & 3)) * kstep + 32 * g, vat = 8 * g * vstep + 8 * c;
     auto fetch = [&](int b, Raw& w) {
         const int left = b < b1 ? there - b * BLK : 0;
         const auto rk = positions_at(kbase + (long)b * BLK * a.k_pos, kstep, left);
@@ -153,9 +169,9 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int z = 0; z < 2; z++) w.k[j][z] = __builtin_amdgcn_raw_buffer_load_b128(rk, kat + 4 * j * kstep + 64 * z, 0, POLICY);
+            for (int z = 0; z < 2; z++) w.k[j][z] = __builtin_amdgcn_raw_buffer_load_b128(rk, kat + 4 * j * kstep + 16 * z, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 8; e++) w.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, vat + e * vstep, 0, POLICY);
+        for (int e = 0; e < 8; e++) w.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, vat + e * vstep, 0, 0);
     };
 
     State<QT> st;
@@ -177,10 +193,12 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
             f32x4 d[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) d[j] = mfma16(kf[j][1], qf[t][1], mfma16(kf[j][0], qf[t][0], f32x4{}));
-            if (!whole)
+            if (!whole) {
+                asm volatile("");  // (a branch: selections would be made for every block)
 #pragma unroll
                 for (int e = 0; e < 8; e++)
                     if (p0 + e >= there) d[e >> 2][e & 3] = -INFINITY;
+            }
             if (ALIGN && al[t] != nullptr) {
                 const f32x4 x[2] = {d[0] * scale2, d[1] * scale2};
                 if (n.kept) {
@@ -191,7 +209,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
                     for (int e = 0; e < 8; e++)
                         if (p0 + e < there && s.first + p0 + e < a.align_cols) {
                             float* o = al[t] + s.first + p0 + e;
-                            if (n.splits > 1) shared_store(o, x[e >> 2][e & 3]);
+                            if (splits > 1) shared_store(o, x[e >> 2][e & 3]);
                             else *o = x[e >> 2][e & 3];
                         }
                 }
@@ -213,9 +231,8 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
             u32x4 high, rest;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const auto h = __builtin_amdgcn_cvt_pkrtz(x[2 * e], x[2 * e + 1]);
-                high[e] = __builtin_bit_cast(unsigned, h);
-                rest[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(x[2 * e] - (float)h[0], x[2 * e + 1] - (float)h[1]));
+                high[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(x[2 * e], x[2 * e + 1]));
+                rest[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(less_low(x[2 * e], high[e]), less_high(x[2 * e + 1], high[e])));
             }
             const f16x8 p = __builtin_bit_cast(f16x8, high), q = __builtin_bit_cast(f16x8, rest);
 #pragma unroll
@@ -223,56 +240,93 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
         }
     };
     if constexpr (OWN) {
-        // Each wave loads a quarter of a block, the keys' two tiles or half of the values' positions, and puts it as operands where
-        // all find it, a block ahead; what is behind the last block is that one again.
-        __shared__ u32x4 pieces[2][8][64];
-        u32x4 raw[2];
-        u32x2 rv[8];
-        const bool values = wave >= 2;
-        auto take = [&](int i) {
-            const int b = min(i, nb - 1), left = there - b * BLK;
+        // Each wave loads a quarter of a block, the keys' two tiles or half of each eight positions' values, and puts it as operands
+        // where all find it, a block ahead; AHEAD more are on their way. What is behind the last block is that one again.
+        constexpr int AHEAD = 2, FOURS = NW / 4;
+        __shared__ u32x4 all_pieces[FOURS][2][8][64];
+        const int four = wave >> 2, w4 = wave & 3;
+        auto& pieces = all_pieces[four];
+        // this four's blocks, and the most that one has
+        const int from = four * ((nb + 1) / 2), to = FOURS == 1 || four ? nb : (nb + 1) / 2, steps = FOURS == 1 ? nb : (nb + 1) / 2;
+        u32x4 raw[AHEAD][2];
+        const bool values = w4 >= 2;
+        auto take = [&](int i, u32x4 (&x)[2]) {
+            const int b = min(from + i, nb - 1), left = there - b * BLK;
             if (!values) {
                 const auto rk = positions_at(kbase + (long)b * BLK * a.k_pos, kstep, left);
 #pragma unroll
-                for (int z = 0; z < 2; z++) raw[z] = __builtin_amdgcn_raw_buffer_load_b128(rk, kat + 4 * wave * kstep + 64 * z, 0, 0);
+                for (int z = 0; z < 2; z++) x[z] = __builtin_amdgcn_raw_buffer_load_b128(rk, kat + 4 * w4 * kstep + 16 * z, 0, 0);
             } else {
-                const auto r2 = positions_at(vbase + (long)b * BLK * a.v_pos, vstep, left);
+                const auto rv = positions_at(vbase + (long)b * BLK * a.v_pos, vstep, left);
 #pragma unroll
-                for (int e = 0; e < 8; e++) rv[e][0] = __builtin_amdgcn_raw_buffer_load_b32(r2, vat + 4 * (wave - 2) + e * vstep, 0, 0);
-            }
-        };
-        auto put = [&](int i) {
-            u32x4* o = &pieces[i & 1][2 * wave][lane];
-            if (!values) {
-                o[0] = raw[0];
-                o[64] = raw[1];
-            } else {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const unsigned sel = u ? 0x07060302u : 0x05040100u;
-                    u32x4 x;
-#pragma unroll
-                    for (int p = 0; p < 4; p++) x[p] = __builtin_amdgcn_perm(rv[2 * p + 1][0], rv[2 * p][0], sel);
-                    o[64 * u] = x;
+                for (int e = 0; e < 4; e++) {
+                    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rv, vat + (4 * (w4 - 2) + e) * vstep, 0, 0);
+                    x[e >> 1][2 * (e & 1)] = v[0];
+                    x[e >> 1][2 * (e & 1) + 1] = v[1];
                 }
             }
+        };
+        auto put = [&](int i, const u32x4 (&y)[2]) {
+            if (!values) {
+                u32x4* o = &pieces[i & 1][2 * w4][lane];
+                o[0] = y[0];
+                o[64] = y[1];
+            } else
+#pragma unroll
+                for (int u = 0; u < 4; u++) {  // channel 4 i + u of positions 4 (w4 - 2) .. + 3 of the lane's eight
+                    const unsigned sel = u & 1 ? 0x07060302u : 0x05040100u;
+                    u32x2 x;
+#pragma unroll
+                    for (int p = 0; p < 2; p++) x[p] = __builtin_amdgcn_perm(y[p][2 + (u >> 1)], y[p][u >> 1], sel);
+                    ((u32x2*)&pieces[i & 1][4 + u][lane])[w4 - 2] = x;
+                }
         };
         if (nb > 0) {
-            take(0);
-            put(0);
-            take(1);
-            __syncthreads();
-            for (int i = 0; i < nb; i++) {
-                put(i + 1);
-                take(i + 2);
-                f16x8 kf[2][2], vf[4];
+            take(0, raw[0]);
+            put(0, raw[0]);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    kf[k >> 1][k & 1] = __builtin_bit_cast(f16x8, pieces[i & 1][k][lane]);
-                    vf[k] = __builtin_bit_cast(f16x8, pieces[i & 1][4 + k][lane]);
+            for (int d = 0; d < AHEAD; d++) take(1 + d, raw[d]);
+            __syncthreads();
+            for (int i0 = 0; i0 < steps; i0 += AHEAD)
+#pragma unroll
+                for (int d = 0; d < AHEAD; d++) {
+                    const int i = i0 + d;
+                    if (i >= steps) break;
+                    put(i + 1, raw[d]);
+                    take(i + 1 + AHEAD, raw[d]);
+                    f16x8 kf[2][2], vf[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        kf[k >> 1][k & 1] = __builtin_bit_cast(f16x8, pieces[i & 1][k][lane]);
+                        vf[k] = __builtin_bit_cast(f16x8, pieces[i & 1][4 + k][lane]);
+                    }
+                    if (FOURS == 1 || from + i < to) products(from + i, kf, vf);
+                    lds_barrier();
                 }
-                products(i, kf, vf);
-                lds_barrier();
+        }
+        if constexpr (FOURS == 2) {  // the second four's states to the first
+            float* const parts = (float*)all_pieces;  // [4 QT][18][64 lanes]
+            static_assert(4 * QT * 18 * 64 * 4 <= sizeof(all_pieces));
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                float* o = parts + (w4 * QT + t) * 18 * 64 + lane;
+                if (four) {
+                    o[0] = st.m[t];
+                    o[64] = st.l[t];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[(2 + e) * 64] = st.acc[t][e >> 2][e & 3];
+                }
+            }
+            __syncthreads();
+            if (four) return;
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                const float* o = parts + (w4 * QT + t) * 18 * 64 + lane;
+                const float m1 = o[0], mn = fmaxf(st.m[t], m1), f0 = __builtin_amdgcn_exp2f(st.m[t] - mn), f1 = __builtin_amdgcn_exp2f(m1 - mn);
+                st.m[t] = mn;
+                st.l[t] = fmaf(st.l[t], f0, o[64] * f1);
+#pragma unroll
+                for (int e = 0; e < 16; e++) st.acc[t][e >> 2][e & 3] = fmaf(st.acc[t][e >> 2][e & 3], f0, o[(2 + e) * 64] * f1);
             }
         }
 #pragma unroll
@@ -414,7 +468,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = fmaf(f, y[e], o[e]);
         }
-        if (n.splits == 1) {
+        if (splits == 1) {
             Few x;
             if (n.kept) {
                 few_scores(t, ALIGN ? rows(t) : 0, x, in_lds);
@@ -429,7 +483,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
             shared_store(w + d4 + 2, o[2], o[3]);
             if (d4 == 0) shared_store(w + 64, mm, ll);
         }
-        if (ALIGN && n.splits > 1 && n.kept)  // the share's scores to where the last workgroup finds them
+        if (ALIGN && splits > 1 && n.kept)  // the share's scores to where the last workgroup finds them
             for (unsigned has = rows(t); has; has &= has - 1) {
                 const int k = __ffs(has) - 1;
                 float* const row = row_of_query(t, k);
@@ -438,7 +492,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
             }
         if (t + 1 < QT) __syncthreads();
     }
-    if (n.splits == 1 || !last_of((unsigned*)a.work + (long)pair * n.tiles + tile, n.splits)) return;
+    if (splits == 1 || !last_of((unsigned*)a.work + (long)pair * n.tiles + tile, splits)) return;
     // the last of the workgroups that share these queries joins their states
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -447,18 +501,18 @@ __global__ void __launch_bounds__(64 * NW, OWN ? 2 : QT == 1 ? 4 : 2) cross_kern
         Few x;
         few_scores(t, ALIGN ? rows(t) : 0, x, in_memory);  // (they come with the states)
         if (mine256 && q0 + 16 * t + col < nq)
-            for (int k0 = 0; k0 < n.splits; k0 += 4) {
+            for (int k0 = 0; k0 < splits; k0 += 4) {
                 float2 y[4][3];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const float* w = states + (min(k0 + k, n.splits - 1) * (16 * QT) + 16 * t + col) * STATE;
+                    const float* w = states + (min(k0 + k, splits - 1) * (16 * QT) + 16 * t + col) * STATE;
                     y[k][0] = shared_load2(w + d4);
                     y[k][1] = shared_load2(w + d4 + 2);
                     y[k][2] = shared_load2(w + 64);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    if (k0 + k >= n.splits) continue;
+                    if (k0 + k >= splits) continue;
                     const float mn = fmaxf(mm, y[k][2].x), f0 = __builtin_amdgcn_exp2f(mm - mn), f1 = __builtin_amdgcn_exp2f(y[k][2].x - mn);
                     mm = mn;
                     ll = fmaf(ll, f0, y[k][2].y * f1);
@@ -484,9 +538,12 @@ Launch cross_shape(const MzCross& a) {
     n.by_group = inverse(n.group);
     n.waves = 4;
     n.splits = 1;
-    n.own = !a.align && nq > 16 && pairs * ((nq + 127) / 128) >= cus;
+    const long groups = pairs * ((nq + 63) / 64);  // of 64 queries
+    n.own = !a.align && nq > 16 && groups >= cus;
     if (n.own) {
-        n.tiles = (int)((nq + 127) / 128);
+        n.qt = groups >= 5 * cus ? 2 : 1;
+        n.waves = groups < 2 * cus ? 8 : 4;
+        n.tiles = (int)((nq + 64 * n.qt - 1) / (64 * n.qt));
         return n;
     }
     n.qt = nq <= 16 ? 1 : 2;
@@ -494,7 +551,8 @@ Launch cross_shape(const MzCross& a) {
     const long units = pairs * n.tiles;
     if (units <= cus && n.qt == 1) n.waves = 8;
     n.splits = (int)std::max(1L, std::min({cus / units, blocks / 10, 256L}));
-    const long keep = (blocks + n.splits - 1) / n.splits * BLK;
+    n.per = (int)((blocks + n.splits - 1) / n.splits);
+    const long keep = (long)n.per * BLK;
     n.kept = a.align && keep * kept_queries(n, nq) <= (units * n.splits <= cus ? KEPT_FLOATS_ALONE : KEPT_FLOATS) ? (int)keep : 0;
     return n;
 }
@@ -506,7 +564,9 @@ void launch(hipStream_t s, const MzCross& a, const Launch& n) {
     const dim3 grid(((long)a.rows * a.kv_heads + 7) / 8 * 8, n.tiles, n.splits);
     if constexpr (!ALIGN)
         if (n.own) {
-            hipLaunchKernelGGL((cross_kernel<2, false, 4, true>), grid, dim3(256), 0, s, a, n);
+            if (n.qt == 2) hipLaunchKernelGGL((cross_kernel<2, false, 4, true>), grid, dim3(256), 0, s, a, n);
+            else if (n.waves == 4) hipLaunchKernelGGL((cross_kernel<1, false, 4, true>), grid, dim3(256), 0, s, a, n);
+            else hipLaunchKernelGGL((cross_kernel<1, false, 8, true>), grid, dim3(512), 0, s, a, n);
             return;
         }
     if (n.qt == 2) hipLaunchKernelGGL((cross_kernel<2, ALIGN, 4, false>), grid, dim3(256), lds, s, a, n);
