@@ -120,14 +120,37 @@ __device__ __forceinline__ Scales<G> scales_at(const f16* p) {
     else return Scales<1>{*p};
 }
 
-__device__ __forceinline__ void finish(const MzW4Linear& a, int m, int n, float y) {
-    if (a.bias) y += (float)a.bias[n];
+__device__ __forceinline__ float bias_of(const MzW4Linear& a, long n) { return a.bias ? (float)a.bias[n] : 0.f; }
+
+// the results of row of weights n for rows m .. m + N - 1 of x, those that there are
+template <int N, typename Y>
+__device__ __forceinline__ void finish(const MzW4Linear& a, int m, long n, float bias, Y y) {
     const long o = m * a.ldo + n;
     switch (a.epilogue) {
-        case 0: ((f16*)a.out)[o] = (f16)y; break;
-        case 1: ((f16*)a.out)[o] = (f16)gelu_erf_h(y); break;
-        case 2: ((float*)a.out)[o] += y; break;
-        default: ((float*)a.out)[o] = y;
+        case 0:
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (m + e < a.m) ((f16*)a.out)[o + e * a.ldo] = (f16)(y(e) + bias);
+            break;
+        case 1:
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (m + e < a.m) ((f16*)a.out)[o + e * a.ldo] = (f16)gelu_erf_h(y(e) + bias);
+            break;
+        case 2: {
+            float* out = (float*)a.out + o;
+            float old[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) old[e] = out[m + e < a.m ? e * a.ldo : 0];
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (m + e < a.m) out[e * a.ldo] = old[e] + (y(e) + bias);
+            break;
+        }
+        default:
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (m + e < a.m) ((float*)a.out)[o + e * a.ldo] = y(e) + bias;
     }
 }
 
@@ -151,6 +174,11 @@ __device__ __forceinline__ void entry_product(u32x4 q, Scales<G> scale, X x, f32
 #pragma unroll
             for (int e = 0; e < 4; e++) sum[t][e] = fmaf(part[t][e], d, sum[t][e]);
     }
+}
+
+// 16 bytes of each lane straight into LDS, lane after lane from `to` on
+__device__ __forceinline__ void to_lds(const f16* from, u32x4* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
 // Few rows of weights: a workgroup takes 16 of them, its waves the entries in turn, x from memory; their sums meet in LDS.
@@ -186,7 +214,7 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW
         const int at = (4 * (m >> 4) + (m & 3)) * LD + 16 * (m >> 2 & 3) + n;
         float y = 0.f;
         for (int k = 0; k < waves; k++) y += red[k * 4 * MT * LD + at];
-        if (m0 + m < a.m && t * 16 + n < w.n) finish(a, m0 + m, (int)(t * 16 + n), y);
+        if (m0 + m < a.m && t * 16 + n < w.n) finish<1>(a, m0 + m, t * 16 + n, bias_of(a, t * 16 + n), [&](int) { return y; });
     }
 }
 
@@ -195,7 +223,7 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW
 template <int MT, int G>
 __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
     extern __shared__ u32x4 xs[];  // [chunk][s][MT][64]
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / 64;
     const int i = lane & 15, j = lane >> 4, chunks = w.k / 128, m0 = blockIdx.y * 16 * MT, tiles = (w.n + 15) / 16;
     const int t = blockIdx.x * waves + wave, tt = min(t, tiles - 1);
@@ -229,33 +257,33 @@ __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
         }
     const int n = t * 16 + i;
     if (t >= tiles || n >= w.n) return;
+    const float bias = bias_of(a, n);
 #pragma unroll
-    for (int u = 0; u < MT; u++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int m = m0 + 16 * u + 4 * j + e;
-            if (m < a.m) finish(a, m, n, sum[u][e]);
-        }
+    for (int u = 0; u < MT; u++) {
+        const int m = m0 + 16 * u + 4 * j;
+        if (m < a.m) finish<4>(a, m, n, bias, [&](int e) { return sum[u][e]; });
+    }
 }
 
-// Many rows of x: tiles of 32 MT rows of x x 32 NT of weights, four waves of 16 MT x 16 NT. 128 columns at a time: those of x go
-// straight into LDS, in two buffers, the weights' codes into registers.
-template <int MT, int NT, int G>
-__global__ void __launch_bounds__(256, 2) tile_kernel(MzW4 w, MzW4Linear a) {
-    extern __shared__ u32x4 xs[];  // [2][32 MT rows][16 pieces of 8 columns, piece p of row r at p ^ r % 16]
-    constexpr int ROWS = 32 * MT;
+// Many rows of x: a workgroup takes 16 MT WM rows of x times 16 NT WN of weights, WM x WN waves. 128 columns at a time: those of x
+// go straight into LDS, in two buffers, the weights' codes into registers.
+template <int MT, int NT, int WM, int WN, int G>
+__global__ void __launch_bounds__(64 * WM * WN, 2) tile_kernel(MzW4 w, MzW4Linear a) {
+    extern __shared__ u32x4 xs[];  // [2][rows][16 pieces of 8 columns, piece p of row r at p ^ r % 16]
+    constexpr int ROWS = 16 * MT * WM, PER = ROWS / (4 * WM * WN);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, j = lane >> 4, chunks = w.k / 128, tiles = (w.n + 15) / 16;
-    const int m0 = blockIdx.y * ROWS, wm = (wave & 1) * 16 * MT, t0 = blockIdx.x * 2 * NT + (wave >> 1) * NT;
-    // row r of the tile is loaded by lanes 16 (r % 4) .. + 15 of wave r / 4 % 4, piece by piece
+    const int m0 = blockIdx.y * ROWS, wm = wave % WM * 16 * MT, t0 = blockIdx.x * WN * NT + wave / WM * NT;
+    // a wave loads four rows at a time, 16 lanes a row
+    const f16* from[PER];
+#pragma unroll
+    for (int z = 0; z < PER; z++) {
+        const int r = 4 * (z * WM * WN + wave) + j;
+        from[z] = a.x + min(m0 + r, a.m - 1) * a.ldx + 8 * (i ^ (r & 15));
+    }
     auto load_x = [&](int c) {
 #pragma unroll
-        for (int z = 0; z < ROWS / 16; z++) {
-            const int r = 16 * z + 4 * wave + j, p = i ^ (r & 15);
-            const f16* from = a.x + min(m0 + r, a.m - 1) * a.ldx + c * 128 + 8 * p;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                             (__attribute__((address_space(3))) void*)(xs + (c & 1) * ROWS * 16 + (16 * z + 4 * wave) * 16), 16, 0, 0);
-        }
+        for (int z = 0; z < PER; z++) to_lds(from[z] + c * 128, xs + (c & 1) * ROWS * 16 + 64 * (z * WM * WN + wave));
     };
     u32x4 q[NT];
     Scales<G> scale[NT];
@@ -307,13 +335,12 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(MzW4 w, MzW4Linear a) {
     for (int v = 0; v < NT; v++) {
         const int n = (t0 + v) * 16 + i;
         if (n >= w.n) continue;
+        const float bias = bias_of(a, n);
 #pragma unroll
-        for (int u = 0; u < MT; u++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int m = m0 + wm + 16 * u + 4 * j + e;
-                if (m < a.m) finish(a, m, n, sum[u][v][e]);
-            }
+        for (int u = 0; u < MT; u++) {
+            const int m = m0 + wm + 16 * u + 4 * j;
+            if (m < a.m) finish<4>(a, m, n, bias, [&](int e) { return sum[u][v][e]; });
+        }
     }
 }
 
@@ -322,26 +349,36 @@ int blocks(long x, long per) { return (int)((x + per - 1) / per); }
 template <int G>
 void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
     const int tiles = blocks(w.n, 16), chunks = w.k / 128, cus = mz_cu_count();
-    if (a.m > 64 && (long)blocks(a.m, 128) * blocks(w.n, 128) >= cus) {
-        hipLaunchKernelGGL((tile_kernel<4, 4, G>), dim3(blocks(w.n, 128), blocks(a.m, 128)), dim3(256), 2 * 128 * 256, s, w, a);
-        return;
-    }
     if (a.m > 64 && (long)blocks(a.m, 64) * blocks(w.n, 64) >= cus / 2) {
-        hipLaunchKernelGGL((tile_kernel<2, 2, G>), dim3(blocks(w.n, 64), blocks(a.m, 64)), dim3(256), 2 * 64 * 256, s, w, a);
+        // eight waves a CU: the width whose last round of workgroups leaves the least idle (64: several workgroups a CU)
+        int best = 64;
+        double least = 1.15 * blocks(a.m, 64) * blocks(w.n, 64) * 64 * 64 / cus + 64 * 64;
+        for (int bn : {320, 256, 192, 128}) {
+            const double cost = (double)blocks((long)blocks(a.m, 128) * blocks(w.n, bn), cus) * 128 * (bn + 16);
+            if (cost < least) least = cost, best = bn;
+        }
+        const dim3 grid(blocks(w.n, best), blocks(a.m, best == 64 ? 64 : 128));
+        if (best == 320) hipLaunchKernelGGL((tile_kernel<4, 5, 2, 4, G>), grid, dim3(512), 2 * 128 * 256, s, w, a);
+        else if (best == 256) hipLaunchKernelGGL((tile_kernel<4, 4, 2, 4, G>), grid, dim3(512), 2 * 128 * 256, s, w, a);
+        else if (best == 192) hipLaunchKernelGGL((tile_kernel<4, 3, 2, 4, G>), grid, dim3(512), 2 * 128 * 256, s, w, a);
+        else if (best == 128) hipLaunchKernelGGL((tile_kernel<4, 2, 2, 4, G>), grid, dim3(512), 2 * 128 * 256, s, w, a);
+        else hipLaunchKernelGGL((tile_kernel<2, 2, 2, 2, G>), grid, dim3(256), 2 * 64 * 256, s, w, a);
         return;
     }
-    const int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4, my = blocks(a.m, 16 * mt);
+    int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
     const size_t lds = (size_t)chunks * 4 * mt * 1024;
     if (tiles >= 4 * cus && lds <= 160 * 1024) {
         const int waves = std::min(16, blocks(tiles, (long)cus * blocks(tiles, 16L * cus)));
-        const dim3 grid(blocks(tiles, waves), my), block(64 * waves);
+        const dim3 grid(blocks(tiles, waves), blocks(a.m, 16 * mt)), block(64 * waves);
         if (mt == 1) hipLaunchKernelGGL((row_kernel<1, G>), grid, block, lds, s, w, a);
         else if (mt == 2) hipLaunchKernelGGL((row_kernel<2, G>), grid, block, lds, s, w, a);
         else hipLaunchKernelGGL((row_kernel<4, G>), grid, block, lds, s, w, a);
         return;
     }
+    // fewer rows of x a workgroup where that leaves CUs without one
+    while (mt > 1 && (long)tiles * blocks(a.m, 16 * mt) < cus) mt /= 2;
     const int most = mt == 4 ? 8 : 16, waves = blocks(chunks, blocks(chunks, most));
-    const dim3 grid(tiles, my), block(64 * waves);
+    const dim3 grid(tiles, blocks(a.m, 16 * mt)), block(64 * waves);
     const size_t red = (size_t)waves * 4 * mt * 68 * 4;
     if (mt == 1) hipLaunchKernelGGL((split_kernel<1, G>), grid, block, red, s, w, a);
     else if (mt == 2) hipLaunchKernelGGL((split_kernel<2, G>), grid, block, red, s, w, a);
