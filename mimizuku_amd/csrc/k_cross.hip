@@ -109,11 +109,18 @@ struct State {
     f32x4 acc[QT][4];  // result u of lane (c, g) holds channels 16 g + 4 e + u of query c
 };
 
-// NW waves, which take the blocks in turn, or, with OWN, four times 16 QT queries of their own and every block, or, eight of them,
-// two such fours that have half of the blocks each (no alignment rows).
+// Four waves that take the blocks in turn, or, with OWN, that have 16 QT queries of their own each and take every block, or, eight of
+// them, two such fours that have half of the blocks each (no alignment rows).
+//
+// Few queries (a decoder's step) are bound by the bytes of keys and values: 32 rows of 20 heads and 300 to 1500 positions, 157 MB in 35.7 us
+// (4.4 TB/s, of 6.6 that a plain read reaches: each wave has the two blocks on their way that its registers hold, and rows of
+// unequal lengths leave the last CUs alone); one row of 6 heads and 250 positions, 4.5 us, is a chain of launch, lengths, keys,
+// values and the join. Prompts are bound by the vector unit: per block and 16 queries 4 products of S and 8 of O on the
+// matrix cores stand against some 60 vector instructions of softmax. 8 rows of 224 tokens, 20 heads: 34.4 us (401 TFLOP/s, counted
+// once for O although P has two parts).
 template <int QT, bool ALIGN, int NW, bool OWN>
 __global__ void __launch_bounds__(64 * NW, OWN ? (NW == 8 && QT == 1 ? 4 : 2) : QT == 1 ? 4 : 2) cross_kernel(MzCross a, Launch n) {
-    static_assert(!(OWN && ALIGN));
+    static_assert(OWN ? !ALIGN : NW == 4);
     __shared__ float red[OWN ? 1 : NW][16][68], ms[NW][16], ls[NW][16];
     __shared__ float lse2s[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
@@ -372,9 +379,8 @@ __global__ void __launch_bounds__(64 * NW, OWN ? (NW == 8 && QT == 1 ? 4 : 2) : 
             }
     }
 
-    // the waves' states joined, 16 queries at a time, by the first 256 threads
-    const int col = tid >> 4 & 15, d4 = (tid & 15) * 4;
-    const bool mine256 = NW == 4 || tid < 256;
+    // the waves' states joined, 16 queries at a time
+    const int col = tid >> 4, d4 = (tid & 15) * 4;
     // Alignment rows of 16 queries: their scores (in powers of two, get(query, row, position)) to probabilities, 0 where nothing
     // is seen, by all threads, eight of a row's scores a thread at a time and the first ones of four rows.
     constexpr int STRIDE = 64 * NW;
@@ -433,12 +439,12 @@ __global__ void __launch_bounds__(64 * NW, OWN ? (NW == 8 && QT == 1 ? 4 : 2) : 
     auto emit = [&](int t, float mm, float ll, f32x4 o, Few& x, auto get) {
         const int q = q0 + 16 * t + col, i = token_of(q), h = kh * grp + q - i * grp;
         const float inv = ll == 0.f ? 0.f : 1.f / ll, lse2 = ll == 0.f ? -INFINITY : mm - UP + __builtin_amdgcn_logf(ll);
-        if (mine256 && q < nq && i < s.count) {
+        if (q < nq && i < s.count) {
             st4(a.out + r * a.out_row + i * a.out_token + h * a.out_head + d4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
             if (a.lse && d4 == 0) a.lse[((long)r * a.tokens + i) * a.heads + h] = lse2 * LN2;
         }
         if (ALIGN) {
-            if (mine256 && d4 == 0) lse2s[col] = lse2;
+            if (d4 == 0) lse2s[col] = lse2;
             __syncthreads();
             probabilities(t, x, get);
             __syncthreads();
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? (NW == 8 && QT == 1 ? 4 : 2) : 
                 few_scores(t, ALIGN ? rows(t) : 0, x, in_place);
                 emit(t, mm, ll, o, x, in_place);
             }
-        } else if (mine256 && q0 + 16 * t + col < nq) {
+        } else if (q0 + 16 * t + col < nq) {
             float* w = states + (split * (16 * QT) + 16 * t + col) * STATE;
             shared_store(w + d4, o[0], o[1]);
             shared_store(w + d4 + 2, o[2], o[3]);
@@ -500,7 +506,7 @@ __global__ void __launch_bounds__(64 * NW, OWN ? (NW == 8 && QT == 1 ? 4 : 2) : 
         f32x4 o = {};
         Few x;
         few_scores(t, ALIGN ? rows(t) : 0, x, in_memory);  // (they come with the states)
-        if (mine256 && q0 + 16 * t + col < nq)
+        if (q0 + 16 * t + col < nq)
             for (int k0 = 0; k0 < splits; k0 += 4) {
                 float2 y[4][3];
 #pragma unroll
@@ -538,19 +544,28 @@ Launch cross_shape(const MzCross& a) {
     n.by_group = inverse(n.group);
     n.waves = 4;
     n.splits = 1;
-    const long groups = pairs * ((nq + 63) / 64);  // of 64 queries
+    // OWN where groups of 64 queries reach every CU. 16 rows of 64 tokens, 20 heads, up to 1500 positions (320 groups): 26.7 us,
+    // 30.3 without; 8 of 224 (640) 34.4 and 42.1, 16 of 224 52.5 and 78.8; but 4 of 224 (320) 26.4 and 22.1.
+    const long groups = pairs * ((nq + 63) / 64);
     n.own = !a.align && nq > 16 && groups >= cus;
     if (n.own) {
-        n.qt = groups >= 5 * cus ? 2 : 1;
+        // Twice the queries a wave where groups of 128 fill the card five times and leave few places empty: 32 of 224 take 109 us,
+        // 115 otherwise, 8 of 1500 188 and 200; but 16 of 224 (640 groups) 59 and 52.5, 64 of 64 96 and 72.
+        const long wide = pairs * ((nq + 127) / 128);
+        n.qt = wide >= 5 * cus && 16 * wide <= 9 * groups ? 2 : 1;
+        // Eight waves where there is but one workgroup for many CUs: 16 of 64 take 26.7 us, 36.5 with four, 4 of 224 25.6 and 30.5;
+        // 8 of 224 37.3 and 34.4.
         n.waves = groups < 2 * cus ? 8 : 4;
         n.tiles = (int)((nq + 64 * n.qt - 1) / (64 * n.qt));
         return n;
     }
+    // (a workgroup of 16 queries reads keys and values once for them, one of 32 for twice as many)
     n.qt = nq <= 16 ? 1 : 2;
     n.tiles = (int)((nq + 16 * n.qt - 1) / (16 * n.qt));
     const long units = pairs * n.tiles;
-    if (units <= cus && n.qt == 1) n.waves = 8;
-    n.splits = (int)std::max(1L, std::min({cus / units, blocks / 10, 256L}));
+    // Shares of at least five blocks: one row of 6 heads and 1500 positions takes 6.5 us with five, 7.0 with ten and 7.2 with three, one
+    // of 20 heads 7.7, 7.6 and 9.6 (12.0 without shares).
+    n.splits = (int)std::max(1L, std::min({cus / units, blocks / 5, 256L}));
     n.per = (int)((blocks + n.splits - 1) / n.splits);
     const long keep = (long)n.per * BLK;
     n.kept = a.align && keep * kept_queries(n, nq) <= (units * n.splits <= cus ? KEPT_FLOATS_ALONE : KEPT_FLOATS) ? (int)keep : 0;
@@ -570,8 +585,7 @@ void launch(hipStream_t s, const MzCross& a, const Launch& n) {
             return;
         }
     if (n.qt == 2) hipLaunchKernelGGL((cross_kernel<2, ALIGN, 4, false>), grid, dim3(256), lds, s, a, n);
-    else if (n.waves == 4) hipLaunchKernelGGL((cross_kernel<1, ALIGN, 4, false>), grid, dim3(256), lds, s, a, n);
-    else hipLaunchKernelGGL((cross_kernel<1, ALIGN, 8, false>), grid, dim3(512), lds, s, a, n);
+    else hipLaunchKernelGGL((cross_kernel<1, ALIGN, 4, false>), grid, dim3(256), lds, s, a, n);
 }
 
 }  // namespace

@@ -1,4 +1,11 @@
-// Products with 4-bit weights (mz_w4 in mimizuku.h).
+// Products with 4-bit weights (mz_w4 in mimizuku.h): y[m, n] = sum over the groups g of a row of weights of
+//     scale[n, g] * (sum over the columns k of g of code[n, k] x[m, k]).
+// A code is a whole number of -8 .. 7, exact in fp16, so the sums of a group run on the matrix cores (products of two fp16
+// numbers are exact in fp32, and so is the accumulator's format), and a group's scale, fp16 too, is applied to its sum in fp32: no
+// weight is ever rounded, and nothing rounds to fewer bits than 32 before the result is stored.
+// Few rows of x are bound by the bytes of the weights, 4 bits and 16 / group each, and below that by the launch; from about 32
+// rows on, by turning codes into fp16 (13 operations for 8 codes) and by reading x from LDS; hundreds of rows of x by the
+// rate at which both feed the matrix cores.
 #include <algorithm>
 
 #include "mz_common.h"
@@ -181,7 +188,9 @@ __device__ __forceinline__ void to_lds(const f16* from, u32x4* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-// Few rows of weights: a workgroup takes 16 of them, its waves the entries in turn, x from memory; their sums meet in LDS.
+// Few rows of weights: a workgroup takes 16 of them, its waves the entries in turn, x from memory (which its caches hold); their
+// sums meet in LDS. 1 x 5120 x 1280 (rows of x, rows of weights, columns): 3.4 us, as long as an empty launch and two
+// dependent reads take; 8 x 1280 x 5120: 5.6 us. Requesting several entries ahead did not help: each wave has two or three.
 template <int MT, int G>
 __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW4Linear a) {
     constexpr int LD = 68;  // (of 64 results: four rows of x 4 banks apart, so that reading 16 columns of 4 rows meets no conflict)
@@ -219,7 +228,9 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW
 }
 
 // Many rows of weights: x lies in LDS, in the order of operands, and each wave takes 16 rows of weights and all of their columns,
-// the next entries on their way.
+// the next entries on their way. 1 x 51866 x 1280, groups of 32: 10.7 us (3.5 TB/s, of weights that no cache held); 32 rows:
+// 16.6 us, as much for the codes' arithmetic and the reads of LDS as for memory. Three, four and five entries ahead
+// took 10.9, 11.1 and 11.1 us for the one row, ten 13.7: more registers, and no wave waits less for its first.
 template <int MT, int G>
 __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
     extern __shared__ u32x4 xs[];  // [chunk][s][MT][64]
@@ -266,7 +277,9 @@ __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
 }
 
 // Many rows of x: a workgroup takes 16 MT WM rows of x times 16 NT WN of weights, WM x WN waves. 128 columns at a time: those of x
-// go straight into LDS, in two buffers, the weights' codes into registers.
+// go straight into LDS, in two buffers, the weights' codes into registers. 1792 x 5120 x 1280, groups of 128: 36.7 us
+// (640 TFLOP/s; a library's product of fp16 weights 27.6), groups of 32: 46.6; 4096 x 4096 x 4096: 165 us (830). What bounds it is
+// the vector unit next to the matrix cores: codes turned into numbers by every wave row, scales applied group by group.
 template <int MT, int NT, int WM, int WN, int G>
 __global__ void __launch_bounds__(64 * WM * WN, 2) tile_kernel(MzW4 w, MzW4Linear a) {
     extern __shared__ u32x4 xs[];  // [2][rows][16 pieces of 8 columns, piece p of row r at p ^ r % 16]
@@ -349,8 +362,12 @@ int blocks(long x, long per) { return (int)((x + per - 1) / per); }
 template <int G>
 void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
     const int tiles = blocks(w.n, 16), chunks = w.k / 128, cus = mz_cu_count();
-    if (a.m > 64 && (long)blocks(a.m, 64) * blocks(w.n, 64) >= cus / 2) {
-        // eight waves a CU: the width whose last round of workgroups leaves the least idle (64: several workgroups a CU)
+    // Tiles, where there are enough of 64 x 64 for a quarter of the CUs: 224 x 1280 x 5120 (80 of them) takes 26.8 us, 31.9 by
+    // split_kernel; 128 x 1280 x 5120 (40) 26.9 and 21.0.
+    if (a.m > 64 && (long)blocks(a.m, 64) * blocks(w.n, 64) >= cus / 4) {
+        // Of the widths, eight waves a CU, the one whose last round of workgroups leaves the least idle (16 more columns stand for
+        // the rows of x; 64: several workgroups a CU, which take 1.15 times as long for a result). 1792 x 5120 x 1280: 36.7 us with
+        // 320, 53, 43, 40 and 44 with 256, 192, 128 and 64; 448 x 5120 x 1280: 30, 25, 20.9, 16.9 and 16.1.
         int best = 64;
         double least = 1.15 * blocks(a.m, 64) * blocks(w.n, 64) * 64 * 64 / cus + 64 * 64;
         for (int bn : {320, 256, 192, 128}) {
@@ -367,6 +384,8 @@ void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
     }
     int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
     const size_t lds = (size_t)chunks * 4 * mt * 1024;
+    // Four tiles a CU and more: 32 x 51866 x 1280 takes 16.6 us by row_kernel, 40.3 by split_kernel (1 row: 10.9, 14.3);
+    // 32 x 5120 x 1280 (320 tiles) 12.6 and 7.5. x has to fit into LDS.
     if (tiles >= 4 * cus && lds <= 160 * 1024) {
         const int waves = std::min(16, blocks(tiles, (long)cus * blocks(tiles, 16L * cus)));
         const dim3 grid(blocks(tiles, waves), blocks(a.m, 16 * mt)), block(64 * waves);
@@ -375,7 +394,7 @@ void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
         else hipLaunchKernelGGL((row_kernel<4, G>), grid, block, lds, s, w, a);
         return;
     }
-    // fewer rows of x a workgroup where that leaves CUs without one
+    // Fewer rows of x a workgroup where that leaves CUs without one: 32 x 1280 x 5120 takes 7.6 us with 16 of them, 12.1 with 32.
     while (mt > 1 && (long)tiles * blocks(a.m, 16 * mt) < cus) mt /= 2;
     const int most = mt == 4 ? 8 : 16, waves = blocks(chunks, blocks(chunks, most));
     const dim3 grid(tiles, blocks(a.m, 16 * mt)), block(64 * waves);
