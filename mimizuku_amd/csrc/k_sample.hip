@@ -110,8 +110,8 @@ struct Weights {
         return sum - V * ABOVE;
     }
     static constexpr u64 ABOVE = 0x433ULL << 52;
-    // whether -inf has weight 0: something finite is further below the top than `lowest`
-    __device__ __forceinline__ bool plain() const { return top > (double)LOWEST; }
+    // whether -inf, taken as `lowest`, has weight 0: not where a temperature leaves every finite number a weight
+    __device__ __forceinline__ bool plain() const { return lowest > LOWEST; }
 };
 
 // ---------------------------------------------------------------- sums over a workgroup

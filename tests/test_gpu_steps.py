@@ -694,3 +694,175 @@ def test_a_captured_decoding_step(ctx, dev):
         check_sample(x, u[:, i], got, mask, temperatures=temps, top_p=0.9, top_k=200)
         tokens = got[0].tolist()
     L.check(L.lib().mz_graph_free(g))
+
+
+# ---------------------------------------------------------------- limits of the choices between variants
+
+
+@pytest.mark.parametrize("m,n,k,group", [(1000, 5129, 128, 64), (1800, 5100, 128, 128), (1025, 4099, 256, 32), (700, 2050, 128, 64),
+                                         (448, 5121, 128, 128), (385, 6150, 256, 64), (4097, 1281, 128, 32), (100, 8200, 128, 64),
+                                         (65, 16384, 128, 128), (2049, 513, 128, 32), (65, 30000, 128, 32), (31, 17000, 256, 64)])
+@pytest.mark.parametrize("epilogue", [L.EPI_RESID_F32, L.EPI_GELU_F16])
+def test_w4_linear_in_tiles(ctx, dev, epilogue, m, n, k, group):
+    """Numbers of rows of either side that fill tiles of every width and leave their last ones ragged; as many workgroups as there
+    are CUs, some more, and several times as many."""
+    rng = np.random.default_rng(m + n)
+    w, x, bias = f16(rng, (n, k), k ** -0.5), f16(rng, (m, k), 1.0), f16(rng, (n,), 0.3)
+    got, before = run_linear(ctx, dev, packed(ctx, dev, w, group), x, bias, epilogue, ldo=n + 1)
+    check_linear(x, R.w4_values(*R.w4_codes(w, group), group), bias, epilogue, got, before if epilogue == L.EPI_RESID_F32 else None)
+
+
+@pytest.mark.parametrize("rows,tokens,heads,pos", [(4, 64, 64, 40), (4, 65, 64, 70), (8, 200, 34, 33), (5, 250, 64, 65), (20, 129, 64, 31),
+                                                   (40, 128, 33, 40), (33, 64, 40, 5), (1, 17, 256, 96), (129, 1, 1, 400), (257, 16, 1, 161)])
+def test_cross_where_the_card_fills(ctx, dev, rows, tokens, heads, pos):
+    """As many groups of queries as there are CUs, some more, and several times as many; rows of unequal lengths, none among them."""
+    length = [(pos * (1 + 7 * r % 11)) // 11 for r in range(rows)]
+    length[rows // 2] = 0
+    cross_case(ctx, dev, rows + tokens, rows, tokens, heads, heads, pos, length=length, count=[tokens - (r % 3 == 2) * (tokens // 2) for r in range(rows)])
+
+
+def test_cross_rows_that_share_a_slot(ctx, dev):
+    """The same slot for every row, seen from other places each, is as good as slots of their own; every call again is bit for bit
+    the same."""
+    rng = np.random.default_rng(21)
+    rows, heads, pos = 9, 6, 700
+    k, v = (f16(rng, (2, pos, heads, 64)) for _ in range(2))
+    for tokens in (1, 20, 300):
+        q = f16(rng, (rows, tokens, heads, 64), 1.5)
+        kw = dict(slot=[1] * rows, first=[0, 5, 31, 32, 33, 200, 699, 0, 700], length=[700, 6, 700, 33, 100, 700, 700, 1, 700])
+        got = run_cross(ctx, dev, q, k, v, **kw)
+        check_cross(q, k, v, got, **kw)
+        again = run_cross(ctx, dev, q, k, v, **kw)
+        for name in got:
+            np.testing.assert_array_equal(got[name], again[name])
+
+
+@pytest.mark.parametrize("vocab", [30000, 51866])
+@pytest.mark.parametrize("temperature", [0.05, 1.0, 3.0])
+@pytest.mark.parametrize("top_k", [0, 65, 512, 513, 1000, 1024, 1025, 2000, 20000])
+def test_sample_where_long_lists_end(ctx, dev, vocab, temperature, top_k):
+    rng = np.random.default_rng(top_k + vocab)
+    n = 9
+    x, u = logits(rng, n, vocab, np.float32), rng.random(n, dtype=np.float32)
+    kw = dict(temperature=temperature, top_k=top_k, top_ps=f32([1, .999, .97, .9, .7, .5, .3, .05, .9999]), min_ps=f32([0, 0, 0, .001, 0, 0, 1e-6, 0, 1e-9]))
+    assert check_sample(x, u, run_sample(ctx, dev, x, u, **dict(kw)), **kw) <= 1
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("values", [[0.0], [0.0, -1.0], [3.0, 2.5, -7.0], [-0.0, 0.0, 2.0 ** -20], [1.0, -60000.0]], ids=str)
+@pytest.mark.parametrize("limits", [dict(), dict(top_k=1500), dict(top_p=0.5), dict(top_k=1025, top_p=0.9), dict(top_p=0.999, temperature=5.0),
+                                    dict(min_p=0.3), dict(top_k=1023, min_p=0.5, top_p=0.25)], ids=str)
+def test_sample_of_more_equal_logits_than_a_list_holds(ctx, dev, dtype, values, limits):
+    rng = np.random.default_rng(len(values))
+    x = rng.choice(np.array(values, np.float64), (4, 20011)).astype(dtype)
+    u = np.array([0.0, 0.3, 0.777, 1.0 - 2.0 ** -24], np.float32)
+    got = run_sample(ctx, dev, x, u, **limits)
+    assert check_sample(x, u, got, **limits) <= 2  # (where all weights but equal ones are 0, sums end on borders)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("t", [1e-44, 0.01, 1.0, 1e6, 1e38])
+def test_sample_of_lowest_logits(ctx, dev, dtype, t):
+    """The type's lowest number is a logit like others: rows of nothing else, rows that have it instead of a mask, rows with one
+    or two tokens above it; so is its least one, next to zeros."""
+    low = np.finfo(dtype).min
+    rng = np.random.default_rng(4)
+    x = np.full((7, 3001), low, dtype)
+    x[1, 5:] = rng.standard_normal(2996).astype(dtype)
+    x[2, 2999] = 0
+    x[3, [7, 8]] = 0.5, 0.25
+    x[4, ::2] = -np.inf
+    x[5, :] = np.finfo(dtype).max
+    x[5, ::3] = low
+    x[6] = -np.finfo(dtype).smallest_subnormal
+    x[6, ::2] = 0
+    u = np.array([.1, .3, .5, .7, .9, .37, .61], np.float32)
+    for limits in (dict(), dict(top_p=0.9), dict(top_k=30), dict(min_p=0.1)):
+        kw = dict(temperature=np.float32(t), **limits)
+        check_sample(x, u, run_sample(ctx, dev, x, u, **kw), **kw)
+
+
+def test_contexts_at_once(ctx):
+    """Contexts of two threads, each with its own stream and workspace, while both are at work: the results of one alone."""
+    import threading
+    rng = np.random.default_rng(8)
+    heads, pos, n, k, v = 6, 1500, 500, 256, 20000
+    w, x = f16(rng, (n, k), 0.1), f16(rng, (9, k))
+    q, (ek, ev) = f16(rng, (2, 1, heads, 64), 1.5), (f16(rng, (2, pos, heads, 64)) for _ in range(2))
+    lg, u = logits(rng, 8, v, np.float32), rng.random(8, dtype=np.float32)
+
+    def work(c, times):
+        d, out = Dev(c), []
+        try:
+            p = packed(c, d, w, 32)
+            for _ in range(times):
+                lin, _ = run_linear(c, d, p, x, None, L.EPI_F32)
+                cr = run_cross(c, d, q, ek, ev, length=[1500, 700])
+                out.append([lin, cr["out"], cr["lse"], *run_sample(c, d, lg, u, top_p=0.95, top_k=700)])
+        finally:
+            d.free()
+        return out
+
+    want, got = work(ctx, 1)[0], {}
+
+    def thread(i):
+        c = model.Context(0)
+        try:
+            got[i] = work(c, 12)
+        finally:
+            c.close()
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 2
+    for runs in got.values():
+        for run in runs:
+            for a, b in zip(run, want):
+                np.testing.assert_array_equal(a, b)
+
+
+def test_graphs_that_share_a_workspace(ctx, dev):
+    """Two captured calls whose workgroups share rows, and a captured choice of tokens, replayed in turns with eager calls of other
+    sizes between: every replay equals the eager result."""
+    rng = np.random.default_rng(9)
+    heads, pos = 6, 1500
+    k, v = (f16(rng, (3, pos, heads, 64)) for _ in range(2))
+    D = {"k": dev(k), "v": dev(v), "len": dev(i32([1500, 900, 40]))}
+    x, u = logits(rng, 5, 30000, np.float32), rng.random(5, dtype=np.float32)
+    dx, du = dev(x), dev(u)
+
+    def attend(rows, tokens, q, out):
+        steps.cross_attention(ctx, q, out, D["k"], D["v"], rows, tokens, heads, pos, k_strides=(pos * heads * 64, heads * 64, 64), len=D["len"])
+
+    calls = []
+    for rows, tokens in ((1, 1), (3, 12)):
+        q, shape = dev(f16(rng, (rows, tokens, heads, 64), 1.5)), (rows, tokens, heads, 64)
+        calls.append((lambda o, rows=rows, tokens=tokens, q=q: attend(rows, tokens, q, o), shape, np.float16))
+    calls.append((lambda o: steps.sample(ctx, dx, 5, 30000, du, o, top_k=600, top_p=0.9), (5,), np.int32))
+    want, outs, graphs = [], [], []
+    for f, shape, t in calls:
+        o = dev(np.zeros(shape, t))
+        f(o)
+        want.append(ctx.download(o, shape, t))
+    for f, shape, t in calls:
+        outs.append(dev(np.zeros(shape, t)))
+        g = C.c_void_p()
+        L.check(L.lib().mz_graph_begin(ctx.h))
+        f(outs[-1])
+        L.check(L.lib().mz_graph_end(ctx.h, C.byref(g)))
+        graphs.append(g)
+    other = dev(np.zeros((2, 1, heads, 64), np.float16))
+    oq = dev(f16(rng, (2, 1, heads, 64)))
+    for i in range(6):
+        for j in ((0, 1, 2), (2, 1, 0), (1, 0, 2))[i % 3]:
+            ctx.upload(outs[j], np.zeros(calls[j][1], calls[j][2]))
+            L.check(L.lib().mz_graph_launch(ctx.h, graphs[j]))
+            if i % 2:
+                attend(2, 1, oq, other)
+        for (f, shape, t), o, w in zip(calls, outs, want):
+            np.testing.assert_array_equal(ctx.download(o, shape, t), w)
+    for g in graphs:
+        L.check(L.lib().mz_graph_free(g))
