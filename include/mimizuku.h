@@ -293,9 +293,8 @@ int mz_w4_linear(mz_ctx* c, const mz_w4* w, const mz_w4_linear_args* a);
  * reads head h / (heads / kv_heads). There is no causal mask: row r's tokens all see the positions first[r] (first 0: 0)
  * to below min(len[r], positions) (len 0: positions). A row that sees nothing, or whose slot lies outside, gets out 0 and
  * lse -inf; keys and values that it does not see do not touch it, NaN or not. An infinite value that is seen comes out as
- * NaN. Probabilities are carried with 20 bits or
- * more down to 2^-31 of a row's largest, sums with 32, the output is rounded once. The
- * last bits of a row may differ with the other rows of the call, its tokens, `positions` and the device's CUs. */
+ * NaN. Probabilities are carried with 20 bits or more down to 2^-31 of a row's largest, sums with 32, the output is rounded
+ * once. The last bits of a row may differ with the other rows of the call, its tokens, `positions` and the device's CUs. */
 typedef struct {
     uint64_t q, out;
     int64_t q_row, q_token, q_head, out_row, out_token, out_head;
@@ -320,8 +319,9 @@ int mz_cross_attention_bytes(mz_ctx* c, const mz_cross_attention_args* a, size_t
  *   not behind the first place up to which the weights sum to top_p times the sum of the first top_k's (1 or more: no limit),
  *   of weight min_p or more (0 or less: no limit; of the largest weight, 1);
  * the first always is. The token drawn is the lowest kept id up to which the kept weights sum to more than u times their
- * sum, at temperature 0 the first. Weights are computed in 64 bits and summed exactly as multiples of 2^-s, s = min(51, 62 -
- * ceil(log2 vocab)): the order of sums does not matter, and tokens of weight below 2^-(s + 1) are not drawn.
+ * sum, at temperature 0 the first (kept 1, logp 0). Weights are computed in 64 bits, to 2e-12 of each, and summed exactly as
+ * multiples of 2^-s, s = min(51, 62 - ceil(log2 vocab)): the order of sums does not matter, and tokens of weight below
+ * 2^-(s + 1) are not drawn.
  * Ids with a nonzero mask byte and logits of -inf are no tokens. A row without any, one with a NaN or a logit of +inf
  * (unmasked), and one whose temperature is negative or no finite number or whose top_p or min_p is NaN has the token -1,
  * kept 0 and logp NaN (-inf where there is just nothing left). u below 0 or NaN counts as 0, of 1 or more as the largest
