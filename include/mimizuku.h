@@ -287,8 +287,9 @@ int mz_w4_linear(mz_ctx* c, const mz_w4* w, const mz_w4_linear_args* a);
 
 /* out = softmax(scale q . k) v of queries over fp16 keys and values of `slots` sequences (an encoder's outputs) of any
  * length: position t, head h of slot s at k + s * k_slot + t * k_pos + h * k_head, its 64 channels together (v likewise;
- * strides in elements, multiples of 8, k_pos and v_pos at most 2^24, addresses multiples of 16 bytes). MZ_BUF_XKV's tiles are such keys and values
- * (k_pos 64, k_head 1536 * 64), and so are the rows of a product (k_pos its width, k_head 64). Queries, outputs, slots,
+ * strides in elements, multiples of 8, k_pos and v_pos at most 2^24, addresses multiples of 16 bytes; positions at most
+ * 2^30). MZ_BUF_XKV's tiles are such keys and values (k_pos 64, k_head 1536 * 64), and so are the rows of a product (k_pos
+ * its width, k_head 64). Queries, outputs, slots,
  * counts, lse, alignment rows and the workspace are those of mz_kv8_attention_args: rows may share slots, query head h
  * reads head h / (heads / kv_heads). There is no causal mask: row r's tokens all see the positions first[r] (first 0: 0)
  * to below min(len[r], positions) (len 0: positions). A row that sees nothing, or whose slot lies outside, gets out 0 and

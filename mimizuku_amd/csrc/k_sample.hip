@@ -13,9 +13,9 @@
 //
 // What bounds it is the vector unit and the passes' latency, not memory: a row is 16 waves of a CU whatever the number of rows, a
 // weight about 20 instructions in 64 bits, a pass 3 to 9 us. One row of 51,865 with every limit 17 us (a pass for the largest,
-// lists, two sorts); 32 rows with top_p 0.9 36 to 50 (a pass that counts tokens in intervals, one that sums the weights around
+// lists, two sorts); 32 rows with top_p 0.9 36 to 47 (a pass that counts tokens in intervals, one that sums the weights around
 // the place exactly, one that draws; what the data leave near the place decides on a second sum); 160 rows without limits 24
-// (the largest, the sums by pieces); 1024 fp16 rows with settings of their own 168 to 175 (four rows a CU, one after the other).
+// (the largest, the sums by pieces); 1024 fp16 rows with settings of their own 160 to 170 (four rows a CU, one after the other).
 // Sums of weights by floating-point atomics in LDS were slower than counts and depend on the order; whole rows in registers need
 // more of them than 16 waves leave.
 #include <algorithm>
@@ -602,14 +602,16 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
             // (the next attempt knows what a sum really is)
             for (int attempt = 0; attempt < 4; attempt++) {
                 const int first = block_all(about + off >= goal ? tid : BINS - 1, Min());
-                // With what is in front of it, and some behind, if that is few enough for one wave; otherwise some intervals around it.
+                // With what is in front of it, and some behind, if that is few enough for one wave; otherwise some intervals around it:
+                // 256 tokens on either side (with 128 the place is missed more often: 32 rows at top_p 0.9 take 36 to 47 us by
+                // their data, with 128 up to 58).
                 if (tid == first) {
                     sh.before = run - mine;
                     sh.here = run;
                 }
                 __syncthreads();
                 const bool few = sh.here <= 56;
-                const u64 room = few ? 0 : 128;
+                const u64 room = few ? 0 : 256;
                 const int b0 = few ? 0 : block_all(run - mine + room >= sh.before ? tid : BINS - 1, Min());
                 const int b1 = block_all(run <= (few ? 60 : sh.here + room) ? tid : 0, Max());
                 const int end = max(b1, first) + 1;

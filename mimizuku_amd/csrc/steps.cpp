@@ -14,6 +14,7 @@ namespace {
 
 constexpr int MAX_K = 1 << 24;
 constexpr int64_t MAX_WEIGHTS = (int64_t)1 << 36;  // a wave packs 2048 of them: a launch has fewer than 2^32 threads along x
+constexpr int MAX_POSITIONS = 1 << 30;         // (blocks of them are counted in 32 bits)
 constexpr int MAX_SAMPLE_ROWS = (1 << 22) - 1;  // a workgroup of 1024 threads each: a launch has fewer than 2^32 along x
 
 bool w4_shape_ok(int n, int k, int group) {
@@ -52,7 +53,7 @@ int check_linear(const char* who, const mz_w4* w, const mz_w4_linear_args* a, Mz
 }
 
 int check_cross(const char* who, const mz_cross_attention_args* a, MzCross* out) {
-    if (a->rows < 0 || a->tokens < 0 || a->slots < 0 || a->positions < 0)
+    if (a->rows < 0 || a->tokens < 0 || a->slots < 0 || a->positions < 0 || a->positions > MAX_POSITIONS)
         return mz_fail(MZ_ERR_ARG, "%s: %d rows, %d tokens, %d slots, %d positions", who, a->rows, a->tokens, a->slots, a->positions);
     if (a->kv_heads <= 0 || a->heads <= 0 || a->heads % a->kv_heads || a->heads / a->kv_heads > 64)
         return mz_fail(MZ_ERR_ARG, "%s: %d query heads over %d", who, a->heads, a->kv_heads);

@@ -174,6 +174,14 @@ def test_cross_refuses(fn):
     assert L.lib().mz_cross_attention(None, C.byref(L.CrossArgs(**CROSS))) == 2
 
 
+@pytest.mark.parametrize("fn", ["mz_cross_attention", "mz_cross_attention_bytes"])
+@pytest.mark.parametrize("positions", [(1 << 30) + 1, (1 << 31) - 1])
+def test_cross_refuses_more_positions_than_it_can_count(fn, positions):
+    a = L.CrossArgs(**{**CROSS, "positions": positions, "k_pos": 0, "v_pos": 0})
+    with pytest.raises(L.MzError, match=fn):
+        L.check(getattr(L.lib(), fn)(C.byref(NOBODY), C.byref(a), *((C.byref(C.c_size_t()),) if fn.endswith("bytes") else ())))
+
+
 def test_cross_definition():
     rng = np.random.default_rng(3)
     q = rng.standard_normal((2, 3, 4, 64)).astype(np.float16)
