@@ -4,7 +4,7 @@
 // numbers are exact in fp32, and so is the accumulator's format), and a group's scale, fp16 too, is applied to its sum in fp32: no
 // weight is ever rounded, and nothing rounds to fewer bits than 32 before the result is stored.
 // Few rows of x are bound by the bytes of the weights, 4 bits and 16 / group each, and below that by the launch; from about 32
-// rows on, by turning codes into fp16 (13 operations for 8 codes) and by reading x from LDS; hundreds of rows of x by the
+// rows on, by turning codes into fp16 (9 operations for 8 codes) and by reading x from LDS; hundreds of rows of x by the
 // rate at which both feed the matrix cores.
 #include <algorithm>
 
@@ -105,16 +105,25 @@ __global__ void __launch_bounds__(256) unpack_kernel(MzW4 w, f16* dst, long ld) 
 // ---------------------------------------------------------------- products
 
 // the eight codes of a word, as they are: 1024 + (c + 8) and 1024 + 16 (c + 8) are fp16 numbers whose low bits are c + 8
-__device__ __forceinline__ f16x8 numbers(unsigned q) {
-    const unsigned one = 0x000F000Fu, sixteen = 0x00F000F0u, magic = 0x64006400u;
-    const unsigned q8 = q >> 8;
-    const f16x2 off1 = {(f16)-1032.f, (f16)-1032.f}, off16 = {(f16)-72.f, (f16)-72.f}, by = {(f16)0.0625f, (f16)0.0625f};
-    const f16x2 a = __builtin_bit_cast(f16x2, (q & one) | magic) + off1;
-    const f16x2 b = __builtin_bit_cast(f16x2, (q & sixteen) | magic) * by + off16;
-    const f16x2 c = __builtin_bit_cast(f16x2, (q8 & one) | magic) + off1;
-    const f16x2 d = __builtin_bit_cast(f16x2, (q8 & sixteen) | magic) * by + off16;
-    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
+struct Codes {
+    // (Numbers that the compiler does not know: with those it knows, taking the bits and setting the others are two instructions
+    // instead of one. 1 x 51866 x 1280 takes 10.0 us, 10.8 with two. `known` where the registers for the results do not suffice.)
+    unsigned one = 0x000F000Fu, sixteen = 0x00F000F0u, magic = 0x64006400u;
+    __device__ __forceinline__ explicit Codes(bool known) {
+        if (known) return;
+        asm("" : "+s"(one), "+s"(sixteen));
+        asm("" : "+v"(magic));
+    }
+    __device__ __forceinline__ f16x8 operator()(unsigned q) const {
+        const unsigned q8 = q >> 8;
+        const f16x2 off1 = {(f16)-1032.f, (f16)-1032.f}, off16 = {(f16)-72.f, (f16)-72.f}, by = {(f16)0.0625f, (f16)0.0625f};
+        const f16x2 a = __builtin_bit_cast(f16x2, (q & one) | magic) + off1;
+        const f16x2 b = __builtin_bit_cast(f16x2, (q & sixteen) | magic) * by + off16;
+        const f16x2 c = __builtin_bit_cast(f16x2, (q8 & one) | magic) + off1;
+        const f16x2 d = __builtin_bit_cast(f16x2, (q8 & sixteen) | magic) * by + off16;
+        return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+};
 
 template <int G>  // groups of 128 columns
 struct Scales {
@@ -164,7 +173,7 @@ __device__ __forceinline__ void finish(const MzW4Linear& a, int m, long n, float
 // One entry, 16 rows of weights x 128 columns, times 16 MT rows of x: operand lane 16 j + i holds row i, columns 32 s + 8 j .. of
 // either; the result's lane 16 j + i holds column i (a row of weights) and rows 4 j .. 4 j + 3 (of x).
 template <int MT, int G, typename X>
-__device__ __forceinline__ void entry_product(u32x4 q, Scales<G> scale, X x, f32x4 (&sum)[MT]) {
+__device__ __forceinline__ void entry_product(const Codes& numbers, u32x4 q, Scales<G> scale, X x, f32x4 (&sum)[MT]) {
 #pragma unroll
     for (int g = 0; g < G; g++) {
         f32x4 part[MT];
@@ -201,6 +210,7 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW
     const f16* x[MT];
 #pragma unroll
     for (int u = 0; u < MT; u++) x[u] = a.x + min(m0 + 16 * u + i, a.m - 1) * a.ldx + 8 * j;
+    const Codes numbers(false);
     f32x4 sum[MT] = {};
     for (int c = wave; c < chunks; c += waves) {
         const long entry = t * chunks + c;
@@ -211,7 +221,7 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW
         for (int u = 0; u < MT; u++)
 #pragma unroll
             for (int s = 0; s < 4; s++) v[u][s] = ld8(x[u] + c * 128 + 32 * s);
-        entry_product<MT, G>(q, scale, [&](int u, int s) { return v[u][s]; }, sum);
+        entry_product<MT, G>(numbers, q, scale, [&](int u, int s) { return v[u][s]; }, sum);
     }
 #pragma unroll
     for (int u = 0; u < MT; u++)
@@ -228,9 +238,9 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW
 }
 
 // Many rows of weights: x lies in LDS, in the order of operands, and each wave takes 16 rows of weights and all of their columns,
-// the next entries on their way. 1 x 51866 x 1280, groups of 32: 10.7 us (3.5 TB/s, of weights that no cache held); 32 rows:
-// 16.6 us, as much for the codes' arithmetic and the reads of LDS as for memory. Three, four and five entries ahead
-// took 10.9, 11.1 and 11.1 us for the one row, ten 13.7: more registers, and no wave waits less for its first.
+// the next entries on their way. 1 x 51866 x 1280, groups of 32: 10.0 us (3.8 TB/s, of weights that no cache held); 32 rows:
+// 15.9 us, as much for the codes' arithmetic and the reads of LDS as for memory. Three, four and five entries ahead
+// took 10.9, 11.1 and 11.1 us for the one row when two took 10.8, ten 13.7: more registers, and no wave waits less for its first.
 template <int MT, int G>
 __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
     extern __shared__ u32x4 xs[];  // [chunk][s][MT][64]
@@ -257,13 +267,14 @@ __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
         xs[f * 64 + lane] = __builtin_bit_cast(u32x4, ld8(a.x + min(m0 + 16 * u + i, a.m - 1) * a.ldx + c4 * 32 + 8 * j));
     }
     __syncthreads();
+    const Codes numbers(false);
     f32x4 sum[MT] = {};
     for (int c0 = 0; c0 < chunks; c0 += AHEAD)
 #pragma unroll
         for (int d = 0; d < AHEAD; d++) {
             const int c = c0 + d;
             if (c < chunks)
-                entry_product<MT, G>(q[d], scale[d], [&](int u, int s) { return __builtin_bit_cast(f16x8, xs[((c * 4 + s) * MT + u) * 64 + lane]); }, sum);
+                entry_product<MT, G>(numbers, q[d], scale[d], [&](int u, int s) { return __builtin_bit_cast(f16x8, xs[((c * 4 + s) * MT + u) * 64 + lane]); }, sum);
             fetch(c + AHEAD, d);
         }
     const int n = t * 16 + i;
@@ -277,8 +288,8 @@ __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
 }
 
 // Many rows of x: a workgroup takes 16 MT WM rows of x times 16 NT WN of weights, WM x WN waves. 128 columns at a time: those of x
-// go straight into LDS, in two buffers, the weights' codes into registers. 1792 x 5120 x 1280, groups of 128: 36.7 us
-// (640 TFLOP/s; a library's product of fp16 weights 27.6), groups of 32: 46.6; 4096 x 4096 x 4096: 165 us (830). What bounds it is
+// go straight into LDS, in two buffers, the weights' codes into registers. 1792 x 5120 x 1280, groups of 128: 34.5 us
+// (680 TFLOP/s; a library's product of fp16 weights 27.6), of 64: 41.4, of 32: 44.4; 4096 x 4096 x 4096: 161 us (850). What bounds it is
 // the vector unit next to the matrix cores: codes turned into numbers by every wave row, scales applied group by group.
 template <int MT, int NT, int WM, int WN, int G>
 __global__ void __launch_bounds__(64 * WM * WN, 2) tile_kernel(MzW4 w, MzW4Linear a) {
@@ -308,6 +319,10 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) tile_kernel(MzW4 w, MzW4Linea
             scale[u] = scales_at<G>(w.scales + (entry * 16 + i) * G);
         }
     };
+    // The widest tile has hardly enough registers: groups of 64 keep the numbers that the compiler knows (2000 x 4800 x 2560 75 us, 90
+    // otherwise, with registers spilled), the others keep it from mixing the steps (1792 x 5120 x 1280 34.5 us, 42 spilled).
+    constexpr bool APART = G != 2;
+    const Codes numbers(NT == 5 && !APART);
     f32x4 sum[MT][NT] = {};
     load_x(0);
     load_w(0);
@@ -326,6 +341,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) tile_kernel(MzW4 w, MzW4Linea
         f32x4 part[MT][NT];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
+            if (APART) __builtin_amdgcn_sched_barrier(0);
             f16x8 x[MT];
 #pragma unroll
             for (int u = 0; u < MT; u++) x[u] = __builtin_bit_cast(f16x8, buf[(wm + 16 * u + i) * 16 + ((4 * s + j) ^ i)]);
