@@ -383,7 +383,7 @@ void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
     if (a.m > 64 && (long)blocks(a.m, 64) * blocks(w.n, 64) >= cus / 4) {
         // Of the widths, eight waves a CU, the one whose last round of workgroups leaves the least idle (16 more columns stand for
         // the rows of x; 64: several workgroups a CU, which take 1.15 times as long for a result). 1792 x 5120 x 1280: 36.7 us with
-        // 320, 53, 43, 40 and 44 with 256, 192, 128 and 64; 448 x 5120 x 1280: 30, 25, 20.9, 16.9 and 16.1.
+        // 320 (34.8 by now), 53, 43, 40 and 44 with 256, 192, 128 and 64; 448 x 5120 x 1280: 30, 25, 20.9, 16.9 and 16.1.
         int best = 64;
         double least = 1.15 * blocks(a.m, 64) * blocks(w.n, 64) * 64 * 64 / cus + 64 * 64;
         for (int bn : {320, 256, 192, 128}) {
