@@ -221,6 +221,8 @@ struct Row {
     int rounds;              // pieces of a thread
     float* largest;          // of each piece, in LDS (null: too many)
 
+    // lds: null, or a word for each piece that a row of this length can have wherever it begins (see launch: which of the two is
+    // decided there, for all rows alike)
     __device__ __forceinline__ void open(const MzSample& a, long r, float* lds) {
         row = (const T*)a.logits + r * a.ld;
         mask = a.mask;
@@ -228,7 +230,7 @@ struct Row {
         off = (int)((uintptr_t)row % 16 / sizeof(T));
         pieces = (vocab + off + V - 1) / V;
         rounds = (pieces + THREADS - 1) / THREADS;
-        largest = rounds <= MOST_ROUNDS ? lds + threadIdx.x : nullptr;
+        largest = lds ? lds + threadIdx.x : nullptr;
     }
     // where this thread's piece j begins, and where it is read: pieces at the row's ends are moved into it
     __device__ __forceinline__ int begin(int j) const { return (j * THREADS + (int)threadIdx.x) * V - off; }
@@ -362,7 +364,7 @@ __device__ __forceinline__ u64 running(Shared& sh, u64& mine, u64& all) {
 }
 
 template <typename T, bool MASK>
-__global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) {
+__global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift, int words) {
     __shared__ Shared sh;
     const int tid = threadIdx.x, lane = tid & 63;
     const long r = blockIdx.x, n = a.at ? (long)*a.at + a.at_add : 0;
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift) 
     const long at = r * a.stride + n;
     extern __shared__ float largest[];
     Row<T, MASK> row;
-    row.open(a, r, largest);
+    row.open(a, r, words ? largest : nullptr);
     const float t = a.temperatures ? a.temperatures[r] : a.temperature, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
     const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, u0 = a.u[at];
     const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
@@ -821,10 +823,11 @@ template <typename T>
 void launch(hipStream_t s, const MzSample& p) {
     constexpr int V = 16 / sizeof(T);
     const dim3 grid(p.rows), block(THREADS);
+    // of the row that has the most pieces, one that begins V - 1 elements behind a multiple of 16 bytes
     const long rounds = (((long)p.vocab + 2 * V - 2) / V + THREADS - 1) / THREADS;
-    const size_t lds = rounds <= MOST_ROUNDS ? rounds * THREADS * 4 : 0;
-    if (p.mask) hipLaunchKernelGGL((sample_kernel<T, true>), grid, block, lds, s, p, shift_of(p.vocab));
-    else hipLaunchKernelGGL((sample_kernel<T, false>), grid, block, lds, s, p, shift_of(p.vocab));
+    const int words = rounds <= MOST_ROUNDS ? (int)rounds * THREADS : 0;
+    if (p.mask) hipLaunchKernelGGL((sample_kernel<T, true>), grid, block, words * 4, s, p, shift_of(p.vocab), words);
+    else hipLaunchKernelGGL((sample_kernel<T, false>), grid, block, words * 4, s, p, shift_of(p.vocab), words);
 }
 
 }  // namespace

@@ -866,3 +866,34 @@ def test_graphs_that_share_a_workspace(ctx, dev):
             np.testing.assert_array_equal(ctx.download(o, shape, t), w)
     for g in graphs:
         L.check(L.lib().mz_graph_free(g))
+
+
+# ---------------------------------------------------------------- where the pieces' largest logits stop lying in LDS
+
+
+@pytest.mark.parametrize("dtype,vocabs", [(np.float32, range(122876, 122885)), (np.float16, range(245752, 245765))], ids=["f32", "f16"])
+@pytest.mark.parametrize("limits", [dict(), dict(temperature=0.0), dict(top_k=40, temperature=0.8), dict(top_p=0.9, temperature=0.6), dict(min_p=0.05),
+                                    dict(top_k=700, top_p=0.95, temperature=1.5)], ids=str)
+def test_sample_at_the_most_pieces_with_a_word(ctx, dev, dtype, vocabs, limits):
+    """Lengths on either side of 30 pieces a thread, rows that begin at every offset from 16 bytes; largest logits above 0.
+
+    Sums here are of more tokens, in coarser multiples, than the bounds at the top are for: n tokens as multiples of 2^-s, s = 62 -
+    ceil(log2 n), are off by n 2^-(s + 1) at most, and by 2e-12 of each weight. The sum is 1 or more (the largest weight is 1), so its
+    logarithm is off by no more than that, and no limit or share whose border is farther away than twice that falls on the other
+    side: 2^-25.9 for the longest. The logarithm is compared in 64 bits (a difference of a numpy float32 and a Python float is
+    one of 32 bits: it rounds the oracle's to a neighbour first)."""
+    per = 16 // np.dtype(dtype).itemsize
+    for vocab in vocabs:
+        rng = np.random.default_rng(vocab)
+        x, u = logits(rng, per, vocab, dtype), rng.random(per, dtype=np.float32)
+        assert (x.max(1) > 0).all()
+        off = vocab * 2.0 ** (int(np.ceil(np.log2(vocab))) - 63) + 4e-12
+        want = [R.sample(x[r], u[r], **{k: np.float32(v) if k != "top_k" else v for k, v in limits.items()}) for r in range(per)]
+        unsure = sum(near < 2 * off for *_, near in want)
+        for pad in {1 - vocab % 2, 0}:  # rows an odd number of elements apart; all at the same offset, where vocab is even
+            got = run_sample(ctx, dev, x, u, pad=pad, **limits)
+            for r, (tok, logp, kept, near) in enumerate(want):
+                if near >= 2 * off:
+                    assert (got[0][r], got[2][r]) == (tok, kept), (vocab, pad, r, got[0][r], tok, got[2][r], kept, near)
+                    assert abs(float(got[1][r]) - logp) <= U * abs(logp) + off, (vocab, pad, r, got[1][r], logp, off)
+        assert unsure <= 1
