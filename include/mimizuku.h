@@ -318,7 +318,7 @@ int mz_cross_attention_bytes(mz_ctx* c, const mz_cross_attention_args* a, size_t
  * +0 are equal) the lower id first, those tokens are kept that are
  *   among the first top_k (0 or less: no limit),
  *   not behind the first place up to which the weights sum to top_p times the sum of the first top_k's (1 or more: no limit),
- *   of weight min_p or more (0 or less: no limit; of the largest weight, 1);
+ *   of weight min_p or more (0 or less: no limit; the largest weight is 1: above 1 there are none);
  * the first always is. The token drawn is the lowest kept id up to which the kept weights sum to more than u times their
  * sum, at temperature 0 the first (kept 1, logp 0). Weights are computed in 64 bits, to 2e-12 of each, and summed exactly as
  * multiples of 2^-s, s = min(51, 62 - ceil(log2 vocab)): the order of sums does not matter, and tokens of weight below

@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift, 
         if (tid == 0) answer(-1, bad ? NAN : -INFINITY, 0);
         return;
     }
-    if (t == 0.f || top_k == 1 || top_p <= 0.f) {  // the first
+    if (t == 0.f || top_k == 1 || top_p <= 0.f || min_p > 1.f) {  // the first
         unsigned id = ~0u;
         row.each_from(top, [&](float, int i) { id = min(id, (unsigned)i); });
         id = block_all(id, Min());
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift, 
     const bool limit_k = top_k > 0 && (unsigned)top_k < count, limit_p = top_p < 1.f, limit_m = min_p > 0.f;
     float low = -INFINITY;  // the lowest logit of weight min_p or more
     if (limit_m) {
-        const double l = (double)top + (double)t * log(fmin((double)min_p, 1.0));
+        const double l = (double)top + (double)t * log((double)min_p);
         low = (float)l;
         if ((double)low < l) low = value_at(order_of(low) - 1);
     }

@@ -125,9 +125,8 @@ def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
         keep = max(1, int(np.searchsorted(run, need)) + 1)
         near = min(near, np.abs(run - need).min() / run[-1]) if p > 0 else near
     if low > 0:
-        m = min(low, 1.0)
-        keep = min(keep, max(1, int((w >= m).sum())))
-        near = min(near, np.abs(w[1:] - m).min()) if m < 1 and len(w) > 1 else near
+        keep = min(keep, max(1, int((w >= low).sum())))
+        near = min(near, np.abs(w[1:] - low).min()) if low < 1 and len(w) > 1 else near  # (the largest weight is exactly 1)
     order, w = order[:keep], w[:keep]
     by_id = np.argsort(order)
     run = np.cumsum(w[by_id])

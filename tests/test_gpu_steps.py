@@ -897,3 +897,25 @@ def test_sample_at_the_most_pieces_with_a_word(ctx, dev, dtype, vocabs, limits):
                     assert (got[0][r], got[2][r]) == (tok, kept), (vocab, pad, r, got[0][r], tok, got[2][r], kept, near)
                     assert abs(float(got[1][r]) - logp) <= U * abs(logp) + off, (vocab, pad, r, got[1][r], logp, off)
         assert unsure <= 1
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("limits", [dict(), dict(top_k=3), dict(top_k=3000, top_p=0.9), dict(top_p=0.5, temperature=4.0)], ids=str)
+@pytest.mark.parametrize("vocab", [60, 20011])
+def test_sample_of_a_share_that_no_token_has(ctx, dev, dtype, vocab, limits):
+    """min_p above 1 keeps the first of several largest logits, min_p 1 all of them: a row's own and for all rows."""
+    rng = np.random.default_rng(vocab)
+    x = rng.choice(np.array([0.0, 2.0, 1.0]), (6, vocab)).astype(dtype)
+    x[4:, 3::7] = 2.0
+    x[5, ::2] = -np.inf
+    u = np.array([0.0, 0.4, 0.6, 0.8, 0.99, 0.7], np.float32)
+    above = np.nextafter(np.float32(1), np.float32(2))
+    kw = dict(min_ps=f32([above, 2.0, 1.0, np.inf, above, 1e30]), **limits)
+    got = run_sample(ctx, dev, x, u, **dict(kw))
+    assert check_sample(x, u, got, **kw) == 0
+    alone = [0, 1, 3, 4, 5]
+    assert (got[2][alone] == 1).all() and (got[1][alone] == 0).all() and (got[0][alone] == x.argmax(1)[alone]).all()
+    assert got[2][2] > 1
+    kw = dict(min_p=3.0, **limits)
+    got = run_sample(ctx, dev, x, u, **kw)
+    assert check_sample(x, u, got, **kw) == 0 and (got[0] == x.argmax(1)).all() and (got[2] == 1).all()

@@ -236,3 +236,11 @@ def test_sample_definition():
     assert R.sample(np.full(4, -np.inf), 0.5)[:3] == (-1, -np.inf, 0)
     assert R.sample([0.0, np.nan], 0.5)[0] == -1 and R.sample([0.0, 1.0], 0.5, temperature=-1)[0] == -1
     np.testing.assert_allclose(R.sample(x, 0.2, top_k=2)[1], np.log(2 / 3))
+
+
+@pytest.mark.parametrize("min_p", [np.nextafter(np.float32(1), np.float32(2)), 2.0, np.inf])
+def test_sample_definition_of_a_share_that_no_token_has(min_p):
+    """Above 1 there is no token of weight min_p or more, also not where several are the largest: the first alone is kept."""
+    assert R.sample([1.0, 1.0, 0.0], 0.9, min_p=min_p)[:3] == (0, 0.0, 1)
+    assert R.sample([0.0, 1.0, 1.0, 1.0], 0.9, min_p=min_p, top_k=2, top_p=0.99)[:3] == (1, 0.0, 1)
+    assert R.sample([1.0, 1.0, 0.0], 0.9, min_p=1.0)[::2][:2] == (1, 2)
