@@ -871,32 +871,39 @@ def test_graphs_that_share_a_workspace(ctx, dev):
 # ---------------------------------------------------------------- where the pieces' largest logits stop lying in LDS
 
 
+def check_sample_of_all_numbers(x, u, got, **kw):
+    """check_sample with a bound that holds for any number of tokens; returns how many rows were too near to a border to tell.
+
+    n tokens as multiples of 2^-s, s = min(51, 62 - ceil(log2 n)), are off by n 2^-(s + 1) at most, and by 2e-12 of each weight. The
+    sum is 1 or more (the largest weight is 1), so its logarithm is off by no more than that, and no limit or share whose border
+    is farther away than twice that falls on the other side: 2^-25.9 for 2^18 tokens. The logarithm is compared in 64 bits (a
+    difference of a numpy float32 and a Python float is one of 32 bits: it rounds the oracle's to a neighbour first)."""
+    unsure, n = 0, x.shape[1]
+    off = n * 2.0 ** (-1 - min(51, 62 - int(np.ceil(np.log2(n))))) + 4e-12
+    for r in range(len(x)):
+        t, k, p, m = (kw[each][r] if kw.get(each) is not None else kw.get(name, usual) for name, each, usual in SETTINGS)
+        tok, logp, kept, near = R.sample(x[r], np.float32(u[r]), np.float32(t), int(k), np.float32(p), np.float32(m))
+        if near < 2 * off:
+            unsure += 1
+            continue
+        assert (got[0][r], got[2][r]) == (tok, kept), (r, got[0][r], tok, got[2][r], kept, near)
+        assert abs(float(got[1][r]) - logp) <= U * abs(logp) + off, (r, got[1][r], logp, off)
+    return unsure
+
+
 @pytest.mark.parametrize("dtype,vocabs", [(np.float32, range(122876, 122885)), (np.float16, range(245752, 245765))], ids=["f32", "f16"])
 @pytest.mark.parametrize("limits", [dict(), dict(temperature=0.0), dict(top_k=40, temperature=0.8), dict(top_p=0.9, temperature=0.6), dict(min_p=0.05),
                                     dict(top_k=700, top_p=0.95, temperature=1.5)], ids=str)
 def test_sample_at_the_most_pieces_with_a_word(ctx, dev, dtype, vocabs, limits):
-    """Lengths on either side of 30 pieces a thread, rows that begin at every offset from 16 bytes; largest logits above 0.
-
-    Sums here are of more tokens, in coarser multiples, than the bounds at the top are for: n tokens as multiples of 2^-s, s = 62 -
-    ceil(log2 n), are off by n 2^-(s + 1) at most, and by 2e-12 of each weight. The sum is 1 or more (the largest weight is 1), so its
-    logarithm is off by no more than that, and no limit or share whose border is farther away than twice that falls on the other
-    side: 2^-25.9 for the longest. The logarithm is compared in 64 bits (a difference of a numpy float32 and a Python float is
-    one of 32 bits: it rounds the oracle's to a neighbour first)."""
+    """Lengths on either side of 30 pieces a thread, rows that begin at every offset from 16 bytes; largest logits above 0."""
     per = 16 // np.dtype(dtype).itemsize
     for vocab in vocabs:
         rng = np.random.default_rng(vocab)
         x, u = logits(rng, per, vocab, dtype), rng.random(per, dtype=np.float32)
         assert (x.max(1) > 0).all()
-        off = vocab * 2.0 ** (int(np.ceil(np.log2(vocab))) - 63) + 4e-12
-        want = [R.sample(x[r], u[r], **{k: np.float32(v) if k != "top_k" else v for k, v in limits.items()}) for r in range(per)]
-        unsure = sum(near < 2 * off for *_, near in want)
         for pad in {1 - vocab % 2, 0}:  # rows an odd number of elements apart; all at the same offset, where vocab is even
             got = run_sample(ctx, dev, x, u, pad=pad, **limits)
-            for r, (tok, logp, kept, near) in enumerate(want):
-                if near >= 2 * off:
-                    assert (got[0][r], got[2][r]) == (tok, kept), (vocab, pad, r, got[0][r], tok, got[2][r], kept, near)
-                    assert abs(float(got[1][r]) - logp) <= U * abs(logp) + off, (vocab, pad, r, got[1][r], logp, off)
-        assert unsure <= 1
+            assert check_sample_of_all_numbers(x, u, got, **limits) <= 1
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
@@ -919,3 +926,53 @@ def test_sample_of_a_share_that_no_token_has(ctx, dev, dtype, vocab, limits):
     kw = dict(min_p=3.0, **limits)
     got = run_sample(ctx, dev, x, u, **kw)
     assert check_sample(x, u, got, **kw) == 0 and (got[0] == x.argmax(1)).all() and (got[2] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("t", [1e-44, 0.01, 1.0, 1e6, 1e38])
+def test_sample_of_lowest_logits_row_by_row(ctx, dev, dtype, t):
+    """Rows of the type's lowest number and of its least one: every row is far enough from a border to tell, but one."""
+    low = np.finfo(dtype).min
+    rng = np.random.default_rng(12)
+    x = np.full((7, 3001), low, dtype)
+    x[1, 5:] = rng.standard_normal(2996).astype(dtype)
+    x[2, 2999] = 0
+    x[3, [7, 8]] = 0.5, 0.25
+    x[4, ::2] = -np.inf
+    x[5, :] = np.finfo(dtype).max
+    x[5, ::3] = low
+    x[6] = -np.finfo(dtype).smallest_subnormal
+    x[6, ::2] = 0
+    u = np.array([.1, .3, .5, .7, .9, .37, .61], np.float32)
+    for limits in (dict(), dict(top_p=0.9), dict(top_k=30), dict(min_p=0.1)):
+        kw = dict(temperature=np.float32(t), **limits)
+        assert check_sample_of_all_numbers(x, u, run_sample(ctx, dev, x, u, **kw), **kw) <= 1
+
+
+@pytest.mark.parametrize("vocab", [50, 3000, 51865])
+@pytest.mark.parametrize("limits", [dict(), dict(top_k=3), dict(top_k=40), dict(top_p=0.45), dict(min_p=0.5), dict(top_p=0.77, top_k=41),
+                                    dict(temperature=0.0)], ids=str)
+def test_sample_of_equal_logits_all_numbers(ctx, dev, vocab, limits):
+    """Ties, their logarithms of shares too."""
+    rng = np.random.default_rng(3)
+    x = np.zeros((5, vocab), np.float32)
+    x[1] = rng.integers(0, 2, vocab)
+    x[2] = rng.integers(-3, 4, vocab)
+    x[3, ::2] = -0.0
+    x[4] = -np.inf
+    x[4, [7, 30, 41]] = -1.5
+    u = np.array([0.3712, 0.8134, 0.1151, 0.7351, 0.9], np.float32)
+    assert check_sample_of_all_numbers(x, u, run_sample(ctx, dev, x, u, **limits), **limits) == 0
+
+
+@pytest.mark.parametrize("m,k,group", [(3, 5120, 128), (16, 5120, 32), (17, 2560, 64), (32, 2560, 128), (40, 1280, 64), (64, 1280, 32),
+                                       (1, 5248, 64), (20, 2688, 32), (64, 1408, 128)])
+def test_w4_linear_of_many_rows_as_long_as_lds(ctx, dev, m, k, group):
+    """Weights of more than four tiles a CU: rows of x that fill the 160 KB of LDS, and rows that are one entry too long for it."""
+    rng = np.random.default_rng(m + k)
+    n = 16385
+    w, x, bias = f16(rng, (n, k), k ** -0.5), f16(rng, (m, k), 1.0), f16(rng, (n,), 0.3)
+    p = packed(ctx, dev, w, group)
+    for epilogue in (L.EPI_F32, L.EPI_GELU_F16):
+        got, _ = run_linear(ctx, dev, p, x, bias, epilogue)
+        check_linear(x, R.w4_values(*R.w4_codes(w, group), group), bias, epilogue, got)
