@@ -344,7 +344,7 @@ typedef struct {
     int64_t stride;
     uint64_t at; /* i32 */
     int at_add;
-    uint64_t work; /* mz_sample_bytes bytes, as mz_kv8_attention_args.work */
+    uint64_t work; /* not read: mz_sample_bytes, which checks the arguments, says 0 bytes for all of them */
     size_t work_bytes;
 } mz_sample_args;
 int mz_sample(mz_ctx* c, const mz_sample_args* a);

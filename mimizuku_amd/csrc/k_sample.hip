@@ -832,8 +832,6 @@ void launch(hipStream_t s, const MzSample& p) {
 
 }  // namespace
 
-size_t mz_sample_work(const MzSample& p) { return 0; }
-
 hipError_t mz_sample_launch(hipStream_t s, const MzSample& p) {
     if (p.half) launch<f16>(s, p);
     else launch<float>(s, p);

@@ -379,7 +379,5 @@ struct MzSample {
     long stride;
     const int* at;
     int at_add;
-    float* work;
 };
-size_t mz_sample_work(const MzSample& p);
 hipError_t mz_sample_launch(hipStream_t s, const MzSample& p);

@@ -101,7 +101,7 @@ int check_sample(const char* who, const mz_sample_args* a, MzSample* out) {
     *out = {a->dtype == MZ_DT_F16, a->rows, a->vocab, DP(const void, a->logits), (long)a->ld, DP(const unsigned char, a->mask),
             a->temperature, a->top_p, a->min_p, a->top_k, DP(const float, a->temperatures), DP(const float, a->top_ps),
             DP(const float, a->min_ps), DP(const int, a->top_ks), DP(const float, a->u), DP(int, a->tokens), DP(float, a->logp),
-            DP(int, a->kept), (long)a->stride, DP(const int, a->at), a->at_add, nullptr};
+            DP(int, a->kept), (long)a->stride, DP(const int, a->at), a->at_add};
     return MZ_OK;
 }
 
@@ -178,12 +178,7 @@ extern "C" int mz_sample_bytes(mz_ctx* c, const mz_sample_args* a, size_t* bytes
     if (!c || !a || !bytes) return mz_fail(MZ_ERR_ARG, "mz_sample_bytes: null argument");
     *bytes = 0;
     MzSample p;
-    if (int r = check_sample("mz_sample_bytes", a, &p)) return r;
-    if (!a->rows) return MZ_OK;
-    OnDevice on(c->device);
-    if (on.status()) return on.status();
-    *bytes = mz_sample_work(p);
-    return MZ_OK;
+    return check_sample("mz_sample_bytes", a, &p);
 }
 
 extern "C" int mz_sample(mz_ctx* c, const mz_sample_args* a) {
@@ -193,7 +188,5 @@ extern "C" int mz_sample(mz_ctx* c, const mz_sample_args* a) {
     if (!a->rows) return MZ_OK;
     OnDevice on(c->device);
     if (on.status()) return on.status();
-    if (int r = check_work("mz_sample", a->work, a->work_bytes, mz_sample_work(p))) return r;
-    p.work = DP(float, a->work);
     return mz_hip(mz_sample_launch(c->stream, p), "mz_sample");
 }

@@ -37,7 +37,7 @@ def cross_bytes(ctx: Context, a: L.CrossArgs) -> int:
 
 
 def sample_bytes(ctx: Context, a: L.SampleArgs) -> int:
-    """Bytes of workspace that mz_sample needs for these arguments."""
+    """Bytes of workspace that mz_sample needs for these arguments: 0."""
     n = C.c_size_t()
     check(L.lib().mz_sample_bytes(ctx.h, C.byref(a), C.byref(n)))
     return n.value
@@ -96,8 +96,9 @@ def sample(ctx: Context, logits: int, rows: int, vocab: int, u: int, tokens: int
            temperatures: int = 0, top_ks: int = 0, top_ps: int = 0, min_ps: int = 0, logp: int = 0, kept: int = 0,
            stride: int = 1, at: int = 0, at_add: int = 0, work: tuple[int, int] | None = None):
     """The next token of rows of logits from given random numbers u, 0 <= u < 1 (mz_sample). temperatures, top_ks, top_ps,
-    min_ps: device arrays of a value per row, in place of the one for all. work: as of Kv8.attention."""
+    min_ps: device arrays of a value per row, in place of the one for all. work: (address, bytes) of a workspace, which it does
+    not read."""
     a = L.SampleArgs(dtype, rows, vocab, logits, ld or vocab, mask, temperature, top_p, min_p, top_k, temperatures, top_ps,
                      min_ps, top_ks, u, tokens, logp, kept, stride, at, at_add)
-    a.work, a.work_bytes = work or ctx.workspace(sample_bytes(ctx, a))
+    a.work, a.work_bytes = work or (0, 0)
     check(L.lib().mz_sample(ctx.h, C.byref(a)))
