@@ -887,7 +887,7 @@ def check_sample_of_all_numbers(x, u, got, **kw):
             unsure += 1
             continue
         assert (got[0][r], got[2][r]) == (tok, kept), (r, got[0][r], tok, got[2][r], kept, near)
-        assert abs(float(got[1][r]) - logp) <= U * abs(logp) + off, (r, got[1][r], logp, off)
+        assert got[1][r] == logp if np.isinf(logp) else abs(float(got[1][r]) - logp) <= U * abs(logp) + off, (r, got[1][r], logp, off)
     return unsure
 
 
