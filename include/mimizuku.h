@@ -272,8 +272,10 @@ int mz_w4_unpack(mz_ctx* c, const mz_w4* w, uint64_t dst, int64_t ld);
 #define MZ_EPI_F32 5 /* mz_w4_linear: out f32 [m][ldo] = acc + bias */
 /* out [m][n] = epilogue(sum over groups of scale * (x . codes) + bias): products of codes and x in 32 bits, exact before
  * they are summed, the scale applied to a group's sum, one rounding at the end (GELU's error included: 0.505 of an fp16
- * step). Any m: 1 to 64 rows read the weights once. The last bits may differ with m and the device's CUs, by which the
- * sums over k are shared out. x, bias and out are read and written by their elements' alignment, x by 16 bytes. */
+ * step). Any m: up to 16 rows of x read the weights once, up to 64 do where there are 16 rows of weights for every CU; with
+ * fewer weights each 16 or 32 rows of x read them again, with more than 64 rows each tile of 64 or 128 does. The last bits may
+ * differ with m and the device's CUs, by which the sums over k are shared out. x, bias and out are read and written by their
+ * elements' alignment, x by 16 bytes. */
 typedef struct {
     int epilogue; /* MZ_EPI_F16, MZ_EPI_GELU_F16, MZ_EPI_RESID_F32 or MZ_EPI_F32 */
     int m;
@@ -294,8 +296,10 @@ int mz_w4_linear(mz_ctx* c, const mz_w4* w, const mz_w4_linear_args* a);
  * reads head h / (heads / kv_heads). There is no causal mask: row r's tokens all see the positions first[r] (first 0: 0)
  * to below min(len[r], positions) (len 0: positions). A row that sees nothing, or whose slot lies outside, gets out 0 and
  * lse -inf; keys and values that it does not see do not touch it, NaN or not. An infinite value that is seen comes out as
- * NaN. Probabilities are carried with 20 bits or more down to 2^-31 of a row's largest, sums with 32, the output is rounded
- * once. The last bits of a row may differ with the other rows of the call, its tokens, `positions` and the device's CUs. */
+ * NaN. A position's probability goes into the output to 2^-21 of itself or 2^-31 of the row's largest, whichever is
+ * more: what n positions lose by the latter is at most n * 2^-31 of the largest value, as much as the output's own
+ * rounding from 2^20 positions on. Sums are in 32 bits, the output is rounded once. The last bits of a row may differ
+ * with the other rows of the call, its tokens, `positions` and the device's CUs. */
 typedef struct {
     uint64_t q, out;
     int64_t q_row, q_token, q_head, out_row, out_token, out_head;

@@ -10,9 +10,14 @@
 // channels 4 i .. 4 i + 3 of those eight positions, eight bytes each, and 16 byte permutations make of them its operands of four
 // products, whose row i is channel 4 i + u.
 //
-// P goes into its product as the sum of two fp16 numbers, 20 bits or more down to 2^-31 of a row's largest: one alone would add an error of
-// the size of the output's rounding. The maximum of a state is moved only when a score passes it by more than 8 (in powers of
-// two), so that most blocks need no exchange between lanes and no rescaling; P is carried times 2^7, at most 2^15.
+// P goes into its product as the sum of two fp16 numbers, both cut: one alone would add an error of the size of the output's
+// rounding. The maximum of a state is moved only when a score passes it by more than 8 (in powers of two), so that most blocks need
+// no exchange between lanes and no rescaling; P is carried times 2^7, at most 2^15. What is lost of it is below 2^-21 of itself, or
+// where the second number would end below fp16's smallest step, 2^-24, below that: 2^-31 of the row's largest.
+//
+// Times here are of a call among 40 back to back, on keys and values of four layers in turn; rows are as long as stated, "unequal"
+// ones 0.27 to 1 times that. Both sides of a rule are of one run. Under a profiler, which runs launches apart, they are up to 2 us
+// longer.
 #include <algorithm>
 
 #include "mz_attn.h"
@@ -112,12 +117,13 @@ struct State {
 // Four waves that take the blocks in turn, or, with OWN, that have 16 QT queries of their own each and take every block, or, eight of
 // them, two such fours that have half of the blocks each (no alignment rows).
 //
-// Few queries (a decoder's step) are bound by the bytes of keys and values: 32 rows of 20 heads and 300 to 1500 positions, 157 MB in 35.7 us
-// (4.4 TB/s, of 6.6 that a plain read reaches: each wave has the two blocks on their way that its registers hold, and rows of
-// unequal lengths leave the last CUs alone); one row of 6 heads and 250 positions, 4.5 us, is a chain of launch, lengths, keys,
-// values and the join. Prompts are bound by the vector unit: per block and 16 queries 4 products of S and 8 of O on the
-// matrix cores stand against some 60 vector instructions of softmax. 8 rows of 224 tokens, 20 heads: 34.4 us (401 TFLOP/s, counted
-// once for O although P has two parts).
+// Few queries (a decoder's step) are bound by the bytes of keys and values: 32 rows of 20 heads and 409 to 1500 positions, 157 MB
+// in 35.9 us (4.4 TB/s, of 6.6 that a plain read reaches: each wave has the two blocks on their way that its registers hold, and rows of
+// unequal lengths leave the last CUs alone); one row of 6 heads and 250 positions, 5.0 us, is a chain of launch, lengths, keys,
+// values and the join. Prompts, 8 rows of 224 tokens, 20 heads, 1500 positions: 39 us (355 TFLOP/s, counted once for O although P
+// has two parts), wait for each other more than for a unit: a barrier every 32 positions with a chain of S, softmax and O between,
+// per 16 queries 4 products of S and 8 of O on the matrix cores and some 60 vector instructions of softmax; vector units are busy
+// 47% of the time, and an eighth of the places of 224 tokens in groups of 64 are empty.
 template <int QT, bool ALIGN, int NW, bool OWN>
 __global__ void __launch_bounds__(64 * NW, OWN ? (NW == 8 && QT == 1 ? 4 : 2) : QT == 1 ? 4 : 2) cross_kernel(MzCross a, Launch n) {
     static_assert(OWN ? !ALIGN : NW == 4);
@@ -544,17 +550,19 @@ Launch cross_shape(const MzCross& a) {
     n.by_group = inverse(n.group);
     n.waves = 4;
     n.splits = 1;
-    // OWN where groups of 64 queries reach every CU. 16 rows of 64 tokens, 20 heads, up to 1500 positions (320 groups): 26.7 us,
-    // 30.3 without; 8 of 224 (640) 34.4 and 42.1, 16 of 224 52.5 and 78.8; but 4 of 224 (320) 26.4 and 22.1.
+    // OWN where groups of 64 queries reach every CU. 20 heads, 1500 positions: 16 rows of 64 tokens (320 groups) 31 to 36 us, 42
+    // without; 4 of 224 (320) 26.1 and 30.2, 8 of 224 (640) 38.8 and 48.8, 16 of 224 69 and 123. Of unequal rows 25.4 and 28.9, 25.3
+    // and 21.9 (the one that it loses), 31.3 and 39.7, 48.7 and 78.3.
     const long groups = pairs * ((nq + 63) / 64);
     n.own = !a.align && nq > 16 && groups >= cus;
     if (n.own) {
-        // Twice the queries a wave where groups of 128 fill the card five times and leave few places empty: 32 of 224 take 109 us,
-        // 115 otherwise, 8 of 1500 188 and 200; but 16 of 224 (640 groups) 59 and 52.5, 64 of 64 96 and 72.
+        // Twice the queries a wave where groups of 128 fill the card five times and leave few places empty: 32 of 224 take 129 us,
+        // 145 otherwise, 8 of 1500 169 and 183; but 16 of 224 (640 groups) 67 and 66, 64 of 64 126 and 95. Of unequal rows 96 and
+        // 103, 124 and 129, 55 and 49, 95 and 74.
         const long wide = pairs * ((nq + 127) / 128);
         n.qt = wide >= 5 * cus && 16 * wide <= 9 * groups ? 2 : 1;
-        // Eight waves where there is but one workgroup for many CUs: 16 of 64 take 26.7 us, 36.5 with four, 4 of 224 25.6 and 30.5;
-        // 8 of 224 37.3 and 34.4.
+        // Eight waves where there is but one workgroup for many CUs: 16 of 64 take 31.5 us, 40.4 with four, 4 of 224 26.4 and 29.9;
+        // 8 of 224 42.9 and 38.3. Of unequal rows 26.3 and 35.8, 25.6 and 29.3, 35.5 and 31.0.
         n.waves = groups < 2 * cus ? 8 : 4;
         n.tiles = (int)((nq + 64 * n.qt - 1) / (64 * n.qt));
         return n;
@@ -563,8 +571,8 @@ Launch cross_shape(const MzCross& a) {
     n.qt = nq <= 16 ? 1 : 2;
     n.tiles = (int)((nq + 16 * n.qt - 1) / (16 * n.qt));
     const long units = pairs * n.tiles;
-    // Shares of at least five blocks: one row of 6 heads and 1500 positions takes 6.5 us with five, 7.0 with ten and 7.2 with three, one
-    // of 20 heads 7.7, 7.6 and 9.6 (12.0 without shares).
+    // Shares of at least five blocks: one row of 6 heads and 1500 positions takes 6.8 us with five, 7.1 with ten and 7.2 with three
+    // (11.0 without shares), one of 20 heads 7.8, 7.6 and 9.8 (11.2).
     n.splits = (int)std::max(1L, std::min({cus / units, blocks / 5, 256L}));
     n.per = (int)((blocks + n.splits - 1) / n.splits);
     const long keep = (long)n.per * BLK;

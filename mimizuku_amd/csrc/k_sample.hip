@@ -12,10 +12,13 @@
 // those that the limits can reach go into a list, and up to 64 of them are put in order by one wave.
 //
 // What bounds it is the vector unit and the passes' latency, not memory: a row is 16 waves of a CU whatever the number of rows, a
-// weight about 20 instructions in 64 bits, a pass 3 to 9 us. One row of 51,865 with every limit 17 us (a pass for the largest,
-// lists, two sorts); 32 rows with top_p 0.9 36 to 47 (a pass that counts tokens in intervals, one that sums the weights around
-// the place exactly, one that draws; what the data leave near the place decides on a second sum); 160 rows without limits 24
-// (the largest, the sums by pieces); 1024 fp16 rows with settings of their own 160 to 170 (four rows a CU, one after the other).
+// weight about 20 instructions in 64 bits, a pass 3 to 9 us. A call among 20 back to back, rows of 51,866 with a dozen likely tokens:
+// 7.3 us at temperature 0 (8.6 for 160 rows); one row with every limit 17 (a pass for the largest, lists, two sorts); 32 rows with
+// top_p 0.9 36 to 47 at temperature 0.6 (a pass that counts tokens in intervals, one that sums the weights around the place
+// exactly, one that draws; what the data leave near the place decides on a second sum; 4 of 40 draws of the data 58 to 61), 63 at 1;
+// 160 rows without limits 24 (the largest, the sums by pieces); 1024 fp16 rows with settings of their own 160 to 170 (one workgroup a CU:
+// four rows one after the other, each idle at its barriers). Where many logits are equal or nearly so a place is looked for among
+// the whole row's tokens: 32 such rows take 213 with top_p 0.9, with equal logits and top_k 400 230.
 // Sums of weights by floating-point atomics in LDS were slower than counts and depend on the order; whole rows in registers need
 // more of them than 16 waves leave.
 #include <algorithm>
@@ -219,7 +222,7 @@ struct Row {
     const unsigned char* mask;
     int vocab, off, pieces;  // 16-byte pieces of memory; the first begins `off` elements before the row
     int rounds;              // pieces of a thread
-    float* largest;          // of each piece, in LDS (null: too many)
+    float* largest;          // of each piece, in LDS (null: some rows of the launch have too many)
 
     // lds: null, or a word for each piece that a row of this length can have wherever it begins (see launch: which of the two is
     // decided there, for all rows alike)
@@ -605,8 +608,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(MzSample a, int shift, 
             for (int attempt = 0; attempt < 4; attempt++) {
                 const int first = block_all(about + off >= goal ? tid : BINS - 1, Min());
                 // With what is in front of it, and some behind, if that is few enough for one wave; otherwise some intervals around it:
-                // 256 tokens on either side (with 128 the place is missed more often: 32 rows at top_p 0.9 take 36 to 47 us by
-                // their data, with 128 up to 58).
+                // 256 tokens on either side (with 128 the place is missed more often, which takes 32 rows from 45 us to 58: 9 times of
+                // 40 at temperature 0.6 and top_p 0.9, 4 with 256; 8 and 3 of 10 at 1 and 0.5).
                 if (tid == first) {
                     sh.before = run - mine;
                     sh.here = run;

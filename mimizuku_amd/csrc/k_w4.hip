@@ -6,6 +6,10 @@
 // Few rows of x are bound by the bytes of the weights, 4 bits and 16 / group each, and below that by the launch; from about 32
 // rows on, by turning codes into fp16 (9 operations for 8 codes) and by reading x from LDS; hundreds of rows of x by the
 // rate at which both feed the matrix cores.
+//
+// Times here are of a call among 40 back to back, fp16 results (logits fp32), the weights each time others of up to 16 that are
+// alike, so that caches hold the small ones only. Both sides of a rule are of one run. A profiler runs launches apart: 1792 x
+// 5120 x 1280 with GELU takes 39 to 40 us there, 35 among others.
 #include <algorithm>
 
 #include "mz_common.h"
@@ -107,7 +111,7 @@ __global__ void __launch_bounds__(256) unpack_kernel(MzW4 w, f16* dst, long ld) 
 // the eight codes of a word, as they are: 1024 + (c + 8) and 1024 + 16 (c + 8) are fp16 numbers whose low bits are c + 8
 struct Codes {
     // (Numbers that the compiler does not know: with those it knows, taking the bits and setting the others are two instructions
-    // instead of one. 1 x 51866 x 1280 takes 10.0 us, 10.8 with two. `known` where the registers for the results do not suffice.)
+    // instead of one. 1 x 51866 x 1280 takes 10.1 us, 11.0 with two. `known` where the registers for the results do not suffice.)
     unsigned one = 0x000F000Fu, sixteen = 0x00F000F0u, magic = 0x64006400u;
     __device__ __forceinline__ explicit Codes(bool known) {
         if (known) return;
@@ -198,8 +202,8 @@ __device__ __forceinline__ void to_lds(const f16* from, u32x4* to) {
 }
 
 // Few rows of weights: a workgroup takes 16 of them, its waves the entries in turn, x from memory (which its caches hold); their
-// sums meet in LDS. 1 x 5120 x 1280 (rows of x, rows of weights, columns): 3.4 us, as long as an empty launch and two
-// dependent reads take; 8 x 1280 x 5120: 5.6 us. Requesting several entries ahead did not help: each wave has two or three.
+// sums meet in LDS. 1 x 5120 x 1280 (rows of x, rows of weights, columns), groups of 64: 4.2 us, of which launch and two
+// dependent reads are most; 8 x 1280 x 5120: 5.8 us. Requesting several entries ahead did not help: each wave has two or three.
 template <int MT, int G>
 __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW4Linear a) {
     constexpr int LD = 68;  // (of 64 results: four rows of x 4 banks apart, so that reading 16 columns of 4 rows meets no conflict)
@@ -238,8 +242,9 @@ __global__ void __launch_bounds__(MT == 4 ? 512 : 1024) split_kernel(MzW4 w, MzW
 }
 
 // Many rows of weights: x lies in LDS, in the order of operands, and each wave takes 16 rows of weights and all of their columns,
-// the next entries on their way. 1 x 51866 x 1280, groups of 32: 10.0 us (3.8 TB/s, of weights that no cache held); 32 rows:
-// 15.9 us, as much for the codes' arithmetic and the reads of LDS as for memory. Three, four and five entries ahead
+// the next entries on their way. 51866 x 1280, groups of 32: 10.1 us for one row (3.7 TB/s, of weights that no cache held), 10.8
+// for 8, 11.1 for 16, 15.7 for 32 (2.8 TB/s), 23.7 for 64: no unit bounds these, x goes into LDS whole before the first product, in
+// the one workgroup that a CU then has room for, and is read again for every 16 rows of weights. Three, four and five entries ahead
 // took 10.9, 11.1 and 11.1 us for the one row when two took 10.8, ten 13.7: more registers, and no wave waits less for its first.
 template <int MT, int G>
 __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
@@ -288,9 +293,10 @@ __global__ void __launch_bounds__(1024) row_kernel(MzW4 w, MzW4Linear a) {
 }
 
 // Many rows of x: a workgroup takes 16 MT WM rows of x times 16 NT WN of weights, WM x WN waves. 128 columns at a time: those of x
-// go straight into LDS, in two buffers, the weights' codes into registers. 1792 x 5120 x 1280, groups of 128: 34.5 us
-// (680 TFLOP/s; a library's product of fp16 weights 27.6), of 64: 41.4, of 32: 44.4; 4096 x 4096 x 4096: 161 us (850). What bounds it is
-// the vector unit next to the matrix cores: codes turned into numbers by every wave row, scales applied group by group.
+// go straight into LDS, in two buffers, the weights' codes into registers. 1792 x 5120 x 1280, groups of 128: 31.6 to 33.6 us
+// (700 to 744 TFLOP/s; a library's product of fp16 weights 27.6), of 64: 37.4, of 32: 40.3; 448 rows 13.8, 14.6 and 16.6; 4096 x
+// 4096 x 4096, groups of 128: 144 us (953). What bounds it is the vector unit next to the matrix cores: codes turned into numbers
+// by every row of waves, scales applied group by group.
 template <int MT, int NT, int WM, int WN, int G>
 __global__ void __launch_bounds__(64 * WM * WN, 2) tile_kernel(MzW4 w, MzW4Linear a) {
     extern __shared__ u32x4 xs[];  // [2][rows][16 pieces of 8 columns, piece p of row r at p ^ r % 16]
@@ -319,8 +325,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) tile_kernel(MzW4 w, MzW4Linea
             scale[u] = scales_at<G>(w.scales + (entry * 16 + i) * G);
         }
     };
-    // The widest tile has hardly enough registers: groups of 64 keep the numbers that the compiler knows (2000 x 4800 x 2560 75 us, 90
-    // otherwise, with registers spilled), the others keep it from mixing the steps (1792 x 5120 x 1280 34.5 us, 42 spilled).
+    // The widest tile has hardly enough registers: groups of 64 keep the numbers that the compiler knows (2000 x 4800 x 2560 69 us,
+    // 81 to 83 otherwise, with registers spilled), the others keep it from mixing the steps (1792 x 5120 x 1280, groups of 128, 31.6
+    // us, 38.7 mixed; groups of 32 take 40.2 either way).
     constexpr bool APART = G != 2;
     const Codes numbers(NT == 5 && !APART);
     f32x4 sum[MT][NT] = {};
@@ -378,12 +385,12 @@ int blocks(long x, long per) { return (int)((x + per - 1) / per); }
 template <int G>
 void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
     const int tiles = blocks(w.n, 16), chunks = w.k / 128, cus = mz_cu_count();
-    // Tiles, where there are enough of 64 x 64 for a quarter of the CUs: 224 x 1280 x 5120 (80 of them) takes 26.8 us, 31.9 by
-    // split_kernel; 128 x 1280 x 5120 (40) 26.9 and 21.0.
+    // Tiles, where there are enough of 64 x 64 for a quarter of the CUs: 224 x 1280 x 5120 (80 of them) takes 24.7 us, 32.0 by
+    // split_kernel; 128 x 1280 x 5120 (40) 24.8 and 21.0.
     if (a.m > 64 && (long)blocks(a.m, 64) * blocks(w.n, 64) >= cus / 4) {
         // Of the widths, eight waves a CU, the one whose last round of workgroups leaves the least idle (16 more columns stand for
-        // the rows of x; 64: several workgroups a CU, which take 1.15 times as long for a result). 1792 x 5120 x 1280: 36.7 us with
-        // 320 (34.8 by now), 53, 43, 40 and 44 with 256, 192, 128 and 64; 448 x 5120 x 1280: 30, 25, 20.9, 16.9 and 16.1.
+        // the rows of x; 64: several workgroups a CU, which take 1.15 times as long for a result). 1792 x 5120 x 1280: 33.6 us with
+        // 320, 47.5, 37.8, 40.3 and 37.7 with 256, 192, 128 and 64; 448 x 5120 x 1280: 27.6, 23.8, 19.3, 14.7 and 13.9.
         int best = 64;
         double least = 1.15 * blocks(a.m, 64) * blocks(w.n, 64) * 64 * 64 / cus + 64 * 64;
         for (int bn : {320, 256, 192, 128}) {
@@ -400,8 +407,8 @@ void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
     }
     int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
     const size_t lds = (size_t)chunks * 4 * mt * 1024;
-    // Four tiles a CU and more: 32 x 51866 x 1280 takes 16.6 us by row_kernel, 40.3 by split_kernel (1 row: 10.9, 14.3);
-    // 32 x 5120 x 1280 (320 tiles) 12.6 and 7.5. x has to fit into LDS.
+    // Four tiles a CU and more: 32 x 51866 x 1280 takes 16.2 us by row_kernel, 43.6 by split_kernel (1 row: 9.8, 13.8);
+    // 32 x 5120 x 1280 (320 tiles) 12.5 and 7.4. x has to fit into LDS.
     if (tiles >= 4 * cus && lds <= 160 * 1024) {
         const int waves = std::min(16, blocks(tiles, (long)cus * blocks(tiles, 16L * cus)));
         const dim3 grid(blocks(tiles, waves), blocks(a.m, 16 * mt)), block(64 * waves);
@@ -410,7 +417,7 @@ void linear_launch(hipStream_t s, const MzW4& w, const MzW4Linear& a) {
         else hipLaunchKernelGGL((row_kernel<4, G>), grid, block, lds, s, w, a);
         return;
     }
-    // Fewer rows of x a workgroup where that leaves CUs without one: 32 x 1280 x 5120 takes 7.6 us with 16 of them, 12.1 with 32.
+    // Fewer rows of x a workgroup where that leaves CUs without one: 32 x 1280 x 5120 takes 7.3 us with 16 of them, 11.7 with 32.
     while (mt > 1 && (long)tiles * blocks(a.m, 16 * mt) < cus) mt /= 2;
     const int most = mt == 4 ? 8 : 16, waves = blocks(chunks, blocks(chunks, most));
     const dim3 grid(tiles, blocks(a.m, 16 * mt)), block(64 * waves);
